@@ -661,6 +661,100 @@ RV_API int rv_attention(const float *q, const uint16_t *k_cache, const uint16_t 
                  size_t n_heads, size_t n_kv_heads, size_t head_dim, float scale, float *scratch,
                  size_t scratch_len, float *out, rv_stream stream);
 
+/* ------------------------------------------- continuations of one prompt */
+/* No counterpart in the reference, which decodes one sequence at a time
+ * (generate/mod.rs).  These entries decode a batch of sequences that share a
+ * prefix -- n continuations of one prompt, or n questions under one long
+ * instruction: their rows go to a KV cache in f16 or 8 bits, the batch attends
+ * with the shared prefix read once for all, and a token is drawn of each row of
+ * logits.  They allocate nothing, do not synchronize and keep nothing between
+ * calls, so a step can be captured into a CUDA graph (the pointers and host
+ * arguments are then fixed; the suffix lengths are read on the device). */
+
+/* Element types of the rows these entries read and write. */
+typedef enum rv_dtype { RV_F32 = 0, RV_F16 = 1, RV_BF16 = 2 } rv_dtype;
+
+/* Cache formats.  RV_KV_F16 holds the values rounded to f16, as the caches of
+ * rv_attn_create.  RV_KV_Q8 holds, for the head_dim values x_i of each (token,
+ * kv head), one f32 scale = max|x| * (1/127) and the int8 levels
+ * rint(x_i * ((1/max|x|) * 127)) (f32 operations, ties to even); the value is
+ * level * scale.  A row with max|x| < 2^-50 is stored as zeros with scale 0; a
+ * row that holds an infinity or a NaN reads back as NaN. */
+typedef enum rv_kv_format { RV_KV_F16 = 0, RV_KV_Q8 = 1 } rv_kv_format;
+
+/* A cache of n_seqs sequences in the caller's device memory (16-byte aligned
+ * planes).  head_dim: a multiple of 8 up to 256.  One layer of an rv_attn
+ * engine is such a cache: n_seqs 1, RV_KV_F16, the pointers of
+ * rv_attn_cache. */
+typedef struct rv_kv_cache {
+  int32_t format;         /* rv_kv_format */
+  uint32_t n_seqs;
+  uint32_t n_kv_heads;
+  uint32_t head_dim;
+  uint64_t capacity;      /* positions per sequence, < 2^31 */
+  void *k, *v;            /* [n_seqs][capacity][n_kv_heads][head_dim] f16 bits / int8 levels */
+  float *k_scale, *v_scale; /* [n_seqs][capacity][n_kv_heads], RV_KV_Q8 only */
+} rv_kv_cache;
+
+/* Writes n_new rows of every sequence: row i of sequence b goes to position
+ * lens[b] - n_new + i (lens: device int32 [n_seqs], the lengths with the new
+ * rows counted; a row before position 0 is skipped) or, without lens, to
+ * position + i.  k, v: device, element (b, i, h, d) at b*seq_stride +
+ * i*token_stride + h*head_dim + d (so both may lie inside the rows of a fused
+ * projection).  A length past the capacity writes nothing for those rows and
+ * sets RV_ERR_CAPACITY_EXCEEDED in the device error word (rv_device_status);
+ * without lens the call returns it. */
+RV_API int rv_kv_append(const rv_kv_cache *cache, int dtype, const void *k, const void *v, size_t seq_stride,
+                        size_t token_stride, size_t n_new, const int32_t *lens, size_t position, rv_stream stream);
+/* Reads rows back as `dtype`, chosen as in rv_kv_append, to k_out / v_out
+ * [n_seqs][n][n_kv_heads][head_dim] (contiguous); a row without a position in
+ * the cache is written as zeros. */
+RV_API int rv_kv_read(const rv_kv_cache *cache, int dtype, size_t n, const int32_t *lens, size_t position,
+                      void *k_out, void *v_out, rv_stream stream);
+
+/* Attention of n_q query tokens of each of n_seqs sequences over a prefix all
+ * of them share and their own suffixes.  prefix: a cache with n_seqs 1, of
+ * which positions 0..prefix_len-1 are attended (NULL with prefix_len 0);
+ * suffix: a cache of n_seqs sequences of the same format and geometry; lens:
+ * device int32 [n_seqs], the suffix lengths with the n_q newest tokens (the
+ * queries' own) counted.  Token i of sequence b sees the whole prefix and
+ * suffix positions 0..lens[b]-n_q+i (none when that is negative); a row that
+ * sees nothing is written as zeros.  q: device, dtype RV_F32 or RV_F16,
+ * element (b, i, h, d) at b*q_seq_stride + i*q_token_stride + h*head_dim + d;
+ * query head h reads kv head h / (n_heads / n_kv_heads); out: device,
+ * [n_seqs][n_q][n_heads][head_dim] contiguous, the same dtype.  scratch:
+ * device, 16-byte aligned, scratch_len bytes of at least
+ * rv_prefix_attention_scratch's result; calls that overlap on the GPU need
+ * scratch of their own.  A length outside [0, capacity] is held inside it and
+ * sets RV_ERR_CAPACITY_EXCEEDED in the device error word. */
+RV_API int rv_prefix_attention(const rv_kv_cache *prefix, size_t prefix_len, const rv_kv_cache *suffix,
+                               const int32_t *lens, int dtype, const void *q, size_t q_seq_stride,
+                               size_t q_token_stride, size_t n_q, size_t n_heads, float scale, void *out,
+                               void *scratch, size_t scratch_len, rv_stream stream);
+/* Bytes of scratch rv_prefix_attention needs for this geometry on the current
+ * device, whatever the lengths. */
+RV_API int rv_prefix_attention_scratch(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                                       size_t *bytes_out);
+
+/* Draws one token of each of n_rows rows of logits (device f32, row r at
+ * r*row_stride, n of them, n < 2^23).  Per row, with l the logits (NaN as
+ * -infinity): z = (l - max l) / temperature, weights exp(z); in descending
+ * order of l, equal values by ascending index, top_k keeps the first k tokens
+ * (k <= 0 or >= n: all), top_p < 1 of those the tokens whose preceding weight
+ * is below top_p of the kept weight (the first always), min_p of those the
+ * ones of weight at least min_p of the largest; of the rest, the first token
+ * in index order whose running weight passes u * (their weight) is drawn.
+ * temperature, top_k (int32), top_p, min_p, u: device arrays of n_rows; every
+ * one but u may be NULL (1, 0, 1, 0).  A temperature of 0 or below takes the
+ * first largest logit.  A row with no logit above -infinity gives token 0.
+ * tokens: int32 [n_rows]; logprobs: [n_rows] or NULL, the natural logarithm of
+ * the drawn token's share of the weight it was drawn from (0 at temperature 0,
+ * -infinity for a row with nothing to draw).  The weights are integers of
+ * 2^-40 of the largest, so the result does not depend on the order of sums. */
+RV_API int rv_sample(const float *logits, size_t row_stride, size_t n_rows, size_t n, const float *u,
+                     const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                     int32_t *tokens, float *logprobs, rv_stream stream);
+
 /* Seeded N(0, sigma^2)-like values: element i is the Irwin-Hall sum of
  * twelve 24-bit uniforms drawn from SplitMix64(seed, offset + i), so the
  * same (seed, offset) gives the same floats on every device and host.

@@ -20,6 +20,11 @@ stream.  Names and error kinds follow the reference:
 - ``rvmp.load_expert_table`` (install files) format/layout.rs, io/expert.rs
 - ``MoeEngine.forward`` (the MoE block)      model/forward.rs:2654-2754,
                                              model/prefill.rs:2136-2263
+
+Without a counterpart in the reference, which decodes one sequence: a batch of
+continuations of one prompt -- ``KvCache`` / ``kv_append`` / ``kv_read`` (f16
+or 8-bit rows), ``prefix_attention`` (the shared prefix is read once for the
+batch) and ``sample``.
 """
 from __future__ import annotations
 
@@ -43,7 +48,8 @@ __all__ = [
     "quantize_weights", "EXACT", "TENSOR", "lib", "Q8_0_BYTES", "quantize_row_q8_0", "gemv_q8_0",
     "gemv_q8_0_rows", "gemv_q8_0_batched", "dequantize_rows", "embed", "device_status",
     "rope_neox_heads", "attention", "AttnEngine", "attn_weights", "rmsnorm_quantize", "ExpertParallel",
-    "EP_HANDLE_BYTES", "wait_probe",
+    "EP_HANDLE_BYTES", "wait_probe", "KvCache", "KV_F16", "KV_Q8", "kv_append", "kv_read", "prefix_attention",
+    "prefix_attention_scratch", "sample",
 ]
 
 Q8K_BYTES = 292
@@ -722,6 +728,184 @@ def rmsnorm_quantize(x: torch.Tensor, w: torch.Tensor, eps: float, q8k_out: torc
     """rmsnorm fused with quantize_row_q8_k (and quantize_row_q8_0)."""
     _check(lib().rv_rmsnorm_quantize(_p(x), _p(w), x.numel(), eps, _p(q8k_out), _p(q80_out), _stream()))
     return q8k_out
+
+
+# ------------------------------------------- continuations of one prompt
+KV_F16, KV_Q8 = 0, 1  # rv_kv_format
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # rv_dtype
+
+
+def _dtype(t: torch.Tensor) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise KernelError(9, f"UnsupportedFormat: rows of {t.dtype}")
+    return code
+
+
+def _i32(t: Optional[torch.Tensor], n: int, what: str):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise KernelError(5, f"LengthMismatch: {what} must be {n} contiguous int32 values")
+    return t.data_ptr()
+
+
+def _f32(t: Optional[torch.Tensor], n: int, what: str):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise KernelError(5, f"LengthMismatch: {what} must be {n} contiguous float32 values")
+    return t.data_ptr()
+
+
+class KvCache:
+    """A KV cache of n_seqs sequences on one device: f16 rows (``KV_F16``) or
+    int8 levels with one f32 scale per (token, kv head) (``KV_Q8``).  ``k`` and
+    ``v`` are [n_seqs, capacity, n_kv_heads, head_dim], ``k_scale`` and
+    ``v_scale`` [n_seqs, capacity, n_kv_heads] (``None`` for f16)."""
+
+    def __init__(self, n_seqs: int, capacity: int, n_kv_heads: int = 4, head_dim: int = 128, format: int = KV_F16,
+                 device: int = 0):
+        shape, d = (n_seqs, capacity, n_kv_heads, head_dim), f"cuda:{device}"
+        q8 = format == KV_Q8
+        k, v = (torch.zeros(shape, dtype=torch.int8 if q8 else torch.float16, device=d) for _ in range(2))
+        ks, vs = (torch.zeros(shape[:3], dtype=torch.float32, device=d) if q8 else None for _ in range(2))
+        self._hold(k, v, ks, vs)
+
+    @classmethod
+    def of(cls, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+           v_scale: Optional[torch.Tensor] = None) -> "KvCache":
+        """A cache over existing tensors (not copied; held by the cache)."""
+        c = cls.__new__(cls)
+        c._hold(k, v, k_scale, v_scale)
+        return c
+
+    @classmethod
+    def of_engine(cls, engine: "AttnEngine", layer: int) -> "KvCache":
+        """The f16 cache of one layer of an ``AttnEngine`` (not copied; the
+        engine is kept alive), as a cache of one sequence."""
+        c = cls.__new__(cls)
+        cfg, (k, v) = engine.cfg, engine.cache(layer)
+        c.k = c.v = c.k_scale = c.v_scale = None
+        c.engine, c.format = engine, KV_F16
+        c.n_seqs, c.capacity, c.n_kv_heads, c.head_dim = 1, cfg.max_positions, cfg.n_kv_heads, cfg.head_dim
+        c._c = _lib.KvCacheC(KV_F16, 1, cfg.n_kv_heads, cfg.head_dim, cfg.max_positions, k, v, None, None)
+        c._ref = ctypes.addressof(c._c)
+        c.device = torch.device(f"cuda:{engine.device}")
+        return c
+
+    def _hold(self, k, v, ks, vs):
+        q8 = k.dtype == torch.int8
+        if k.dtype not in (torch.int8, torch.float16) or v.dtype != k.dtype:
+            raise KernelError(9, f"UnsupportedFormat: a cache of {k.dtype} keys and {v.dtype} values")
+        if k.dim() != 4 or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous():
+            raise KernelError(5, "LengthMismatch: k and v must be contiguous [n_seqs, capacity, n_kv_heads, head_dim]")
+        for t in (ks, vs):
+            if q8 and (t is None or t.dtype != torch.float32 or t.shape != k.shape[:3] or not t.is_contiguous()):
+                raise KernelError(5, "LengthMismatch: scales must be contiguous float32 [n_seqs, capacity, n_kv_heads]")
+        if not q8 and (ks is not None or vs is not None):
+            raise KernelError(9, "UnsupportedFormat: an f16 cache has no scales")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, ks, vs
+        self.n_seqs, self.capacity, self.n_kv_heads, self.head_dim = k.shape
+        self.format, self.device = (KV_Q8 if q8 else KV_F16), k.device
+        self._c = _lib.KvCacheC(self.format, *(self.n_seqs, self.n_kv_heads, self.head_dim), self.capacity, _p(k),
+                                _p(v), _p(ks), _p(vs))
+        self._ref = ctypes.addressof(self._c)
+
+
+def _rows_of(cache: KvCache, x: torch.Tensor):
+    """(seq stride, token stride, tokens) of rows [n_seqs, n, n_kv_heads, head_dim]."""
+    if x.dim() != 4 or (x.shape[0], x.shape[2], x.shape[3]) != (cache.n_seqs, cache.n_kv_heads, cache.head_dim):
+        raise KernelError(5, f"LengthMismatch: rows {tuple(x.shape)} for a cache of {cache.n_seqs} sequences, "
+                             f"{cache.n_kv_heads} kv heads of {cache.head_dim}")
+    s = x.stride()
+    if s[3] != 1 or (s[2] != cache.head_dim and cache.n_kv_heads > 1):
+        raise KernelError(5, "LengthMismatch: the heads of a token must be contiguous")
+    return s[0], s[1], x.shape[1]
+
+
+def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[torch.Tensor] = None,
+              position: int = 0) -> None:
+    """Write rows k, v [n_seqs, n, n_kv_heads, head_dim] (f32, f16 or bf16; any
+    token and sequence strides, the same for both) as the last n positions of
+    sequences of `lens` tokens (int32 [n_seqs], on the device, the new rows
+    counted), or from `position` on."""
+    seq, token, n = _rows_of(cache, k)
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+        raise KernelError(5, "LengthMismatch: k and v must be alike in shape, strides and type")
+    _check(lib().rv_kv_append(cache._ref, _dtype(k), k.data_ptr(), v.data_ptr(), seq, token, n,
+                              _i32(lens, cache.n_seqs, "lens"), position, _stream()))
+
+
+def kv_read(cache: KvCache, n: int, lens: Optional[torch.Tensor] = None, position: int = 0,
+            dtype: torch.dtype = torch.float32):
+    """(k, v) of n positions of every sequence, [n_seqs, n, n_kv_heads,
+    head_dim] of `dtype`, chosen as in ``kv_append``."""
+    k = torch.empty((cache.n_seqs, n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    _check(lib().rv_kv_read(cache._ref, _dtype(k), n, _i32(lens, cache.n_seqs, "lens"), position, k.data_ptr(),
+                            v.data_ptr(), _stream()))
+    return k, v
+
+
+def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int, suffix: KvCache, lens: torch.Tensor,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [n_seqs, n_q, n_heads, head_dim] (f32 or f16, heads
+    contiguous) over positions 0..prefix_len-1 of `prefix`, shared by all
+    sequences, and each sequence's own `lens` suffix positions (int32, on the
+    device; the n_q query tokens are the newest of them and see no later one).
+    scale defaults to head_dim ** -0.5; scratch: a uint8 tensor of at least
+    ``prefix_attention_scratch`` bytes."""
+    if q.dim() != 4 or q.shape[0] != suffix.n_seqs or q.shape[3] != suffix.head_dim:
+        raise KernelError(5, f"LengthMismatch: queries {tuple(q.shape)} for a suffix of {suffix.n_seqs} sequences, "
+                             f"head_dim {suffix.head_dim}")
+    n, n_q, H, D = q.shape
+    s = q.stride()
+    if s[3] != 1 or (s[2] != D and H > 1):
+        raise KernelError(5, "LengthMismatch: the heads of a query token must be contiguous")
+    if out is None:
+        out = torch.empty((n, n_q, H, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise KernelError(5, "LengthMismatch: out must be contiguous and like q in shape and type")
+    if scratch is None:
+        scratch = torch.empty(prefix_attention_scratch(n, n_q, H, suffix.n_kv_heads, D), dtype=torch.uint8,
+                              device=q.device)
+    _check(lib().rv_prefix_attention(prefix._ref if prefix is not None else None, prefix_len, suffix._ref,
+                                     _i32(lens, n, "lens"), _dtype(q), q.data_ptr(), s[0], s[1], n_q, H,
+                                     D ** -0.5 if scale is None else scale, out.data_ptr(), scratch.data_ptr(),
+                                     _nbytes(scratch), _stream()))
+    return out
+
+
+def prefix_attention_scratch(n_seqs: int, n_q: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    """Bytes of scratch ``prefix_attention`` needs on the current device."""
+    n = ctypes.c_size_t()
+    _check(lib().rv_prefix_attention_scratch(n_seqs, n_q, n_heads, n_kv_heads, head_dim, ctypes.byref(n)))
+    return n.value
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None,
+           logprobs: Optional[torch.Tensor] = None):
+    """Draw one token of each row of logits [n_rows, n] (f32, rows contiguous)
+    with the uniforms u [n_rows] in [0, 1): (tokens int32, logprobs f32).  The
+    filters are per-row device arrays (top_k int32); ``None`` switches one off."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError(5, "LengthMismatch: logits must be float32 [n_rows, n] with contiguous rows")
+    rows, n = logits.shape
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    if logprobs is None:
+        logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    if u is None:
+        raise KernelError(13, "InvalidArgument: u is required")
+    _check(lib().rv_sample(logits.data_ptr(), logits.stride(0), rows, n, _f32(u, rows, "u"),
+                           _f32(temperature, rows, "temperature"), _i32(top_k, rows, "top_k"),
+                           _f32(top_p, rows, "top_p"), _f32(min_p, rows, "min_p"), _i32(tokens, rows, "tokens"),
+                           _f32(logprobs, rows, "logprobs"), _stream()))
+    return tokens, logprobs
 
 
 def device_status(device: int = 0) -> None:

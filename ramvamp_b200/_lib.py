@@ -88,6 +88,11 @@ class MoeTaps(ctypes.Structure):
                 ("acts_moe_stride", SZ), ("staged", P), ("logit_bounds", P)]
 
 
+class KvCacheC(ctypes.Structure):
+    _fields_ = [("format", ctypes.c_int32), ("n_seqs", U32), ("n_kv_heads", U32), ("head_dim", U32),
+                ("capacity", U64), ("k", P), ("v", P), ("k_scale", P), ("v_scale", P)]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
     "rv_version": (ctypes.c_char_p, []),
@@ -161,6 +166,11 @@ SIGNATURES = {
     "rv_moe_profile_rewind": (I32, [P]),
     "rv_moe_profile_read": (I32, [P, P, SZ, ctypes.POINTER(SZ)]),
     "rv_moe_forward_static": (I32, [ctypes.POINTER(MoeConfig), ctypes.POINTER(LayerLayout), P, P, P, P, SZ, P, P, P]),
+    "rv_kv_append": (I32, [P, I32, P, P, SZ, SZ, SZ, P, SZ, P]),
+    "rv_kv_read": (I32, [P, I32, SZ, P, SZ, P, P, P]),
+    "rv_prefix_attention": (I32, [P, SZ, P, P, I32, P, SZ, SZ, SZ, SZ, F32, P, P, SZ, P]),
+    "rv_prefix_attention_scratch": (I32, [SZ, SZ, SZ, SZ, SZ, ctypes.POINTER(SZ)]),
+    "rv_sample": (I32, [P, SZ, SZ, SZ, P, P, P, P, P, P, P, P]),
     "rv_synth_normal": (I32, [U64, U64, F32, P, SZ, P]),
     "rv_quantize_weights": (I32, [I32, P, SZ, P, P]),
     "rv_expert_table_fill_synthetic": (I32, [P, U32, U64, F32, P]),

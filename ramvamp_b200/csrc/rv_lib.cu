@@ -21,6 +21,9 @@
 #include "rv_tc.cuh"
 #include "rv_ep.cuh"
 #include "rv_attn.cuh"
+#include "rv_kv.cuh"
+#include "rv_prefix.cuh"
+#include "rv_sample.cuh"
 
 #include "_gen/expf_exceptions.inc"
 
@@ -2621,5 +2624,236 @@ extern "C" int rv_moe_forward_static(const rv_moe_config *cfg, const rv_layer_la
   RV_LAUNCH_CHECK();
   if (topk_ids) RV_CUDA(cudaMemcpyAsync(topk_ids, B.ids, n_tokens * d.K * 4, cudaMemcpyDeviceToDevice, s));
   if (topk_weights) RV_CUDA(cudaMemcpyAsync(topk_weights, B.w, n_tokens * d.K * 4, cudaMemcpyDeviceToDevice, s));
+  return RV_OK;
+}
+
+// ============================================ continuations of one prompt
+static size_t dtype_bytes(int dtype) { return dtype == RV_F32 ? 4 : dtype == RV_F16 || dtype == RV_BF16 ? 2 : 0; }
+
+static int check_kv_cache(const char *what, const rv_kv_cache *c) {
+  if (!c) RV_FAIL(RV_ERR_INVALID_ARGUMENT, "%s: null cache", what);
+  if (c->format != RV_KV_F16 && c->format != RV_KV_Q8)
+    RV_FAIL(RV_ERR_UNSUPPORTED_FORMAT, "%s: cache format %d", what, c->format);
+  if (c->n_seqs == 0 || c->n_kv_heads == 0) RV_FAIL(RV_ERR_EMPTY, "%s: a cache of no sequences or heads", what);
+  if (c->head_dim == 0 || c->head_dim % 2) RV_FAIL(RV_ERR_INVALID_HEAD_DIM, "%s: head_dim %u", what, c->head_dim);
+  if (c->head_dim % 8 || c->head_dim > 256)
+    RV_FAIL(RV_ERR_UNIMPLEMENTED, "%s: head_dim %u (multiples of 8 up to 256)", what, c->head_dim);
+  if (c->n_seqs > 65535 || c->n_kv_heads > 65535 || c->capacity >= (1ull << 31))
+    RV_FAIL(RV_ERR_UNIMPLEMENTED, "%s: %u sequences (<= 65535), %u kv heads (<= 65535), capacity %llu (< 2^31)", what,
+            c->n_seqs, c->n_kv_heads, (unsigned long long)c->capacity);
+  return RV_OK;
+}
+static int check_kv_planes(const char *what, const rv_kv_cache *c) {
+  if (!c->k || !c->v || (((uintptr_t)c->k | (uintptr_t)c->v) & 15))
+    RV_FAIL(RV_ERR_INVALID_ARGUMENT, "%s: null cache plane or one not 16-byte aligned", what);
+  if (c->format == RV_KV_Q8 &&
+      (!c->k_scale || !c->v_scale || (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3)))
+    RV_FAIL(RV_ERR_INVALID_ARGUMENT, "%s: an 8-bit cache without scales", what);
+  return RV_OK;
+}
+
+// What rv_kv_append and rv_kv_read share: the checks and the arguments.
+static int kv_rows_args(const char *what, const rv_kv_cache *c, int dtype, const void *k, const void *v,
+                        size_t seq_stride, size_t token_stride, size_t n, const int32_t *lens, size_t position,
+                        KvArgs *a, dim3 *grid) {
+  int rc = check_kv_cache(what, c);
+  if (rc) return rc;
+  const size_t eb = dtype_bytes(dtype);
+  if (eb == 0) RV_FAIL(RV_ERR_UNSUPPORTED_FORMAT, "%s: dtype %d", what, dtype);
+  if (n > c->capacity || (!lens && position > c->capacity - n))
+    RV_FAIL(RV_ERR_CAPACITY_EXCEEDED, "%s: %zu rows from position %zu in a cache of %llu", what, n, position,
+            (unsigned long long)c->capacity);
+  if (n == 0) return RV_OK;
+  if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & (eb - 1)) || ((uintptr_t)lens & 3))
+    RV_FAIL(RV_ERR_INVALID_ARGUMENT, "%s: null or misaligned pointer", what);
+  if (token_stride < (size_t)c->n_kv_heads * c->head_dim && n > 1)
+    RV_FAIL(RV_ERR_LENGTH_MISMATCH, "%s: token stride %zu below a token's %u x %u values", what, token_stride,
+            c->n_kv_heads, c->head_dim);
+  rc = check_kv_planes(what, c);
+  if (rc) return rc;
+  *a = KvArgs{};
+  a->k = c->k;
+  a->v = c->v;
+  a->k_scale = c->k_scale;
+  a->v_scale = c->v_scale;
+  a->k_io = const_cast<void *>(k);
+  a->v_io = const_cast<void *>(v);
+  a->lens = lens;
+  a->seq_stride = seq_stride;
+  a->token_stride = token_stride;
+  a->position = position;
+  a->capacity = c->capacity;
+  a->n = (uint32_t)n;
+  a->n_kv = c->n_kv_heads;
+  a->hd = c->head_dim;
+  a->lanes = 1;
+  while (a->lanes * 8 < c->head_dim) a->lanes *= 2;
+  a->aligned = ((((uintptr_t)k | (uintptr_t)v) | token_stride * eb | seq_stride * eb) & 15) == 0;
+  const size_t per = RV_KV_THREADS / a->lanes, rows = n * c->n_kv_heads;
+  if (rows > 0xFFFFFFFFull - per) RV_FAIL(RV_ERR_UNIMPLEMENTED, "%s: %zu rows of one sequence", what, rows);
+  *grid = dim3((unsigned)((rows + per - 1) / per), c->n_seqs, 2);
+  return ensure_current_device();
+}
+
+template <typename T>
+static void kv_append_launch(const KvArgs &a, bool q8, dim3 grid, cudaStream_t s) {
+  if (q8) k_kv_append<T, true><<<grid, RV_KV_THREADS, 0, s>>>(a);
+  else k_kv_append<T, false><<<grid, RV_KV_THREADS, 0, s>>>(a);
+}
+template <typename T>
+static void kv_read_launch(const KvArgs &a, bool q8, dim3 grid, cudaStream_t s) {
+  if (q8) k_kv_read<T, true><<<grid, RV_KV_THREADS, 0, s>>>(a);
+  else k_kv_read<T, false><<<grid, RV_KV_THREADS, 0, s>>>(a);
+}
+
+extern "C" int rv_kv_append(const rv_kv_cache *c, int dtype, const void *k, const void *v, size_t seq_stride,
+                            size_t token_stride, size_t n_new, const int32_t *lens, size_t position,
+                            rv_stream stream) {
+  KvArgs a;
+  dim3 grid;
+  const int rc = kv_rows_args("kv_append", c, dtype, k, v, seq_stride, token_stride, n_new, lens, position, &a, &grid);
+  if (rc || n_new == 0) return rc;
+  const bool q8 = c->format == RV_KV_Q8;
+  if (dtype == RV_F32) kv_append_launch<float>(a, q8, grid, (cudaStream_t)stream);
+  else if (dtype == RV_F16) kv_append_launch<__half>(a, q8, grid, (cudaStream_t)stream);
+  else kv_append_launch<__nv_bfloat16>(a, q8, grid, (cudaStream_t)stream);
+  RV_LAUNCH_CHECK();
+  return RV_OK;
+}
+
+extern "C" int rv_kv_read(const rv_kv_cache *c, int dtype, size_t n, const int32_t *lens, size_t position, void *k_out,
+                          void *v_out, rv_stream stream) {
+  KvArgs a;
+  dim3 grid;
+  const size_t token = c ? (size_t)c->n_kv_heads * c->head_dim : 0;
+  const int rc = kv_rows_args("kv_read", c, dtype, k_out, v_out, sat_mul(n, token), token, n, lens, position, &a, &grid);
+  if (rc || n == 0) return rc;
+  const bool q8 = c->format == RV_KV_Q8;
+  if (dtype == RV_F32) kv_read_launch<float>(a, q8, grid, (cudaStream_t)stream);
+  else if (dtype == RV_F16) kv_read_launch<__half>(a, q8, grid, (cudaStream_t)stream);
+  else kv_read_launch<__nv_bfloat16>(a, q8, grid, (cudaStream_t)stream);
+  RV_LAUNCH_CHECK();
+  return RV_OK;
+}
+
+extern "C" int rv_prefix_attention_scratch(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv_heads,
+                                           size_t head_dim, size_t *bytes_out) {
+  if (!bytes_out) RV_FAIL(RV_ERR_INVALID_ARGUMENT, "prefix_attention_scratch: null pointer");
+  if (n_heads == 0 || n_kv_heads == 0) RV_FAIL(RV_ERR_EMPTY, "prefix_attention_scratch: no heads");
+  if (n_heads % n_kv_heads)
+    RV_FAIL(RV_ERR_LENGTH_MISMATCH, "prefix_attention_scratch: %zu query heads over %zu kv heads", n_heads, n_kv_heads);
+  (void)n_seqs;
+  (void)n_q;
+  (void)head_dim;
+  *bytes_out = 16;
+  return RV_OK;
+}
+
+extern "C" int rv_prefix_attention(const rv_kv_cache *prefix, size_t prefix_len, const rv_kv_cache *suffix,
+                                   const int32_t *lens, int dtype, const void *q, size_t q_seq_stride,
+                                   size_t q_token_stride, size_t n_q, size_t n_heads, float scale, void *out,
+                                   void *scratch, size_t scratch_len, rv_stream stream) {
+  int rc = check_kv_cache("prefix_attention", suffix);
+  if (rc) return rc;
+  if (prefix_len) {
+    rc = check_kv_cache("prefix_attention", prefix);
+    if (rc) return rc;
+    if (prefix->format != suffix->format)
+      RV_FAIL(RV_ERR_UNSUPPORTED_FORMAT, "prefix_attention: prefix format %d, suffix format %d", prefix->format,
+              suffix->format);
+    if (prefix->n_seqs != 1 || prefix->n_kv_heads != suffix->n_kv_heads || prefix->head_dim != suffix->head_dim)
+      RV_FAIL(RV_ERR_LENGTH_MISMATCH,
+              "prefix_attention: a prefix of %u sequences, %u kv heads of %u against a suffix of %u kv heads of %u",
+              prefix->n_seqs, prefix->n_kv_heads, prefix->head_dim, suffix->n_kv_heads, suffix->head_dim);
+    if (prefix_len > prefix->capacity)
+      RV_FAIL(RV_ERR_CAPACITY_EXCEEDED, "prefix_attention: prefix_len %zu of a cache of %llu", prefix_len,
+              (unsigned long long)prefix->capacity);
+  }
+  if (dtype != RV_F32 && dtype != RV_F16) RV_FAIL(RV_ERR_UNSUPPORTED_FORMAT, "prefix_attention: dtype %d", dtype);
+  if (n_q == 0) return RV_OK;
+  if (n_heads == 0) RV_FAIL(RV_ERR_EMPTY, "prefix_attention: no query heads");
+  if (n_heads % suffix->n_kv_heads)
+    RV_FAIL(RV_ERR_LENGTH_MISMATCH, "prefix_attention: %zu query heads over %u kv heads", n_heads, suffix->n_kv_heads);
+  if (n_q > 65535 || n_heads > 65535)
+    RV_FAIL(RV_ERR_UNIMPLEMENTED, "prefix_attention: %zu query tokens, %zu heads (<= 65535)", n_q, n_heads);
+  size_t need = 0;
+  rc = rv_prefix_attention_scratch(suffix->n_seqs, n_q, n_heads, suffix->n_kv_heads, suffix->head_dim, &need);
+  if (rc) return rc;
+  if (scratch_len < need)
+    RV_FAIL(RV_ERR_LENGTH_MISMATCH, "prefix_attention: scratch of %zu bytes, needs %zu", scratch_len, need);
+  const size_t eb = dtype_bytes(dtype);
+  if (!q || !out || !lens || !scratch || (((uintptr_t)q | (uintptr_t)out) & (eb - 1)) || ((uintptr_t)lens & 3) ||
+      ((uintptr_t)scratch & 15))
+    RV_FAIL(RV_ERR_INVALID_ARGUMENT, "prefix_attention: null or misaligned pointer");
+  rc = check_kv_planes("prefix_attention", suffix);
+  if (rc == RV_OK && prefix_len) rc = check_kv_planes("prefix_attention", prefix);
+  if (rc) return rc;
+  rc = ensure_current_device();
+  if (rc) return rc;
+  PrefixArgs a{};
+  a.q = q;
+  a.out = out;
+  if (prefix_len) {
+    a.pk = prefix->k;
+    a.pv = prefix->v;
+    a.pks = prefix->k_scale;
+    a.pvs = prefix->v_scale;
+  }
+  a.sk = suffix->k;
+  a.sv = suffix->v;
+  a.sks = suffix->k_scale;
+  a.svs = suffix->v_scale;
+  a.lens = lens;
+  a.q_seq_stride = q_seq_stride;
+  a.q_token_stride = q_token_stride;
+  a.prefix_len = (uint32_t)prefix_len;
+  a.cap = (uint32_t)suffix->capacity;
+  a.n_seqs = suffix->n_seqs;
+  a.n_q = (uint32_t)n_q;
+  a.n_heads = (uint32_t)n_heads;
+  a.n_kv = suffix->n_kv_heads;
+  a.hd = suffix->head_dim;
+  a.scale_log2 = scale * RV_LOG2E;
+  const bool q8 = suffix->format == RV_KV_Q8;
+  const dim3 grid((unsigned)n_heads, (unsigned)n_q, suffix->n_seqs);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dtype == RV_F32) {
+    if (q8) k_prefix_any<float, true><<<grid, 256, 0, s>>>(a);
+    else k_prefix_any<float, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    if (q8) k_prefix_any<__half, true><<<grid, 256, 0, s>>>(a);
+    else k_prefix_any<__half, false><<<grid, 256, 0, s>>>(a);
+  }
+  RV_LAUNCH_CHECK();
+  return RV_OK;
+}
+
+extern "C" int rv_sample(const float *logits, size_t row_stride, size_t n_rows, size_t n, const float *u,
+                         const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                         int32_t *tokens, float *logprobs, rv_stream stream) {
+  if (n_rows == 0) return RV_OK;
+  if (n == 0) RV_FAIL(RV_ERR_EMPTY, "sample: no logits");
+  if (n >= (1u << 23)) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu logits a row (< 2^23)", n);
+  if (n_rows > 0x7FFFFFFFull) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu rows (< 2^31)", n_rows);
+  if (row_stride < n && n_rows > 1) RV_FAIL(RV_ERR_LENGTH_MISMATCH, "sample: row stride %zu below %zu logits", row_stride, n);
+  if (!logits || !u || !tokens ||
+      (((uintptr_t)logits | (uintptr_t)u | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p |
+        (uintptr_t)min_p | (uintptr_t)tokens | (uintptr_t)logprobs) & 3))
+    RV_FAIL(RV_ERR_INVALID_ARGUMENT, "sample: null or misaligned pointer");
+  const int rc = ensure_current_device();
+  if (rc) return rc;
+  SampleArgs a{};
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.n = (uint32_t)n;
+  a.u = u;
+  a.temperature = temperature;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.top_k = top_k;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  k_sample<<<(unsigned)n_rows, RV_SAMPLE_THREADS, 0, (cudaStream_t)stream>>>(a);
+  RV_LAUNCH_CHECK();
   return RV_OK;
 }
