@@ -117,6 +117,15 @@ static int g_dev_sms[64];  // multiprocessor count, read at set-up
 
 #define RV_SMEM_PER_CTA (227u * 1024u)  // the per-CTA shared-memory limit of sm_100
 
+template <int D>
+static void prefix_tc_smem() {
+  const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaFuncSetAttribute(k_prefix_tc<D, float, false>, attr, (int)PfxCfg<D, float, false>::total);
+  cudaFuncSetAttribute(k_prefix_tc<D, float, true>, attr, (int)PfxCfg<D, float, true>::total);
+  cudaFuncSetAttribute(k_prefix_tc<D, __half, false>, attr, (int)PfxCfg<D, __half, false>::total);
+  cudaFuncSetAttribute(k_prefix_tc<D, __half, true>, attr, (int)PfxCfg<D, __half, true>::total);
+}
+
 static int ensure_device(int dev) {
   if (dev < 0 || dev >= 64) RV_FAIL(RV_ERR_INVALID_ARGUMENT, "device %d out of range", dev);
   std::lock_guard<std::mutex> lk(g_init_mu);
@@ -163,6 +172,8 @@ static int ensure_device(int dev) {
   cudaFuncSetAttribute(k_route_spec<RV_GEO_QWEN3>, cudaFuncAttributeMaxDynamicSharedMemorySize, big);
 
   cudaFuncSetAttribute(k_router_logits, cudaFuncAttributeMaxDynamicSharedMemorySize, big);
+  prefix_tc_smem<64>();
+  prefix_tc_smem<128>();
   cudaError_t e3 = cudaGetLastError();
   cudaSetDevice(prev);
   if (e1 != cudaSuccess || e2 != cudaSuccess || e3 != cudaSuccess)
@@ -2736,17 +2747,109 @@ extern "C" int rv_kv_read(const rv_kv_cache *c, int dtype, size_t n, const int32
   return RV_OK;
 }
 
+// Work shape and scratch sections of a tensor-core call (offsets in bytes;
+// *end is the size).  sr: rows of a segment.
+struct PfxScratch {
+  size_t cum, ml_p, ml_s, o_p, o_s, end;
+};
+static bool prefix_tc_dim(size_t head_dim) { return head_dim == 64 || head_dim == 128; }
+static PfxScratch prefix_scratch(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv, size_t hd, size_t sr) {
+  const size_t rows_s = n_q * (n_heads / n_kv), rows_p = rows_s * n_seqs, rw_s = std::min<size_t>(RV_PFX_M, rows_s);
+  // A part for every piece: the cut points are at most one per CTA, and a
+  // segment has one piece more than cuts.  Two streams a piece.
+  const size_t parts_p = 2 * (n_kv * ((rows_p + sr - 1) / sr) + RV_PFX_CTAS);
+  const size_t parts_s = 2 * (n_seqs * n_kv * ((rows_s + sr - 1) / sr) + RV_PFX_CTAS);
+  const auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  PfxScratch o;
+  o.cum = 0;
+  o.ml_p = up((n_seqs + 1) * sizeof(int));
+  o.ml_s = o.ml_p + up(parts_p * RV_PFX_M * sizeof(float2));
+  o.o_p = o.ml_s + up(parts_s * rw_s * sizeof(float2));
+  o.o_s = o.o_p + up(parts_p * RV_PFX_M * hd * sizeof(float));
+  o.end = o.o_s + up(parts_s * rw_s * hd * sizeof(float));
+  return o;
+}
+
 extern "C" int rv_prefix_attention_scratch(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv_heads,
                                            size_t head_dim, size_t *bytes_out) {
   if (!bytes_out) RV_FAIL(RV_ERR_INVALID_ARGUMENT, "prefix_attention_scratch: null pointer");
   if (n_heads == 0 || n_kv_heads == 0) RV_FAIL(RV_ERR_EMPTY, "prefix_attention_scratch: no heads");
   if (n_heads % n_kv_heads)
     RV_FAIL(RV_ERR_LENGTH_MISMATCH, "prefix_attention_scratch: %zu query heads over %zu kv heads", n_heads, n_kv_heads);
-  (void)n_seqs;
-  (void)n_q;
-  (void)head_dim;
-  *bytes_out = 16;
+  if (sat_mul(sat_mul(n_seqs, n_q), n_heads) > (1u << 30))
+    RV_FAIL(RV_ERR_UNIMPLEMENTED, "prefix_attention: %zu x %zu x %zu query rows (<= 2^30)", n_seqs, n_q, n_heads);
+  // Segments of 128 rows (f32 queries) need the most parts.
+  *bytes_out = prefix_tc_dim(head_dim)
+                   ? prefix_scratch(n_seqs, n_q, n_heads, n_kv_heads, head_dim, RV_PFX_M).end
+                   : 16;
   return RV_OK;
+}
+
+// Tensor map over a cache plane of f16 rows [seqs][positions][n_kv][hd]; box =
+// 64 values of 128 positions of one head, 128-byte swizzle.  Positions past
+// `positions` read as zeros.
+static int kv_plane_map(const void *plane, size_t seqs, size_t positions, size_t seq_positions, size_t n_kv, size_t hd,
+                        CUtensorMap *map) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
+  const int rc = tmap_encoder(&enc);
+  if (rc) return rc;
+  const cuuint64_t dims[4] = {hd, n_kv, positions, seqs};
+  const cuuint64_t strides[3] = {hd * 2, n_kv * hd * 2, seq_positions * n_kv * hd * 2};
+  const cuuint32_t box[4] = {64, 1, RV_PFX_N, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(plane), dims, strides, box, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) RV_FAIL(RV_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return RV_OK;
+}
+
+template <int D, typename T, bool Q8>
+static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t s) {
+  using C = PfxCfg<D, T, Q8>;
+  PfxWork w{};
+  const size_t G = a.n_heads / a.n_kv;
+  w.tp = (int)((a.prefix_len + RV_PFX_N - 1) / RV_PFX_N);
+  w.rows_s = (int)(a.n_q * G);
+  w.rows_p = (int)(a.n_seqs * a.n_q * G);
+  w.rw_s = std::min(RV_PFX_M, w.rows_s);
+  w.sr = C::PRECISE ? RV_PFX_M : 2 * RV_PFX_M;
+  w.nrt_p = (w.rows_p + w.sr - 1) / w.sr;
+  w.nrt_s = (w.rows_s + w.sr - 1) / w.sr;
+  int dev = 0;
+  RV_CUDA(cudaGetDevice(&dev));
+  const size_t sms = g_dev_sms[dev] > 0 ? (size_t)g_dev_sms[dev] : RV_PFX_CTAS;
+  // No more CTAs than units at the suffixes' greatest lengths.
+  const size_t most = (size_t)a.n_kv * w.nrt_p * w.tp +
+                      (size_t)a.n_kv * w.nrt_s * a.n_seqs * (((size_t)a.cap + RV_PFX_N - 1) / RV_PFX_N);
+  w.grid = (int)std::max<size_t>(1, std::min(std::min<size_t>(sms, RV_PFX_CTAS), most));
+  const PfxScratch o = prefix_scratch(a.n_seqs, a.n_q, a.n_heads, a.n_kv, D, (size_t)w.sr);
+  w.cum = (int *)(scratch + o.cum);
+  w.ml_p = (float2 *)(scratch + o.ml_p);
+  w.ml_s = (float2 *)(scratch + o.ml_s);
+  w.o_p = (float4 *)(scratch + o.o_p);
+  w.o_s = (float4 *)(scratch + o.o_s);
+  const size_t eb = sizeof(T);
+  w.q_aligned = (((uintptr_t)a.q | a.q_seq_stride * eb | a.q_token_stride * eb) & 15) == 0;
+  w.out_aligned = ((uintptr_t)a.out & 15) == 0;
+  CUtensorMap m[4] = {};
+  if (!Q8) {
+    const size_t cap = std::max<size_t>(a.cap, 1);
+    int rc = kv_plane_map(a.sk, a.n_seqs, cap, cap, a.n_kv, D, &m[2]);
+    if (rc == RV_OK) rc = kv_plane_map(a.sv, a.n_seqs, cap, cap, a.n_kv, D, &m[3]);
+    if (rc == RV_OK && a.prefix_len) rc = kv_plane_map(a.pk, 1, a.prefix_len, a.prefix_len, a.n_kv, D, &m[0]);
+    if (rc == RV_OK && a.prefix_len) rc = kv_plane_map(a.pv, 1, a.prefix_len, a.prefix_len, a.n_kv, D, &m[1]);
+    if (rc) return rc;
+  }
+  k_prefix_tc<D, T, Q8><<<w.grid, C::THREADS, C::total, s>>>(a, w, m[0], m[1], m[2], m[3]);
+  RV_LAUNCH_CHECK();
+  RV_CUDA(launch_pdl(k_prefix_join<D, T>, dim3((unsigned)((w.rows_p + 31) / 32), a.n_kv), dim3(D * 8), 0, s, a, w));
+  return RV_OK;
+}
+template <int D>
+static int prefix_tc(const PrefixArgs &a, bool f32, bool q8, uint8_t *scratch, cudaStream_t s) {
+  if (f32) return q8 ? prefix_tc_launch<D, float, true>(a, scratch, s) : prefix_tc_launch<D, float, false>(a, scratch, s);
+  return q8 ? prefix_tc_launch<D, __half, true>(a, scratch, s) : prefix_tc_launch<D, __half, false>(a, scratch, s);
 }
 
 extern "C" int rv_prefix_attention(const rv_kv_cache *prefix, size_t prefix_len, const rv_kv_cache *suffix,
@@ -2815,8 +2918,10 @@ extern "C" int rv_prefix_attention(const rv_kv_cache *prefix, size_t prefix_len,
   a.hd = suffix->head_dim;
   a.scale_log2 = scale * RV_LOG2E;
   const bool q8 = suffix->format == RV_KV_Q8;
-  const dim3 grid((unsigned)n_heads, (unsigned)n_q, suffix->n_seqs);
   cudaStream_t s = (cudaStream_t)stream;
+  if (a.hd == 64) return prefix_tc<64>(a, dtype == RV_F32, q8, (uint8_t *)scratch, s);
+  if (a.hd == 128) return prefix_tc<128>(a, dtype == RV_F32, q8, (uint8_t *)scratch, s);
+  const dim3 grid((unsigned)n_heads, (unsigned)n_q, suffix->n_seqs);
   if (dtype == RV_F32) {
     if (q8) k_prefix_any<float, true><<<grid, 256, 0, s>>>(a);
     else k_prefix_any<float, false><<<grid, 256, 0, s>>>(a);
