@@ -2822,6 +2822,8 @@ static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t 
   // No more CTAs than units at the suffixes' greatest lengths.
   const size_t most = (size_t)a.n_kv * w.nrt_p * w.tp +
                       (size_t)a.n_kv * w.nrt_s * a.n_seqs * (((size_t)a.cap + RV_PFX_N - 1) / RV_PFX_N);
+  if (most > 0x7FFFFFFFull - RV_PFX_CTAS)
+    RV_FAIL(RV_ERR_UNIMPLEMENTED, "prefix_attention: %zu tiles of queries times keys (< 2^31)", most);
   w.grid = (int)std::max<size_t>(1, std::min(std::min<size_t>(sms, RV_PFX_CTAS), most));
   const PfxScratch o = prefix_scratch(a.n_seqs, a.n_q, a.n_heads, a.n_kv, D, (size_t)w.sr);
   w.cum = (int *)(scratch + o.cum);
@@ -2843,7 +2845,8 @@ static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t 
   }
   k_prefix_tc<D, T, Q8><<<w.grid, C::THREADS, C::total, s>>>(a, w, m[0], m[1], m[2], m[3]);
   RV_LAUNCH_CHECK();
-  RV_CUDA(launch_pdl(k_prefix_join<D, T>, dim3((unsigned)((w.rows_p + 31) / 32), a.n_kv), dim3(D * 8), 0, s, a, w));
+  RV_CUDA(launch_pdl(k_prefix_join<D, T>, dim3((unsigned)((w.rows_p + RV_PFX_JOIN_ROWS - 1) / RV_PFX_JOIN_ROWS), a.n_kv),
+                     dim3(D * 4), 0, s, a, w));
   return RV_OK;
 }
 template <int D>

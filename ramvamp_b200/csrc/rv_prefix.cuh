@@ -165,7 +165,7 @@ struct PfxCfg {
   static constexpr int THREADS = Q8 ? 512 : 384;
   static constexpr int NBARS = 2 * R + 8 + RV_PFX_SCALE_SLOTS + 1;
   static constexpr size_t ring = 2 * TILE, scales = ring + (size_t)R * TILE, bars = scales + SCALES;
-  static constexpr size_t total = 1024 + bars + NBARS * 8 + 32 * 8 + 64;
+  static constexpr size_t total = 1024 + bars + NBARS * 8 + 32 * 4 + 64 + 2 * RV_PFX_M * 4;
 };
 
 struct PfxPiece {
@@ -175,7 +175,7 @@ struct PfxPiece {
 
 // A CTA's way along the line of units [u, end).
 struct PfxWalk {
-  long long u, end, wp, ub;  // wp: units of the prefix; ub: suffix units before sequence b
+  int u, end, wp, ub;  // wp: units of the prefix; ub: suffix units before sequence b
   int b, c;
 };
 RV_DEVFN int pfx_tiles(int keys) { return (keys + RV_PFX_N - 1) / RV_PFX_N; }
@@ -185,8 +185,8 @@ RV_DEVFN bool pfx_next(const PrefixArgs &a, const PfxWork &w, PfxWalk &k, PfxPie
   int seg, tiles, rt, nrt;
   if (k.u < k.wp) {
     tiles = w.tp;
-    seg = (int)(k.u / tiles);
-    p.tile0 = (int)(k.u - (long long)seg * tiles);
+    seg = k.u / tiles;
+    p.tile0 = k.u - seg * tiles;
     nrt = w.nrt_p;
     p.suffix = false;
     p.b = 0;
@@ -197,16 +197,16 @@ RV_DEVFN bool pfx_next(const PrefixArgs &a, const PfxWork &w, PfxWalk &k, PfxPie
     p.slot = seg + k.c;
   } else {
     const int segs = (int)a.n_kv * w.nrt_s;
-    const long long us = k.u - k.wp;
+    const int us = k.u - k.wp;
     for (;;) {
       p.keys = prefix_suffix_len(a, (uint32_t)k.b);
       tiles = pfx_tiles(p.keys);
-      if (us < k.ub + (long long)tiles * segs) break;
-      k.ub += (long long)tiles * segs;
+      if (us < k.ub + tiles * segs) break;
+      k.ub += tiles * segs;
       k.b++;
     }
-    const int local = (int)((us - k.ub) / tiles);
-    p.tile0 = (int)(us - k.ub - (long long)local * tiles);
+    const int local = (us - k.ub) / tiles;
+    p.tile0 = us - k.ub - local * tiles;
     nrt = w.nrt_s;
     p.suffix = true;
     p.b = k.b;
@@ -216,7 +216,7 @@ RV_DEVFN bool pfx_next(const PrefixArgs &a, const PfxWork &w, PfxWalk &k, PfxPie
     p.slot = k.b * segs + local + k.c;
   }
   p.row0 = rt * w.sr;
-  p.n = (int)min((long long)(tiles - p.tile0), k.end - k.u);
+  p.n = min(tiles - p.tile0, k.end - k.u);
   p.pair = p.nrows > RV_PFX_M;
   k.u += p.n;
   return true;
@@ -292,68 +292,77 @@ RV_DEVFN PfxRow pfx_row(const PrefixArgs &a, bool suffix, int b, int kvh, int r)
   return o;
 }
 
-// A row of queries into its place(s) of the A operand (K-major, 128-byte
-// swizzle, 64 values a half tile).  Returns the power of two that f32 queries
-// were divided by.  With store = false only that is computed.
+// The query rows of a stream's tile into the A operand(s) (K-major, 128-byte
+// swizzle, 64 values a half tile), by the stream's 128 threads: D / 8 threads a
+// row, so a row's loads are contiguous, and four rows a thread in flight.  f32
+// rows are divided by a power of two first (2^e in `up`, the largest value
+// then lies in [1, 2)) and held as hi + lo.  With store = false only `up` is
+// formed.  neg: the queries change sign.
 template <int D, typename T>
-RV_DEVFN float pfx_load_q(const PrefixArgs &a, const T *q, bool aligned, bool neg, int row, uint8_t *hi, uint8_t *lo,
-                          bool store) {
-  float up = 1.0f, down = 1.0f;
-  if constexpr (sizeof(T) == 4) {
-    float m = 0;
-    for (int c = 0; c < D / 8; c++) {
-      float x[8];
-      if (aligned) {
-        *(float4 *)x = __ldg((const float4 *)q + 2 * c);
-        *(float4 *)(x + 4) = __ldg((const float4 *)q + 2 * c + 1);
-      } else {
+RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr, bool aligned, bool neg, int tid,
+                         uint8_t *hi, uint8_t *lo, float *up, bool store) {
+  constexpr int LPR = D / 8, RP = RV_PFX_M / LPR;  // threads a row, rows a pass
+  constexpr bool F32 = sizeof(T) == 4;
+  if (!F32 && !store) return;
+  const int c = tid % LPR;
+  for (int b0 = 0; b0 < nr; b0 += 4 * RP) {
+    float x[4][8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = q[8 * c + j];
-      }
+    for (int k = 0; k < 4; k++) {
+      const int row = b0 + k * RP + tid / LPR;
+      if (row < nr) {
+        const PfxRow pr = pfx_row(a, p.suffix, p.b, p.kvh, r0 + row);
+        const T *q = (const T *)a.q + (size_t)pr.b * a.q_seq_stride + (size_t)pr.i * a.q_token_stride +
+                     (size_t)pr.h * D + 8 * c;
+        if (aligned) {
+          if constexpr (F32) {
+            *(float4 *)x[k] = __ldg((const float4 *)q);
+            *(float4 *)(x[k] + 4) = __ldg((const float4 *)q + 1);
+          } else {
+            *(uint4 *)x[k] = __ldg((const uint4 *)q);  // eight f16, taken apart below
+          }
+        } else {
 #pragma unroll
-      for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(x[j]));
-    }
-    // 2^e with m * 2^-e in [1, 2), e within the floats' normal exponents both ways.
-    const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 126);
-    up = __uint_as_float((uint32_t)(e + 127) << 23);
-    down = __uint_as_float((uint32_t)(127 - e) << 23);
-    if (!store) return up;
-  } else if (!store) {
-    return up;
-  }
-  for (int c = 0; c < D / 8; c++) {
-    float x[8];
-    if (aligned) {
-      if constexpr (sizeof(T) == 4) {
-        *(float4 *)x = __ldg((const float4 *)q + 2 * c);
-        *(float4 *)(x + 4) = __ldg((const float4 *)q + 2 * c + 1);
-      } else {
-        const uint4 v = __ldg((const uint4 *)q + c);
-        const __half2 *h = (const __half2 *)&v;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 f = __half22float2(h[j]);
-          x[2 * j] = f.x;
-          x[2 * j + 1] = f.y;
+          for (int j = 0; j < 8; j++)
+            if constexpr (F32) x[k][j] = q[j];
+            else ((T *)x[k])[j] = q[j];
         }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) x[j] = (float)q[8 * c + j];
     }
-    uint32_t o[4], r[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float x0 = (neg ? -x[2 * j] : x[2 * j]) * down, x1 = (neg ? -x[2 * j + 1] : x[2 * j + 1]) * down;
-      o[j] = pack_f16(x0, x1);
-      const float2 f = __half22float2(*(const __half2 *)&o[j]);
-      r[j] = pack_f16(x0 - f.x, x1 - f.y);
+    for (int k = 0; k < 4; k++) {
+      const int row = b0 + k * RP + tid / LPR;
+      const uint32_t off = (uint32_t)(c >> 3) * (RV_PFX_M * 128) + tc_sw_off(row, c & 7);
+      if constexpr (F32) {
+        float m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(x[k][j]));
+        if (row >= nr) m = 0;
+#pragma unroll
+        for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(RV_FULL, m, o));
+        // Both 2^e and 2^-e are normal floats.
+        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 126);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23), sg = neg ? -down : down;
+        if (row >= nr) continue;
+        if (c == 0) up[row] = __uint_as_float((uint32_t)(e + 127) << 23);
+        if (!store) continue;
+        uint32_t o[4], r[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float x0 = x[k][2 * j] * sg, x1 = x[k][2 * j + 1] * sg;
+          o[j] = pack_f16(x0, x1);
+          const float2 f = __half22float2(*(const __half2 *)&o[j]);
+          r[j] = pack_f16(x0 - f.x, x1 - f.y);
+        }
+        *(uint4 *)(hi + off) = make_uint4(o[0], o[1], o[2], o[3]);
+        *(uint4 *)(lo + off) = make_uint4(r[0], r[1], r[2], r[3]);
+      } else if (row < nr) {
+        uint4 v = *(const uint4 *)x[k];
+        const uint32_t sg = neg ? 0x80008000u : 0;
+        *(uint4 *)(hi + off) = make_uint4(v.x ^ sg, v.y ^ sg, v.z ^ sg, v.w ^ sg);
+      }
     }
-    const uint32_t off = (uint32_t)(c >> 3) * (RV_PFX_M * 128) + tc_sw_off(row, c & 7);
-    *(uint4 *)(hi + off) = make_uint4(o[0], o[1], o[2], o[3]);
-    if constexpr (sizeof(T) == 4) *(uint4 *)(lo + off) = make_uint4(r[0], r[1], r[2], r[3]);
   }
-  return up;
 }
 
 // Four int8 levels of a word as two half2, in order.
@@ -406,11 +415,12 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
   uint64_t *bars = (uint64_t *)(sm + C::bars);
   uint64_t *kv_full = bars, *kv_empty = bars + R, *s_full = bars + 2 * R, *p_ready = s_full + 2, *o_full = p_ready + 2,
            *q_ready = o_full + 2, *sc_full = q_ready + 2, *drained = sc_full + RV_PFX_SCALE_SLOTS;
-  long long *s_scan = (long long *)(bars + C::NBARS);  // [16] warp sums, then total, start ub
-  int *s_int = (int *)(s_scan + 32);
+  int *s_scan = (int *)(bars + C::NBARS);  // [16] warp sums, [17] the first sequence's ub
+  int *s_int = s_scan + 32;
   uint32_t *s_tmem = (uint32_t *)s_int;
   volatile int *s_fail = s_int + 1;
   int *s_b = s_int + 2;
+  float *s_up = (float *)(s_int + 16);  // [stream][128] powers of two of f32 query rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   if (threadIdx.x == 0) {
@@ -438,11 +448,11 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
   // The line of units: each thread counts the tiles of a run of sequences.
   const int run = ((int)a.n_seqs + (int)blockDim.x - 1) / (int)blockDim.x;
   const int b0 = min((int)threadIdx.x * run, (int)a.n_seqs), b1 = min(b0 + run, (int)a.n_seqs);
-  long long mine = 0, before;
+  int mine = 0, before;
   for (int b = b0; b < b1; b++) mine += pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
   before = mine;
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(RV_FULL, before, o);
+    const int v = __shfl_up_sync(RV_FULL, before, o);
     if (lane >= o) before += v;
   }
   if (lane == 31) s_scan[warp] = before;
@@ -450,7 +460,7 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  long long all = 0;
+  int all = 0;
   for (int i = 0; i < (int)blockDim.x / 32; i++) {
     if (i < warp) before += s_scan[i];
     all += s_scan[i];
@@ -458,23 +468,23 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
   before -= mine;
   const int segs = (int)a.n_kv * w.nrt_s;
   PfxWalk walk;
-  walk.wp = (long long)a.n_kv * w.nrt_p * w.tp;
-  const long long W = walk.wp + all * segs, per = (W + w.grid - 1) / w.grid;
+  walk.wp = (int)a.n_kv * w.nrt_p * w.tp;
+  const int W = walk.wp + all * segs, per = (W + w.grid - 1) / w.grid;
   walk.c = blockIdx.x;
   walk.u = min(W, blockIdx.x * per);
   walk.end = min(W, walk.u + per);
   if (blockIdx.x == 0) {
-    long long x = before;
+    int x = before;
     for (int b = b0; b < b1; b++) {
-      w.cum[b] = (int)x;
+      w.cum[b] = x;
       x += pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
     }
-    if (threadIdx.x == 0) w.cum[a.n_seqs] = (int)all;
+    if (threadIdx.x == 0) w.cum[a.n_seqs] = all;
   }
   if (walk.u >= walk.wp && walk.u < W) {  // the sequence whose units hold the first
-    const long long us = walk.u - walk.wp;
+    const int us = walk.u - walk.wp;
     if (us >= before * segs && us < (before + mine) * segs) {
-      long long x = before;
+      int x = before;
       int b = b0;
       for (;; b++) {
         const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
@@ -630,16 +640,21 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
       int seen = p.keys;  // keys of the segment that this row sees
       if (p.suffix) seen = min(max(p.keys - (int)a.n_q + 1 + pr.i, 0), p.keys);
       if (!on) seen = 0;
-      float up = 1.0f;
-      if (on) {
-        const T *q = (const T *)a.q + (size_t)pr.b * a.q_seq_stride + (size_t)pr.i * a.q_token_stride + (size_t)pr.h * D;
-        uint8_t *dst = sm + (p.pair && s ? TILE : 0);
-        up = pfx_load_q<D, T>(a, q, w.q_aligned, neg, row, dst, sm + TILE, p.pair || s == 0);
-      }
+      pfx_load_q<D, T>(a, p, p.row0 + (p.pair ? RV_PFX_M * s : 0), min(RV_PFX_M, p.nrows - (p.pair ? RV_PFX_M * s : 0)),
+                       w.q_aligned, neg, row, sm + (p.pair && s ? TILE : 0), sm + TILE, s_up + RV_PFX_M * s,
+                       p.pair || s == 0);
       if (p.pair || s == 0) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_ready[s]);
+      }
+      float up = 1.0f;
+      if constexpr (PRECISE) {
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory");  // the stream's four warps
+        if (on) up = s_up[RV_PFX_M * s + row];
+        // The next piece's are written once every warp has read these: a
+        // stream with tiles waits for its O, which needs all four warps' P.
+        if (t_first >= p.n) asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory");
       }
       const float c = Q8 ? up : up * scale;
       float m_ref = -INFINITY, l = 0.0f;
@@ -841,65 +856,78 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
 }
 
 // The parts of each query row added up: out = sum 2^(m_p - M) O_p / sum
-// 2^(m_p - M) l_p.  grid = (32-row groups of a kv head's rows, kv heads);
-// thread = (row, four values).
+// 2^(m_p - M) l_p.  grid = (8-row groups of a kv head's rows, kv heads); a warp
+// holds eight rows times four part lanes (each takes every fourth part) and
+// two groups of four values, so a load is 128 contiguous bytes a part.
+#define RV_PFX_JOIN_ROWS 8
 template <int D, typename T>
-__global__ void __launch_bounds__(D * 8) k_prefix_join(PrefixArgs a, PfxWork w) {
-  pdl_wait();  // the parts and cum are k_prefix_tc's
-  const int r = blockIdx.x * 32 + (threadIdx.x & 31), d4 = threadIdx.x >> 5, kvh = blockIdx.y;
-  if (r >= w.rows_p) return;
+__global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) {
+  const int lane = threadIdx.x & 31, d4 = threadIdx.x >> 5, kvh = blockIdx.y, pl = lane >> 3;
+  const int r = min((int)blockIdx.x * RV_PFX_JOIN_ROWS + (lane & 7), w.rows_p - 1);
+  const bool on = (int)blockIdx.x * RV_PFX_JOIN_ROWS + (lane & 7) < w.rows_p;
   const PfxRow pr = pfx_row(a, false, 0, kvh, r);
-  const int segs = (int)a.n_kv * w.nrt_s;
-  const long long wp = (long long)a.n_kv * w.nrt_p * w.tp;
-  const long long W = wp + (long long)w.cum[a.n_seqs] * segs, per = max(1ll, (W + w.grid - 1) / w.grid);
-  // Up to two runs of parts: (slot, stream) of the prefix segment and of the
-  // sequence's suffix segment.
+  const int segs = (int)a.n_kv * w.nrt_s, wp = (int)a.n_kv * w.nrt_p * w.tp;
+  pdl_wait();  // cum and the parts are k_prefix_tc's
+  const int W = wp + w.cum[a.n_seqs] * segs, per = max(1, (W + w.grid - 1) / w.grid);
+  // The row's parts: those of its prefix segment, then of its sequence's
+  // suffix segment; each a run with a constant step.
+  const float2 *ml[2];
+  const float4 *po[2];
+  int n[2], step[2], rw[2];
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+    const int rows = s ? w.rows_s : w.rows_p, x = s ? r - pr.b * w.rows_s : r, in = x % w.sr;
+    const int c0 = s ? w.cum[pr.b] : 0, tiles = s ? w.cum[pr.b + 1] - c0 : w.tp;
+    const int local = kvh * (s ? w.nrt_s : w.nrt_p) + x / w.sr, seg = s ? pr.b * segs + local : local;
+    const int u0 = s ? wp + c0 * segs + local * tiles : seg * tiles;
+    const bool pair = min(w.sr, rows - (x - in)) > RV_PFX_M;
+    const int first = u0 / per, last = (u0 + tiles - 1) / per;
+    const size_t part = (size_t)(seg + first) * 2 + (pair ? in / RV_PFX_M : 0);
+    rw[s] = s ? w.rw_s : RV_PFX_M;
+    step[s] = pair ? 2 : 1;
+    n[s] = tiles == 0 ? 0 : (last - first + 1) * (pair ? 1 : 2);
+    ml[s] = (s ? w.ml_s : w.ml_p) + part * rw[s] + in % RV_PFX_M;
+    po[s] = (s ? w.o_s : w.o_p) + (part * (D / 4) + d4) * rw[s] + in % RV_PFX_M;
+  }
   float M = -INFINITY, L = 0;
-  float4 o = make_float4(0, 0, 0, 0);
-  auto run = [&](bool suffix, auto f) {
-    long long u0;
-    int tiles, seg, x, rows;
-    if (suffix) {
-      x = r - pr.b * w.rows_s;
-      rows = w.rows_s;
-      const int c0 = w.cum[pr.b];
-      tiles = w.cum[pr.b + 1] - c0;
-      const int local = kvh * w.nrt_s + x / w.sr;
-      seg = pr.b * segs + local;
-      u0 = wp + (long long)c0 * segs + (long long)local * tiles;
-    } else {
-      x = r;
-      rows = w.rows_p;
-      tiles = w.tp;
-      seg = kvh * w.nrt_p + x / w.sr;
-      u0 = (long long)seg * tiles;
+#pragma unroll
+  for (int s = 0; s < 2; s++)
+#pragma unroll 4
+    for (int i = pl; i < n[s]; i += 4) M = fmaxf(M, ml[s][(size_t)i * step[s] * rw[s]].x);
+  M = fmaxf(M, __shfl_xor_sync(RV_FULL, M, 8));
+  M = fmaxf(M, __shfl_xor_sync(RV_FULL, M, 16));
+  float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < 2; s++)
+#pragma unroll 4
+    for (int i = pl; i < n[s]; i += 4) {
+      const float2 x = ml[s][(size_t)i * step[s] * rw[s]];
+      const float4 *q = po[s] + (size_t)i * step[s] * (D / 4) * rw[s];
+      const float4 v[2] = {q[0], q[(D / 8) * rw[s]]};
+      // -infinity: the row saw none of the part's keys, whose O may be anything.
+      const bool sees = x.x != -INFINITY;
+      const float f = sees ? exp2f(x.x - M) : 0.0f;
+      L += sees ? x.y * f : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        o[4 * j] += sees ? v[j].x * f : 0.0f;
+        o[4 * j + 1] += sees ? v[j].y * f : 0.0f;
+        o[4 * j + 2] += sees ? v[j].z * f : 0.0f;
+        o[4 * j + 3] += sees ? v[j].w * f : 0.0f;
+      }
     }
-    if (tiles == 0) return;
-    const int in = x % w.sr, nrows = min(w.sr, rows - (x - in));
-    const bool pair = nrows > RV_PFX_M;
-    const int rw = suffix ? w.rw_s : RV_PFX_M, row = in % RV_PFX_M;
-    const int c0 = (int)(u0 / per), c1 = (int)((u0 + tiles - 1) / per);
-    const size_t p0 = (size_t)(seg + c0) * 2 + (pair ? in / RV_PFX_M : 0);
-    const int n = (c1 - c0 + 1) * (pair ? 1 : 2), stride = pair ? 2 : 1;
-    for (int i = 0; i < n; i++) f((suffix ? w.ml_s : w.ml_p), (suffix ? w.o_s : w.o_p), p0 + (size_t)i * stride, rw, row);
-  };
-  for (int s = 0; s < 2; s++)
-    run(s, [&](const float2 *ml, const float4 *, size_t part, int rw, int row) { M = fmaxf(M, ml[part * rw + row].x); });
-  for (int s = 0; s < 2; s++)
-    run(s, [&](const float2 *ml, const float4 *po, size_t part, int rw, int row) {
-      const float2 x = ml[part * rw + row];
-      if (x.x == -INFINITY) return;  // the row saw none of the part's keys
-      const float f = exp2f(x.x - M);
-      const float4 v = po[(part * (D / 4) + d4) * rw + row];
-      L = fmaf(x.y, f, L);
-      o.x = fmaf(v.x, f, o.x);
-      o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z);
-      o.w = fmaf(v.w, f, o.w);
-    });
+#pragma unroll
+  for (int k = 8; k <= 16; k *= 2) {
+    L += __shfl_xor_sync(RV_FULL, L, k);
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] += __shfl_xor_sync(RV_FULL, o[j], k);
+  }
+  if (!on || pl >= 2) return;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  T *out = (T *)a.out + (((size_t)pr.b * a.n_q + pr.i) * a.n_heads + pr.h) * D + 4 * d4;
-  const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  T *out = (T *)a.out + (((size_t)pr.b * a.n_q + pr.i) * a.n_heads + pr.h) * D + 4 * (d4 + pl * (D / 8));
+  float v[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) v[j] = (pl ? o[4 + j] : o[j]) * inv;
   if (!w.out_aligned) {
 #pragma unroll
     for (int j = 0; j < 4; j++) out[j] = (T)v[j];
