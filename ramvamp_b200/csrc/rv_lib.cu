@@ -2747,26 +2747,40 @@ extern "C" int rv_kv_read(const rv_kv_cache *c, int dtype, size_t n, const int32
   return RV_OK;
 }
 
-// Work shape and scratch sections of a tensor-core call (offsets in bytes;
-// *end is the size).  sr: rows of a segment.
+// Scratch sections of a tensor-core call (offsets in bytes; `end` is the
+// size).
 struct PfxScratch {
   size_t cum, ml_p, ml_s, o_p, o_s, end;
 };
 static bool prefix_tc_dim(size_t head_dim) { return head_dim == 64 || head_dim == 128; }
-static PfxScratch prefix_scratch(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv, size_t hd, size_t sr) {
-  const size_t rows_s = n_q * (n_heads / n_kv), rows_p = rows_s * n_seqs, rw_s = std::min<size_t>(RV_PFX_M, rows_s);
-  // A part for every piece: the cut points are at most one per CTA, and a
-  // segment has one piece more than cuts.  Two streams a piece.
-  const size_t parts_p = 2 * (n_kv * ((rows_p + sr - 1) / sr) + RV_PFX_CTAS);
-  const size_t parts_s = 2 * (n_seqs * n_kv * ((rows_s + sr - 1) / sr) + RV_PFX_CTAS);
+// The work shape: paired prefix segments of 2 * 128 rows or solo ones of sr.
+static void prefix_shape(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv, size_t prefix_len, size_t sr,
+                         bool may_pair, PfxWork *w) {
+  const size_t G = n_heads / n_kv;
+  w->tp = (int)((prefix_len + RV_PFX_N - 1) / RV_PFX_N);
+  w->rows_s = (int)(n_q * G);
+  w->rows_p = (int)(n_seqs * n_q * G);
+  w->pair = may_pair && w->rows_p > RV_PFX_M && prefix_len;
+  w->sr_p = w->pair ? 2 * RV_PFX_M : (int)sr;
+  w->sr_s = (int)sr;
+  w->nrt_p = (w->rows_p + w->sr_p - 1) / w->sr_p;
+  w->nrt_s = (w->rows_s + w->sr_s - 1) / w->sr_s;
+  w->rw_p = w->pair ? RV_PFX_M : std::min((int)sr, w->rows_p);
+  w->rw_s = std::min((int)sr, w->rows_s);
+}
+static PfxScratch prefix_scratch(size_t n_seqs, size_t n_kv, size_t hd, const PfxWork &w) {
+  // A segment has one piece more than cuts, and the cuts of a line are fewer
+  // than the CTAs (paired; a part a stream) or streams (solo) on it.
+  const size_t parts_p = w.pair ? 2 * (n_kv * w.nrt_p + RV_PFX_CTAS) : n_kv * w.nrt_p + 2 * RV_PFX_CTAS;
+  const size_t parts_s = n_seqs * n_kv * w.nrt_s + 2 * RV_PFX_CTAS;
   const auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   PfxScratch o;
   o.cum = 0;
-  o.ml_p = up((n_seqs + 1) * sizeof(int));
-  o.ml_s = o.ml_p + up(parts_p * RV_PFX_M * sizeof(float2));
-  o.o_p = o.ml_s + up(parts_s * rw_s * sizeof(float2));
-  o.o_s = o.o_p + up(parts_p * RV_PFX_M * hd * sizeof(float));
-  o.end = o.o_s + up(parts_s * rw_s * hd * sizeof(float));
+  o.ml_p = up(2 * (n_seqs + 1) * sizeof(int));
+  o.ml_s = o.ml_p + up(parts_p * w.rw_p * sizeof(float2));
+  o.o_p = o.ml_s + up(parts_s * w.rw_s * sizeof(float2));
+  o.o_s = o.o_p + up(parts_p * w.rw_p * hd * sizeof(float));
+  o.end = o.o_s + up(parts_s * w.rw_s * hd * sizeof(float));
   return o;
 }
 
@@ -2778,10 +2792,15 @@ extern "C" int rv_prefix_attention_scratch(size_t n_seqs, size_t n_q, size_t n_h
     RV_FAIL(RV_ERR_LENGTH_MISMATCH, "prefix_attention_scratch: %zu query heads over %zu kv heads", n_heads, n_kv_heads);
   if (sat_mul(sat_mul(n_seqs, n_q), n_heads) > (1u << 30))
     RV_FAIL(RV_ERR_UNIMPLEMENTED, "prefix_attention: %zu x %zu x %zu query rows (<= 2^30)", n_seqs, n_q, n_heads);
-  // Segments of 128 rows (f32 queries) need the most parts.
-  *bytes_out = prefix_tc_dim(head_dim)
-                   ? prefix_scratch(n_seqs, n_q, n_heads, n_kv_heads, head_dim, RV_PFX_M).end
-                   : 16;
+  // The most that f32 and f16 queries, paired or not, need.
+  size_t most = 16;
+  if (prefix_tc_dim(head_dim) && n_seqs && n_q)
+    for (int i = 0; i < 3; i++) {
+      PfxWork w{};
+      prefix_shape(n_seqs, n_q, n_heads, n_kv_heads, 1, i ? RV_PFX_M : RV_PFX_M / 2, i == 2, &w);
+      most = std::max(most, prefix_scratch(n_seqs, n_kv_heads, head_dim, w).end);
+    }
+  *bytes_out = most;
   return RV_OK;
 }
 
@@ -2808,24 +2827,19 @@ template <int D, typename T, bool Q8>
 static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t s) {
   using C = PfxCfg<D, T, Q8>;
   PfxWork w{};
-  const size_t G = a.n_heads / a.n_kv;
-  w.tp = (int)((a.prefix_len + RV_PFX_N - 1) / RV_PFX_N);
-  w.rows_s = (int)(a.n_q * G);
-  w.rows_p = (int)(a.n_seqs * a.n_q * G);
-  w.rw_s = std::min(RV_PFX_M, w.rows_s);
-  w.sr = C::PRECISE ? RV_PFX_M : 2 * RV_PFX_M;
-  w.nrt_p = (w.rows_p + w.sr - 1) / w.sr;
-  w.nrt_s = (w.rows_s + w.sr - 1) / w.sr;
+  prefix_shape(a.n_seqs, a.n_q, a.n_heads, a.n_kv, a.prefix_len, C::SR, !C::PRECISE, &w);
   int dev = 0;
   RV_CUDA(cudaGetDevice(&dev));
   const size_t sms = g_dev_sms[dev] > 0 ? (size_t)g_dev_sms[dev] : RV_PFX_CTAS;
-  // No more CTAs than units at the suffixes' greatest lengths.
-  const size_t most = (size_t)a.n_kv * w.nrt_p * w.tp +
-                      (size_t)a.n_kv * w.nrt_s * a.n_seqs * (((size_t)a.cap + RV_PFX_N - 1) / RV_PFX_N);
-  if (most > 0x7FFFFFFFull - RV_PFX_CTAS)
+  // No more CTAs than places on the lines at the suffixes' greatest lengths
+  // (two at least, so that a paired prefix leaves one to the suffixes).
+  const size_t cap_tiles = ((size_t)a.cap + RV_PFX_N - 1) / RV_PFX_N;
+  const size_t most = (size_t)a.n_kv * w.nrt_p * (w.tp + RV_PFX_OV) +
+                      (size_t)a.n_kv * w.nrt_s * a.n_seqs * (cap_tiles + RV_PFX_OV);
+  if (most > 0x7FFFFFFFull - 4 * RV_PFX_CTAS)
     RV_FAIL(RV_ERR_UNIMPLEMENTED, "prefix_attention: %zu tiles of queries times keys (< 2^31)", most);
-  w.grid = (int)std::max<size_t>(1, std::min(std::min<size_t>(sms, RV_PFX_CTAS), most));
-  const PfxScratch o = prefix_scratch(a.n_seqs, a.n_q, a.n_heads, a.n_kv, D, (size_t)w.sr);
+  w.grid = (int)std::max<size_t>(2, std::min(std::min<size_t>(sms, RV_PFX_CTAS), most));
+  const PfxScratch o = prefix_scratch(a.n_seqs, a.n_kv, D, w);
   w.cum = (int *)(scratch + o.cum);
   w.ml_p = (float2 *)(scratch + o.ml_p);
   w.ml_s = (float2 *)(scratch + o.ml_s);
@@ -2843,7 +2857,7 @@ static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t 
     if (rc == RV_OK && a.prefix_len) rc = kv_plane_map(a.pv, 1, a.prefix_len, a.prefix_len, a.n_kv, D, &m[1]);
     if (rc) return rc;
   }
-  k_prefix_tc<D, T, Q8><<<w.grid, C::THREADS, C::total, s>>>(a, w, m[0], m[1], m[2], m[3]);
+  k_prefix_tc<D, T, Q8><<<w.grid, RV_PFX_THREADS, C::total, s>>>(a, w, m[0], m[1], m[2], m[3]);
   RV_LAUNCH_CHECK();
   RV_CUDA(launch_pdl(k_prefix_join<D, T>, dim3((unsigned)((w.rows_p + RV_PFX_JOIN_ROWS - 1) / RV_PFX_JOIN_ROWS), a.n_kv),
                      dim3(D * 4), 0, s, a, w));

@@ -9,6 +9,8 @@
 // l = sum exp(s_j - m) and o = sum exp(s_j - m) v_j, and the parts add up as
 // sum_p exp(m_p - M) (l_p, o_p) with M = max m_p.  A row that sees nothing is 0.
 #pragma once
+#include <type_traits>
+
 #include "rv_kv.cuh"
 #include "rv_tc.cuh"
 
@@ -107,119 +109,175 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 // exp(S - m), O += P V, with the running maximum and sum of every row kept in
 // registers and S, P and O in tensor memory.
 //
-// Work: a segment is up to 256 (f32: 128) query rows of one kv head against the prefix or
-// against one sequence's suffix, cut into units of 128 keys.  The units of all
-// segments form one line that the CTAs (one per SM) split evenly, so a CTA
-// walks one to a few pieces of segments whatever the lengths are; each piece
-// leaves (m, l, O) of its rows in scratch and k_prefix_join adds the pieces of
-// a row up.  Piece and slot numbers follow from the lengths alone, so the
-// result does not depend on timing.
+// Work: a segment is a run of query rows of one kv head against the prefix or
+// against one sequence's suffix, cut into units of 128 keys.  The segments'
+// units stand on a line, with RV_PFX_OV places more for each segment's fixed
+// cost, and the line is split evenly; every stretch of a segment is a piece
+// that leaves (m, l, O) of its rows in scratch, and k_prefix_join adds the
+// pieces of a row up.  The split follows from the lengths alone, so the result
+// does not depend on timing.
 //
-// Per CTA two streams of tiles run through the tensor cores, each with its own
-// S, P and O columns and its own softmax warpgroup (thread = row), so one
-// stream's products run under the other's exponentials.  Segments of more than
-// 128 rows (f16 queries) pair the streams: each takes 128 of the rows and both
-// read the same key and value tiles.  Otherwise the streams take alternate
-// tiles of the same rows and leave a part each; f32 queries, whose two operands
-// fill the space of the paired streams' query tiles, have segments of at most
-// 128 rows.
+// Per CTA (one an SM) two streams run through the tensor cores, each with its
+// own S, P and O columns and its own softmax warpgroup (thread = row), so one
+// stream's products run under the other's exponentials.
+//   solo: each stream walks a stretch of the line of its own.
+//   pair: more than 128 query rows of a kv head share the prefix (f16 queries):
+//   the streams take 128 rows each of a segment of 256 and read the same key
+//   and value tiles, halving the traffic per product.  The prefix then has a
+//   line of its own, over a share of the CTAs that follows the costs.
 //
 // f32 queries are held to 2^-22 of their row's largest value as a sum of two
 // f16 (after scaling by a power of two), and so is P: products of f16 with the
 // f16 (or 8-bit) keys and values are exact, so the result carries f32's
-// rounding only; the price is twice the products.  f16 queries round P to f16
-// once, the size of the output's own rounding.  P is scaled by 2^7 and the
-// reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
+// rounding only; the price is twice the products, and for head_dim 128 query
+// tiles of 64 rows (two operands a stream in shared memory).  f16 queries round
+// P to f16 once, the size of the output's own rounding.  P is lifted by 2^7 and
+// the reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
 // normal f16 down to 2^-21 of the largest.
 //
 // 8-bit cache: levels are exact in f16, so the products run on levels.  With
 // sk and sv the tokens' scales, t = s * sk + log2(sv): P = 2^(t - m) already
 // holds sv, and l adds P / sv.
 #define RV_PFX_CTAS 148       // CTAs at most: one per SM of a B200
-#define RV_PFX_M 128          // rows of a stream's tile
+#define RV_PFX_THREADS 384    // loads, products and conversion; two softmax warpgroups
+#define RV_PFX_CONV 96        // threads that turn 8-bit rows into f16 (warps 0, 2, 3)
+#define RV_PFX_M 128          // rows of a product
 #define RV_PFX_N 128          // keys of a tile
+#define RV_PFX_OV 1           // a segment's fixed cost, in units
 #define RV_PFX_LAG 8.0f       // the reference maximum may lag by this (log2)
 #define RV_PFX_LIFT 7.0f      // P is lifted by 2^7
-#define RV_PFX_SCALE_SLOTS 8  // tiles whose token scales are in shared memory
+#define RV_PFX_SCALE_SLOTS 8  // tiles a stream whose token scales are in shared memory
+#define RV_PFX_TABLE 32       // pieces a stream works through between plans
 #define RV_PFX_O 256          // first tensor-memory column of O (S and P: 0..255)
 
 struct PfxWork {
   int tp;              // prefix tiles
   int rows_p, rows_s;  // query rows of one kv head: all sequences', one sequence's
-  int sr;              // rows of a segment: 256 (f16 queries) or 128 (f32)
-  int nrt_p, nrt_s;    // segments of sr rows in them
-  int rw_s;            // rows of a part of a suffix piece: min(128, rows_s)
+  int sr_p, sr_s;      // rows of a prefix / suffix segment
+  int nrt_p, nrt_s;    // segments per kv head (per sequence)
+  int rw_p, rw_s;      // rows of a part
+  int pair;            // the prefix runs on paired streams
   int grid;
   int q_aligned, out_aligned;  // 16-byte loads and stores
-  int *cum;            // [n_seqs + 1] suffix tiles before sequence b, written by CTA 0
-  float4 *o_p, *o_s;   // parts: [slot][stream][hd / 4][rows]
-  float2 *ml_p, *ml_s; // [slot][stream][rows] (m, l)
+  int *cum;            // [2 n_seqs + 1]: suffix tiles, then suffixes that are not empty, before sequence b
+  float4 *o_p, *o_s;   // parts: [part][hd / 4][rows]
+  float2 *ml_p, *ml_s; // [part][rows] (m, l)
 };
+
+// How the lines are split: the same on every CTA and in the join.
+struct PfxLine {
+  int gp;            // CTAs of the paired prefix (0: none)
+  int per_p, per;    // places a paired CTA / a solo stream takes
+  int wp, w;         // places of the paired prefix; of the solo line
+  int solo_p;        // places of the prefix on the solo line (they come first)
+};
+RV_DEVFN int pfx_tiles(int keys) { return (keys + RV_PFX_N - 1) / RV_PFX_N; }
+RV_DEVFN PfxLine pfx_line(const PrefixArgs &a, const PfxWork &w, int tiles, int filled) {
+  PfxLine l;
+  const int seg_p = (int)a.n_kv * w.nrt_p, seg_s = (int)a.n_kv * w.nrt_s;
+  const int suffix = (tiles + filled * RV_PFX_OV) * seg_s;
+  l.solo_p = w.pair || w.tp == 0 ? 0 : seg_p * (w.tp + RV_PFX_OV);
+  l.wp = w.pair ? seg_p * w.tp : 0;
+  l.w = l.solo_p + suffix;
+  // A paired unit costs a CTA about what two solo units (one a stream) do.
+  l.gp = 0;
+  if (l.wp) {
+    const long long cost = 2ll * l.wp, both = cost + l.w;
+    l.gp = min(max((int)((cost * w.grid + both / 2) / both), 1), l.w ? w.grid - 1 : w.grid);
+  }
+  l.per_p = l.gp ? (l.wp + l.gp - 1) / l.gp : 1;
+  const int streams = 2 * (w.grid - l.gp);
+  l.per = max(1, streams ? (l.w + streams - 1) / streams : 1);
+  return l;
+}
+
+// A piece: a stretch of a segment.  n = 0: nothing to do.
+struct __align__(16) PfxPiece {
+  int b, head, row0, keys;  // head: 2 * kv head + (1: a suffix)
+  int tile0, n, part, pad;
+};
+// A stream's stretch of its line: places [u, end), which is stretch v, over
+// the segments g0..g1 (counted along the line, empty ones included).
+struct PfxStretch {
+  int u, end, v, g0, g1;
+};
+// Segment [at, at + len) of the line (fixed cost ov, then tiles) cut to a stretch.
+RV_DEVFN void pfx_cut(PfxPiece &p, const PfxStretch &k, int at, int tiles, int ov) {
+  const int x0 = max(k.u - at, 0), x1 = min(k.end - at, tiles + ov);
+  p.tile0 = max(0, x0 - ov);
+  p.n = max(0, x1 - ov - p.tile0);
+}
 
 template <int D, typename T, bool Q8>
 struct PfxCfg {
   static constexpr bool PRECISE = sizeof(T) == 4;
-  static constexpr int TILE = RV_PFX_M * D * 2;                 // bytes of a Q, K or V tile
+  static constexpr int SR = PRECISE && D == 128 ? 64 : 128;     // query rows of a stream
+  static constexpr int QT = SR * D * 2;                         // bytes of one query operand
+  static constexpr int QS = QT * (PRECISE ? 2 : 1);             // of a stream's
+  static constexpr int TILE = RV_PFX_N * D * 2;                 // of a K or V tile
   static constexpr int R = D == 64 ? 8 : Q8 ? 4 : 5;            // K/V ring stages
-  static constexpr int SCALES = Q8 ? RV_PFX_SCALE_SLOTS * 3 * RV_PFX_N * 4 : 0;
-  static constexpr int THREADS = Q8 ? 512 : 384;
-  static constexpr int NBARS = 2 * R + 8 + RV_PFX_SCALE_SLOTS + 1;
-  static constexpr size_t ring = 2 * TILE, scales = ring + (size_t)R * TILE, bars = scales + SCALES;
-  static constexpr size_t total = 1024 + bars + NBARS * 8 + 32 * 4 + 64 + 2 * RV_PFX_M * 4;
+  static constexpr int SCALES = Q8 ? 2 * RV_PFX_SCALE_SLOTS * 3 * RV_PFX_N * 4 : 0;
+  static constexpr int NBARS = 2 * R + 8 + 2 * RV_PFX_SCALE_SLOTS + 1;
+  static constexpr size_t ring = 2 * QS, scales = ring + (size_t)R * TILE, table = scales + SCALES,
+                          ups = table + 2 * RV_PFX_TABLE * sizeof(PfxPiece), bars = ups + (PRECISE ? 4 * SR : 0);
+  static constexpr size_t total = bars + NBARS * 8 + 48 * 4;
+  static_assert(total <= 227 * 1024, "shared memory of a CTA");
 };
 
-struct PfxPiece {
-  bool suffix, pair;
-  int b, kvh, row0, nrows, keys, tile0, n, slot;
+// The order in which K and V tiles are first used, for the warps that bring
+// them in: K of each stream's first unit, then in turn for each stream V of its
+// unit and K of its next.  Paired streams use the same tiles: one stream here.
+struct PfxFeed {
+  int i[2], j[2], n[2], unit[2];  // entry, tile of it, its tiles (0: the stream has ended), units so far
+  int boot, turn;
+  bool want_k;
+  // The current load.
+  bool is_k;
+  int s, entry, tile, u;
 };
-
-// A CTA's way along the line of units [u, end).
-struct PfxWalk {
-  int u, end, wp, ub;  // wp: units of the prefix; ub: suffix units before sequence b
-  int b, c;
-};
-RV_DEVFN int pfx_tiles(int keys) { return (keys + RV_PFX_N - 1) / RV_PFX_N; }
-
-RV_DEVFN bool pfx_next(const PrefixArgs &a, const PfxWork &w, PfxWalk &k, PfxPiece &p) {
-  if (k.u >= k.end) return false;
-  int seg, tiles, rt, nrt;
-  if (k.u < k.wp) {
-    tiles = w.tp;
-    seg = k.u / tiles;
-    p.tile0 = k.u - seg * tiles;
-    nrt = w.nrt_p;
-    p.suffix = false;
-    p.b = 0;
-    p.keys = (int)a.prefix_len;
-    p.kvh = seg / nrt;
-    rt = seg - p.kvh * nrt;
-    p.nrows = min(w.sr, w.rows_p - rt * w.sr);
-    p.slot = seg + k.c;
-  } else {
-    const int segs = (int)a.n_kv * w.nrt_s;
-    const int us = k.u - k.wp;
-    for (;;) {
-      p.keys = prefix_suffix_len(a, (uint32_t)k.b);
-      tiles = pfx_tiles(p.keys);
-      if (us < k.ub + tiles * segs) break;
-      k.ub += tiles * segs;
-      k.b++;
+RV_DEVFN void pfx_entry(const PfxPiece *tab, int count, int &i, int &n) {
+  for (n = 0; i < count; i++)
+    if ((n = tab[i].n) > 0) return;
+}
+RV_DEVFN bool pfx_feed(const PfxPiece (*tab)[RV_PFX_TABLE], const int (&count)[2], int ns, PfxFeed &f) {
+  for (;;) {
+    int s;
+    if (f.boot < ns) {
+      s = f.boot++;
+      f.i[s] = f.j[s] = 0;
+      pfx_entry(tab[s], count[s], f.i[s], f.n[s]);
+      if (!f.n[s]) continue;
+      f.is_k = true;
+    } else if (f.want_k) {
+      f.want_k = false;
+      s = f.turn;
+      f.turn = ns == 2 ? s ^ 1 : 0;
+      if (!f.n[s]) continue;
+      f.is_k = true;
+    } else {
+      if (!f.n[0] && !f.n[1]) return false;
+      s = f.turn;
+      if (!f.n[s]) {
+        f.turn = s ^ 1;
+        continue;
+      }
+      f.is_k = false;
+      f.want_k = true;
     }
-    const int local = (us - k.ub) / tiles;
-    p.tile0 = us - k.ub - local * tiles;
-    nrt = w.nrt_s;
-    p.suffix = true;
-    p.b = k.b;
-    p.kvh = local / nrt;
-    rt = local - p.kvh * nrt;
-    p.nrows = min(w.sr, w.rows_s - rt * w.sr);
-    p.slot = k.b * segs + local + k.c;
+    f.s = s;
+    f.entry = f.i[s];
+    f.tile = tab[s][f.i[s]].tile0 + f.j[s];
+    f.u = f.unit[s];
+    if (!f.is_k) {
+      f.unit[s]++;
+      if (++f.j[s] == f.n[s]) {
+        f.j[s] = 0;
+        f.i[s]++;
+        pfx_entry(tab[s], count[s], f.i[s], f.n[s]);
+      }
+    }
+    return true;
   }
-  p.row0 = rt * w.sr;
-  p.n = min(tiles - p.tile0, k.end - k.u);
-  p.pair = p.nrows > RV_PFX_M;
-  k.u += p.n;
-  return true;
 }
 
 RV_DEVFN float ex2(float x) {
@@ -227,9 +285,42 @@ RV_DEVFN float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 32 consecutive 32-bit columns of this thread's tensor-memory lane, loaded
-// when it returns (one statement, so no use can be moved before the wait).
-RV_DEVFN void tc_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+// Two f32 operations an instruction.
+RV_DEVFN float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*(unsigned long long *)&d)
+      : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b), "l"(*(unsigned long long *)&c));
+  return d;
+}
+RV_DEVFN float2 add_f32x2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(*(unsigned long long *)&d)
+      : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
+  return d;
+}
+// Consecutive 32-bit columns of this thread's tensor-memory lane, loaded when
+// it returns (one statement, so no use can be moved before the wait).
+RV_DEVFN void tc_ld_wait(uint32_t taddr, uint32_t (&v)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, "
+      "%36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, "
+      "%57, %58, %59, %60, %61, %62, %63}, [%64];\n"
+      " tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]),
+        "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]),
+        "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]),
+        "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]),
+        "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+      : "r"(taddr)
+      : "memory");
+}
+RV_DEVFN void tc_ld_wait(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
       "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
@@ -242,12 +333,20 @@ RV_DEVFN void tc_ld32(uint32_t taddr, uint32_t (&v)[32]) {
       : "memory");
 }
 RV_DEVFN void tc_st16(uint32_t taddr, const uint32_t *v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+      "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+               : "memory");
+}
+RV_DEVFN void tc_st32(uint32_t taddr, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+      "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+      "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+      "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+               : "memory");
 }
 RV_DEVFN void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D[tmem] (+)= A[tmem] * B[smem], kind::f16, issued by one thread.
@@ -263,22 +362,7 @@ RV_DEVFN uint32_t pack_f16(float lo, float hi) {  // element order: lo first
   return *(const uint32_t *)&h;
 }
 
-// Load number of K(t) and V(t) within a piece of n tiles, in the order of first
-// use by the products.  Paired streams: K0 V0 K1 V1 ...; alternating streams:
-// K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1).
-RV_DEVFN int pfx_k_at(bool pair, int t) { return pair ? 2 * t : t == 0 ? 0 : 2 * t - 1; }
-RV_DEVFN int pfx_v_at(bool pair, int t, int n) { return pair ? 2 * t + 1 : min(2 * t + 2, 2 * n - 1); }
-RV_DEVFN void pfx_load_at(bool pair, int i, int n, bool &is_k, int &t) {
-  if (pair) {
-    is_k = !(i & 1);
-    t = i >> 1;
-  } else {
-    is_k = i == 0 || ((i & 1) && i != 2 * n - 1);
-    t = i == 0 ? 0 : i == 2 * n - 1 ? n - 1 : is_k ? (i + 1) >> 1 : (i - 2) >> 1;
-  }
-}
-
-// Query row r of a segment: its sequence, token and head.
+// Query row r of a segment's row space: its sequence, token and head.
 struct PfxRow {
   int b, i, h;
 };
@@ -292,18 +376,17 @@ RV_DEVFN PfxRow pfx_row(const PrefixArgs &a, bool suffix, int b, int kvh, int r)
   return o;
 }
 
-// The query rows of a stream's tile into the A operand(s) (K-major, 128-byte
+// The query rows of a stream's tile into its A operand(s) (K-major, 128-byte
 // swizzle, 64 values a half tile), by the stream's 128 threads: D / 8 threads a
 // row, so a row's loads are contiguous, and four rows a thread in flight.  f32
-// rows are divided by a power of two first (2^e in `up`, the largest value
-// then lies in [1, 2)) and held as hi + lo.  With store = false only `up` is
-// formed.  neg: the queries change sign.
-template <int D, typename T>
+// rows are divided by a power of two first (2^e, e in `up`; the largest value
+// then lies in [1, 2)) and held as hi + lo.  neg: the queries change sign.
+template <int D, typename T, int SR>
 RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr, bool aligned, bool neg, int tid,
-                         uint8_t *hi, uint8_t *lo, float *up, bool store) {
+                         uint8_t *hi, int8_t *up) {
   constexpr int LPR = D / 8, RP = RV_PFX_M / LPR;  // threads a row, rows a pass
   constexpr bool F32 = sizeof(T) == 4;
-  if (!F32 && !store) return;
+  uint8_t *lo = hi + SR * D * 2;
   const int c = tid % LPR;
   for (int b0 = 0; b0 < nr; b0 += 4 * RP) {
     float x[4][8];
@@ -311,7 +394,7 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr,
     for (int k = 0; k < 4; k++) {
       const int row = b0 + k * RP + tid / LPR;
       if (row < nr) {
-        const PfxRow pr = pfx_row(a, p.suffix, p.b, p.kvh, r0 + row);
+        const PfxRow pr = pfx_row(a, p.head & 1, p.b, p.head >> 1, r0 + row);
         const T *q = (const T *)a.q + (size_t)pr.b * a.q_seq_stride + (size_t)pr.i * a.q_token_stride +
                      (size_t)pr.h * D + 8 * c;
         if (aligned) {
@@ -319,7 +402,7 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr,
             *(float4 *)x[k] = __ldg((const float4 *)q);
             *(float4 *)(x[k] + 4) = __ldg((const float4 *)q + 1);
           } else {
-            *(uint4 *)x[k] = __ldg((const uint4 *)q);  // eight f16, taken apart below
+            *(uint4 *)x[k] = __ldg((const uint4 *)q);  // eight f16 as they are
           }
         } else {
 #pragma unroll
@@ -332,7 +415,7 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr,
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const int row = b0 + k * RP + tid / LPR;
-      const uint32_t off = (uint32_t)(c >> 3) * (RV_PFX_M * 128) + tc_sw_off(row, c & 7);
+      const uint32_t off = (uint32_t)(c >> 3) * (SR * 128) + tc_sw_off(row, c & 7);
       if constexpr (F32) {
         float m = 0;
 #pragma unroll
@@ -344,8 +427,7 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr,
         const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 126);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), sg = neg ? -down : down;
         if (row >= nr) continue;
-        if (c == 0) up[row] = __uint_as_float((uint32_t)(e + 127) << 23);
-        if (!store) continue;
+        if (c == 0) up[row] = (int8_t)e;
         uint32_t o[4], r[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -375,57 +457,55 @@ RV_DEVFN void pfx_levels(uint32_t w, uint32_t &a, uint32_t &b) {
   b = *(const uint32_t *)&h;
 }
 
-// Barrier phases that a warp role waits for, with the CTA's failure flag.
+// One lane of a converged warp, known to the compiler as one: the operands of
+// the products it issues are then uniform without a check per lane.
+RV_DEVFN bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// Barrier phases that a whole warp waits for.
 RV_DEVFN bool pfx_wait(uint64_t *bar, uint32_t parity) {
   return __all_sync(RV_FULL, mbar_wait_bounded(bar, parity));
 }
 
-// One 32-key chunk of a row's scores as t = log2 of the unnormalised weights.
-template <bool PRECISE, bool Q8>
-RV_DEVFN void pfx_scores(const uint32_t (&v)[32], float c, const float *ck, const float *lv, float (&t)[32]) {
-#pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    if constexpr (Q8) {
-      const float4 k4 = *(const float4 *)(ck + j), l4 = *(const float4 *)(lv + j);
-      const float kk[4] = {k4.x, k4.y, k4.z, k4.w}, ll[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-      for (int x = 0; x < 4; x++) {
-        const float s = __uint_as_float(v[j + x]);
-        t[j + x] = fmaf(PRECISE ? s * c : s, kk[x], ll[x]);
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 4; x++) t[j + x] = __uint_as_float(v[j + x]) * c;
-    }
-  }
-}
-
 template <int D, typename T, bool Q8>
-__global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
+__global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     k_prefix_tc(PrefixArgs a, PfxWork w, const __grid_constant__ CUtensorMap map_pk,
                 const __grid_constant__ CUtensorMap map_pv, const __grid_constant__ CUtensorMap map_sk,
                 const __grid_constant__ CUtensorMap map_sv) {
   using C = PfxCfg<D, T, Q8>;
   constexpr bool PRECISE = C::PRECISE;
-  constexpr int R = C::R, TILE = C::TILE;
-  extern __shared__ __align__(16) uint8_t sm_raw_[];
-  uint8_t *sm = (uint8_t *)(((uintptr_t)sm_raw_ + 1023) & ~(uintptr_t)1023);
+  constexpr int R = C::R, TILE = C::TILE, SLOTS = RV_PFX_SCALE_SLOTS;
+  extern __shared__ __align__(1024) uint8_t sm[];  // the operand tiles are whole swizzle atoms
   uint8_t *ring = sm + C::ring;
-  float *s_scale = (float *)(sm + C::scales);  // [slot][ck, lv, 1 / sv][128]
+  float *s_scale = (float *)(sm + C::scales);  // [stream][slot][ck, lv, 1 / sv][128]
+  PfxPiece(*tab)[RV_PFX_TABLE] = (PfxPiece(*)[RV_PFX_TABLE])(sm + C::table);
+  int8_t *s_up = (int8_t *)(sm + C::ups);  // [stream][piece & 1][SR] exponents of f32 query rows
   uint64_t *bars = (uint64_t *)(sm + C::bars);
   uint64_t *kv_full = bars, *kv_empty = bars + R, *s_full = bars + 2 * R, *p_ready = s_full + 2, *o_full = p_ready + 2,
-           *q_ready = o_full + 2, *sc_full = q_ready + 2, *drained = sc_full + RV_PFX_SCALE_SLOTS;
-  int *s_scan = (int *)(bars + C::NBARS);  // [16] warp sums, [17] the first sequence's ub
-  int *s_int = s_scan + 32;
-  uint32_t *s_tmem = (uint32_t *)s_int;
-  volatile int *s_fail = s_int + 1;
-  int *s_b = s_int + 2;
-  float *s_up = (float *)(s_int + 16);  // [stream][128] powers of two of f32 query rows
+           *q_ready = o_full + 2, *sc_full = q_ready + 2, *drained = sc_full + 2 * SLOTS;
+  int *s_scan = (int *)(bars + C::NBARS);  // [32] warp sums, then per stream its first and last segment
+  uint32_t *s_tmem = (uint32_t *)(s_scan + 40);
+  volatile int *s_fail = s_scan + 41;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
-  if (threadIdx.x == 0) {
+  if (smem_addr(sm) & 1023) {
+    rv_dev_fail(RV_ERR_CUDA);
+    return;
+  }
+  // Tiles of a run of sequences, and how many have any.
+  const int run = ((int)a.n_seqs + RV_PFX_THREADS - 1) / RV_PFX_THREADS;
+  const int b0 = min((int)threadIdx.x * run, (int)a.n_seqs), b1 = min(b0 + run, (int)a.n_seqs);
+  int mine = 0, filled = 0;
+  for (int b = b0; b < b1; b++) {
+    const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
+    mine += t;
+    filled += t != 0;
+  }
+  if (threadIdx.x == 32) {
     for (int i = 0; i < R; i++) {
-      mbar_init(&kv_full[i], Q8 ? 4 : 1);
+      mbar_init(&kv_full[i], Q8 ? RV_PFX_CONV / 32 : 1);
       mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) {
@@ -434,421 +514,530 @@ __global__ void __launch_bounds__(PfxCfg<D, T, Q8>::THREADS, 1)
       mbar_init(&o_full[i], 1);
       mbar_init(&q_ready[i], 4);
     }
-    for (int i = 0; i < RV_PFX_SCALE_SLOTS; i++) mbar_init(&sc_full[i], 4);
+    if (Q8)
+      for (int i = 0; i < 2 * SLOTS; i++) mbar_init(&sc_full[i], RV_PFX_CONV / 32);
     mbar_init(drained, 1);
     *s_fail = 0;
-    *s_b = 0;
-    s_scan[17] = 0;
+    for (int i = 32; i < 36; i++) s_scan[i] = i & 1 ? -1 : 0;
   }
   if (warp == 0) {
-    __syncwarp();
     tc_alloc(s_tmem, 512);
     tc_relinquish();
   }
-  // The line of units: each thread counts the tiles of a run of sequences.
-  const int run = ((int)a.n_seqs + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int b0 = min((int)threadIdx.x * run, (int)a.n_seqs), b1 = min(b0 + run, (int)a.n_seqs);
-  int mine = 0, before;
-  for (int b = b0; b < b1; b++) mine += pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
-  before = mine;
+  int before = mine, fbefore = filled;
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(RV_FULL, before, o);
-    if (lane >= o) before += v;
+    const int v = __shfl_up_sync(RV_FULL, before, o), f = __shfl_up_sync(RV_FULL, fbefore, o);
+    if (lane >= o) {
+      before += v;
+      fbefore += f;
+    }
   }
-  if (lane == 31) s_scan[warp] = before;
+  if (lane == 31) {
+    s_scan[warp] = before;
+    s_scan[16 + warp] = fbefore;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  int all = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; i++) {
-    if (i < warp) before += s_scan[i];
-    all += s_scan[i];
+  int all = 0, fall = 0;
+#pragma unroll
+  for (int i = 0; i < RV_PFX_THREADS / 32; i++) {
+    const int v = s_scan[i], f = s_scan[16 + i];
+    if (i < warp) {
+      before += v;
+      fbefore += f;
+    }
+    all += v;
+    fall += f;
   }
   before -= mine;
-  const int segs = (int)a.n_kv * w.nrt_s;
-  PfxWalk walk;
-  walk.wp = (int)a.n_kv * w.nrt_p * w.tp;
-  const int W = walk.wp + all * segs, per = (W + w.grid - 1) / w.grid;
-  walk.c = blockIdx.x;
-  walk.u = min(W, blockIdx.x * per);
-  walk.end = min(W, walk.u + per);
+  fbefore -= filled;
+  const PfxLine line = pfx_line(a, w, all, fall);
+  const bool pair = (int)blockIdx.x < line.gp;
+  const int segs = (int)a.n_kv * w.nrt_s, ov_p = pair ? 0 : RV_PFX_OV, len_p = w.tp + ov_p;
+  const int seg_p = pair || line.solo_p ? (int)a.n_kv * w.nrt_p : 0;  // prefix segments on this CTA's line
+  PfxStretch str[2];
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+    PfxStretch &k = str[s];
+    // Solo streams: first stream 0 of every CTA, then stream 1, so few units
+    // spread over all SMs.
+    k.v = pair ? (int)blockIdx.x : (int)blockIdx.x - line.gp + s * (w.grid - line.gp);
+    const int end = pair ? line.wp : line.w, per = pair ? line.per_p : line.per;
+    k.u = min(end, k.v * per);
+    k.end = min(end, k.u + per);
+  }
   if (blockIdx.x == 0) {
-    int x = before;
+    int x = before, f = fbefore;
     for (int b = b0; b < b1; b++) {
       w.cum[b] = x;
-      x += pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
+      w.cum[a.n_seqs + 1 + b] = f;
+      const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
+      x += t;
+      f += t != 0;
     }
-    if (threadIdx.x == 0) w.cum[a.n_seqs] = all;
+    if (threadIdx.x == 0) {
+      w.cum[a.n_seqs] = all;
+      w.cum[2 * a.n_seqs + 1] = fall;
+    }
   }
-  if (walk.u >= walk.wp && walk.u < W) {  // the sequence whose units hold the first
-    const int us = walk.u - walk.wp;
-    if (us >= before * segs && us < (before + mine) * segs) {
-      int x = before;
-      int b = b0;
-      for (;; b++) {
-        const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
-        if (us < (x + t) * segs) break;
-        x += t;
+  // The segments that hold a stretch's first and last place.
+  if (!pair) {
+    int x = line.solo_p + (before + fbefore * RV_PFX_OV) * segs;
+    for (int b = b0; b < b1; b++) {
+      const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b)), len = t ? t + RV_PFX_OV : 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const PfxStretch &k = str[i >> 1];
+        const int u = i & 1 ? k.end - 1 : k.u;
+        if (k.u < k.end && u >= x && u < x + len * segs) s_scan[32 + i] = seg_p + b * segs + (u - x) / len;
       }
-      *s_b = b;
-      s_scan[17] = x * segs;
+      x += len * segs;
     }
   }
   __syncthreads();
-  walk.b = *s_b;
-  walk.ub = s_scan[17];
-  PfxPiece p;
-
-  if (!Q8 && warp == 0) {
-    // ------------------------------------------------------------ loads
-    if (lane == 0) {
-      bool ok = true;
-      int n0 = 0;  // loads of earlier pieces
-      while (ok && !*s_fail && pfx_next(a, w, walk, p)) {
-        const CUtensorMap *mk = p.suffix ? &map_sk : &map_pk, *mv = p.suffix ? &map_sv : &map_pv;
-        for (int i = 0; i < 2 * p.n; i++) {
-          bool is_k;
-          int t;
-          pfx_load_at(p.pair, i, p.n, is_k, t);
-          const int n = n0 + i, slot = n % R;
-          if (!mbar_wait_bounded(&kv_empty[slot], ((n / R) & 1) ^ 1)) {
-            ok = false;
-            n0 = n - 2 * p.n;  // loads issued so far are n (see the drain below)
-            break;
-          }
-          mbar_arrive_expect_tx(&kv_full[slot], (uint32_t)TILE);
 #pragma unroll
-          for (int h = 0; h < D / 64; h++)
-            tma_load_4d(ring + (size_t)slot * TILE + h * (RV_PFX_N * 128), is_k ? mk : mv, 64 * h, p.kvh,
-                        (p.tile0 + t) * RV_PFX_N, p.suffix ? p.b : 0, &kv_full[slot]);
+  for (int s = 0; s < 2; s++) {
+    PfxStretch &k = str[s];
+    const int lim = seg_p * len_p;
+    k.g0 = k.u < lim ? k.u / len_p : s_scan[32 + 2 * s];
+    k.g1 = k.u >= k.end ? k.g0 - 1 : k.end - 1 < lim ? (k.end - 1) / len_p : s_scan[33 + 2 * s];
+  }
+  // Counters that run on over the plans (each role uses its own).
+  int n = 0, np[2] = {0, 0}, nq[2] = {0, 0}, unit = 0, piece = 0;
+  bool ok = true;
+  PfxFeed feed{};
+  for (int base = 0;; base += RV_PFX_TABLE) {
+  // ------------------------------------------------ the next pieces
+  int count[2];
+#pragma unroll
+  for (int s = 0; s < 2; s++) count[s] = min(max(str[s].g1 - str[s].g0 + 1 - base, 0), RV_PFX_TABLE);
+  if (count[0] + count[1] == 0) break;
+  for (int i = threadIdx.x; i < 2 * RV_PFX_TABLE; i += RV_PFX_THREADS) {
+    const int s = i / RV_PFX_TABLE, idx = i % RV_PFX_TABLE;
+    const PfxStretch &k = s ? str[1] : str[0];
+    const int g = k.g0 + base + idx;
+    PfxPiece p{};
+    if (g < seg_p && g <= k.g1) {
+      const int kvh = g / w.nrt_p;
+      p.head = 2 * kvh;
+      p.row0 = (g - kvh * w.nrt_p) * w.sr_p;
+      p.keys = (int)a.prefix_len;
+      p.part = (g + k.v) * (pair ? 2 : 1);
+      pfx_cut(p, k, g * len_p, w.tp, ov_p);
+    }
+    tab[s][idx] = p;
+  }
+  __syncthreads();
+  if (!pair) {
+    int x = line.solo_p + (before + fbefore * RV_PFX_OV) * segs;
+    for (int b = b0; b < b1; b++) {
+      const int keys = prefix_suffix_len(a, (uint32_t)b), t = pfx_tiles(keys), len = t ? t + RV_PFX_OV : 0;
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        const PfxStretch &k = str[s];
+        const int g = seg_p + b * segs, lo = max(0, k.g0 + base - g), hi = min(segs - 1, min(k.g1, k.g0 + base + RV_PFX_TABLE - 1) - g);
+        if (t)
+          for (int local = lo; local <= hi; local++) {
+            PfxPiece p{};
+            const int kvh = local / w.nrt_s;
+            p.b = b;
+            p.head = 2 * kvh + 1;
+            p.row0 = (local - kvh * w.nrt_s) * w.sr_s;
+            p.keys = keys;
+            p.part = b * segs + local + k.v;
+            pfx_cut(p, k, x + local * len, t, RV_PFX_OV);
+            tab[s][g + local - k.g0 - base] = p;
+          }
+      }
+      x += len * segs;
+    }
+    __syncthreads();
+  }
+
+  if (warp < 4) {
+    if (!Q8 && warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- loads
+      PfxFeed &f = feed;
+      f.boot = f.turn = 0;
+      f.want_k = false;
+      f.n[0] = f.n[1] = 0;
+      for (; ok && !*s_fail && pfx_feed(tab, count, pair ? 1 : 2, f); n++) {
+        const int slot = n % R;
+        if (!mbar_wait_bounded(&kv_empty[slot], ((n / R) & 1) ^ 1)) {
+          ok = false;
+          break;
         }
-        n0 += 2 * p.n;
+        mbar_arrive_expect_tx(&kv_full[slot], (uint32_t)TILE);
+        const PfxPiece &p = tab[f.s][f.entry];
+        const bool suffix = p.head & 1;
+        const CUtensorMap *m = suffix ? (f.is_k ? &map_sk : &map_sv) : (f.is_k ? &map_pk : &map_pv);
+#pragma unroll
+        for (int h = 0; h < D / 64; h++)
+          tma_load_4d(ring + (size_t)slot * TILE + h * (RV_PFX_N * 128), m, 64 * h, p.head >> 1, f.tile * RV_PFX_N, p.b,
+                      &kv_full[slot]);
       }
       if (!ok) *s_fail = 1;
       if (*s_fail)  // let the copies in flight land before the CTA ends
-        for (int n = max(0, n0 - R); n < n0; n++) mbar_wait_bounded(&kv_full[n % R], (n / R) & 1);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------- MMA issue
-    const uint32_t hi_sw = (1024u >> 4) | (1u << 14) | (2u << 29);
-    const uint32_t lbo_k = 1u << 16, lbo_v = (uint32_t)(RV_PFX_N * 128 >> 4) << 16;
-    const uint32_t q_lo = smem_addr(sm) >> 4, ring_lo = smem_addr(ring) >> 4;
-    const uint32_t idesc_s = tc_idesc(RV_PFX_N), idesc_o = tc_idesc(D) | (1u << 16);  // B of P V: keys down the rows
-    auto mk = [](uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; };
-    bool ok = true;
-    int n0 = 0, np[2] = {0, 0}, nq[2] = {0, 0};
-    while (ok && !*s_fail && pfx_next(a, w, walk, p)) {
-      const int step = p.pair ? 1 : 2;
-      // S of tile t of stream s; the key tile is released by its last reader.
-      auto qk = [&](int s, int t) {
-        const int n = n0 + pfx_k_at(p.pair, t), slot = n % R;
-        if (!pfx_wait(&kv_full[slot], (n / R) & 1)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t qa = q_lo + (p.pair && s ? TILE >> 4 : 0), kb = ring_lo + (uint32_t)(slot * (TILE >> 4));
+        for (int i = max(0, n - R); i < n; i++) mbar_wait_bounded(&kv_full[i % R], (i / R) & 1);
+    } else if (warp == 1) {
+      // ----------------------------------------------------- MMA issue
+      const uint32_t hi_sw = (1024u >> 4) | (1u << 14) | (2u << 29);
+      const uint32_t lbo_k = 1u << 16, lbo_v = (uint32_t)(RV_PFX_N * 128 >> 4) << 16;
+      const uint32_t q_lo = smem_addr(sm) >> 4, ring_lo = smem_addr(ring) >> 4;
+      const uint32_t idesc_s = tc_idesc(RV_PFX_N), idesc_o = tc_idesc(D) | (1u << 16);  // B of P V: keys down the rows
+      auto mk = [](uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; };
+      int at[2] = {0, 0}, j[2] = {0, 0}, len[2], nk = 0, nv = 0;
+      // One batch of products: S = Q K^T of a stream.
+      auto issue_qk = [&](int s, int slot) {
+        const uint32_t qa = q_lo + s * (C::QS >> 4), kb = ring_lo + (uint32_t)(slot * (TILE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < D / 16; kk++) {
-            const uint32_t o = (uint32_t)(kk >> 2) * (RV_PFX_M * 128 >> 4) + 2 * (kk & 3);
-            tc_mma_f16(tmem + 128 * s, mk(lbo_k | (qa + o), hi_sw), mk(lbo_k | (kb + o), hi_sw), idesc_s, kk != 0);
-            if (PRECISE)
-              tc_mma_f16(tmem + 128 * s, mk(lbo_k | (qa + (TILE >> 4) + o), hi_sw), mk(lbo_k | (kb + o), hi_sw),
-                         idesc_s, 1u);
-          }
-          if (!p.pair || s) tc_commit(&kv_empty[slot]);
-          tc_commit(&s_full[s]);
+        for (int kk = 0; kk < D / 16; kk++) {
+          const uint32_t oq = (uint32_t)(kk >> 2) * (C::SR * 128 >> 4) + 2 * (kk & 3),
+                         okk = (uint32_t)(kk >> 2) * (RV_PFX_N * 128 >> 4) + 2 * (kk & 3);
+          tc_mma_f16(tmem + 128 * s, mk(lbo_k | (qa + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, kk != 0);
+          if (PRECISE)
+            tc_mma_f16(tmem + 128 * s, mk(lbo_k | (qa + (C::QT >> 4) + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw),
+                       idesc_s, 1u);
         }
-        __syncwarp();
-        return true;
+        tc_commit(&s_full[s]);
+        if (!pair || s) tc_commit(&kv_empty[slot]);  // released by its last reader
       };
-      auto pv = [&](int s, int t, bool first, bool last) {
-        const int n = n0 + pfx_v_at(p.pair, t, p.n), slot = n % R;
-        if (!pfx_wait(&kv_full[slot], (n / R) & 1)) return false;
-        const int valid = min(RV_PFX_N, p.keys - (p.tile0 + t) * RV_PFX_N);
-        if (!Q8 && p.suffix && (valid & 15) && !(p.pair && s)) {
+      auto wait_full = [&](int i) { return pfx_wait(&kv_full[i % R], (i / R) & 1); };
+      // A new piece's first S.
+      auto start = [&](int s) {
+        pfx_entry(tab[pair ? 0 : s], count[pair ? 0 : s], at[s], len[s]);
+        j[s] = 0;
+        if (!len[s]) return;
+        ok = pfx_wait(&q_ready[s], nq[s] & 1);
+        nq[s]++;
+        if (!(pair && s)) nk = n++;
+        ok = ok && wait_full(nk);
+        tc_fence_after();
+        if (ok && elect_one()) issue_qk(s, nk % R);
+        __syncwarp();
+      };
+      // O += P V of a stream's unit and the next S of the same piece, in one go.
+      auto turn = [&](int s) {
+        if (!ok || !len[s]) return;
+        const PfxPiece &p = tab[pair ? 0 : s][at[s]];
+        const int valid = min(RV_PFX_N, p.keys - (p.tile0 + j[s]) * RV_PFX_N), steps = (valid + 15) >> 4;
+        const bool more = j[s] + 1 < len[s];
+        if (!(pair && s)) nv = n++;
+        ok = wait_full(nv);
+        if (!Q8 && (p.head & 1) && (valid & 15)) {
           // Rows past the sequence's end hold whatever the cache held: zero
           // those the last K step reads (0 * NaN is not 0).
-          const int rows = ((valid + 15) & ~15) - valid;
-          for (int i = lane; i < rows * (D / 8); i += 32) {
+          for (int i = lane; i < (16 * steps - valid) * (D / 8); i += 32) {
             const int r = valid + i / (D / 8), ch = i % (D / 8);
-            *(uint4 *)(ring + (size_t)slot * TILE + (ch >> 3) * (RV_PFX_N * 128) + tc_sw_off(r, ch & 7)) =
+            *(uint4 *)(ring + (size_t)(nv % R) * TILE + (ch >> 3) * (RV_PFX_N * 128) + tc_sw_off(r, ch & 7)) =
                 make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
           __syncwarp();
         }
-        if (!pfx_wait(&p_ready[s], np[s] & 1)) return false;
+        if (more) {
+          if (!(pair && s)) nk = n++;
+          ok = ok && wait_full(nk);
+        }
+        ok = ok && pfx_wait(&p_ready[s], np[s] & 1);
         np[s]++;
+        if (!ok) return;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t vb = ring_lo + (uint32_t)(slot * (TILE >> 4)), d = tmem + RV_PFX_O + 128 * s;
-          const int steps = (valid + 15) >> 4;
-          for (int kk = 0; kk < steps; kk++) {
-            const uint32_t pa = tmem + 128 * s + 32 * (kk >> 1) + 8 * (kk & 1);
-            const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
-            tc_mma_f16_ta(d, pa, bd, idesc_o, !(first && kk == 0));
-            if (PRECISE) tc_mma_f16_ta(d, pa + 16, bd, idesc_o, 1u);
+        if (elect_one()) {
+          const uint32_t vb = ring_lo + (uint32_t)(nv % R * (TILE >> 4)), d = tmem + RV_PFX_O + 128 * s;
+#pragma unroll
+          for (int kk = 0; kk < 8; kk++) {
+            if (kk < steps) {
+              const uint32_t pa = tmem + 128 * s + 32 * (kk >> 1) + 8 * (kk & 1);
+              const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
+              tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || j[s] != 0);
+              if (PRECISE) tc_mma_f16_ta(d, pa + 16, bd, idesc_o, 1u);
+            }
           }
-          if (!p.pair || s) tc_commit(&kv_empty[slot]);
-          if (last) tc_commit(&o_full[s]);
+          if (more) issue_qk(s, nk % R);
+          else tc_commit(&o_full[s]);
+          if (!pair || s) tc_commit(&kv_empty[nv % R]);
         }
         __syncwarp();
-        return true;
-      };
-      // The query tiles: one for both streams, or one each.
-      for (int s = 0; ok && s < (p.pair ? 2 : 1); s++) {
-        ok = pfx_wait(&q_ready[s], nq[s] & 1);
-        nq[s]++;
-      }
-      tc_fence_after();
-      for (int s = 0; ok && s < 2; s++)
-        if (p.pair || s < p.n) ok = qk(s, p.pair ? 0 : s);
-      for (int j = 0; ok && j < p.n; j += step)
-        for (int s = 0; ok && s < 2; s++) {
-          const int t = p.pair ? j : j + s;
-          if (t >= p.n) break;
-          const bool more = t + step < p.n;
-          ok = pv(s, t, j == 0, !more);
-          if (ok && more) ok = qk(s, t + step);
+        j[s]++;
+        if (!more) {
+          at[s]++;
+          start(s);
         }
-      n0 += 2 * p.n;
-    }
-    if (!ok) *s_fail = 1;
-    if (*s_fail) {  // products in flight end before tensor memory is freed
-      if (lane == 0) {
-        tc_commit(drained);
-        mbar_wait_bounded(drained, 0);
+      };
+      start(0);
+      if (ok) start(1);
+      while (ok && !*s_fail && (len[0] || len[1])) {
+        turn(0);
+        turn(1);
       }
-      __syncwarp();
+      if (!ok) *s_fail = 1;
+      if (*s_fail) {  // products in flight end before tensor memory is freed
+        if (lane == 0) {
+          tc_commit(drained);
+          mbar_wait_bounded(drained, 0);
+        }
+        __syncwarp();
+      }
+    } else if (Q8) {
+      // ---------------------------------- 8-bit rows into f16 operands
+      // 16 levels a load, D / 16 loads a token.  The next tile's levels are in
+      // registers before its stage is free.
+      constexpr int TPT = D / 16, LOADS = RV_PFX_N * TPT, IT = (LOADS + RV_PFX_CONV - 1) / RV_PFX_CONV;
+      const int ct = (warp == 0 ? 0 : 32 * (warp - 1)) + lane;
+      PfxFeed &f = feed;
+      f.boot = f.turn = 0;
+      f.want_k = false;
+      f.n[0] = f.n[1] = 0;
+      for (; ok && !*s_fail && pfx_feed(tab, count, pair ? 1 : 2, f); n++) {
+        const PfxPiece &p = tab[f.s][f.entry];
+        const bool suffix = p.head & 1;
+        const int kvh = p.head >> 1, slot = n % R, valid = min(RV_PFX_N, p.keys - f.tile * RV_PFX_N);
+        const size_t first = (size_t)p.b * a.cap * suffix + (size_t)f.tile * RV_PFX_N;
+        const int8_t *src = (const int8_t *)(f.is_k ? (suffix ? a.sk : a.pk) : (suffix ? a.sv : a.pv));
+        uint4 x[IT];
+#pragma unroll
+        for (int j = 0; j < IT; j++) {
+          const int id = j * RV_PFX_CONV + ct, tok = id / TPT;
+          x[j] = tok < valid ? __ldg((const uint4 *)(src + ((first + tok) * a.n_kv + kvh) * D + (id % TPT) * 16))
+                             : make_uint4(0, 0, 0, 0);
+        }
+        float ks[2] = {0, 0}, vs[2] = {0, 0};
+        if (f.is_k) {
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+            if (ct + j * RV_PFX_CONV < valid) {
+              const size_t at = (first + ct + j * RV_PFX_CONV) * a.n_kv + kvh;
+              ks[j] = (suffix ? a.sks : a.pks)[at];
+              vs[j] = (suffix ? a.svs : a.pvs)[at];
+            }
+        }
+        ok = pfx_wait(&kv_empty[slot], ((n / R) & 1) ^ 1);
+        if (!ok) break;
+        if (f.is_k) {
+          const int at = f.s * SLOTS + f.u % SLOTS;
+          float *sc = s_scale + (size_t)at * 3 * RV_PFX_N;
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const int tok = ct + j * RV_PFX_CONV;
+            // A scale of 0 stands for a row of zeros: any scale does.  One
+            // that is not finite makes the weight NaN by itself, and its
+            // reciprocal must not: rows that do not see the token multiply it
+            // by 0.
+            const float v1 = vs[j] < 0x1p-60f ? 0x1p-60f : vs[j], r1 = __frcp_rn(v1);
+            if (tok < RV_PFX_N) {
+              sc[tok] = ks[j] * fabsf(a.scale_log2);
+              sc[RV_PFX_N + tok] = log2f(v1);
+              sc[2 * RV_PFX_N + tok] = r1 > 0.0f ? r1 : 1.0f;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[at]);
+        }
+        uint8_t *dst = ring + (size_t)slot * TILE;
+#pragma unroll
+        for (int j = 0; j < IT; j++) {
+          const int id = j * RV_PFX_CONV + ct, tok = id / TPT, ch = (id % TPT) * 2;
+          uint32_t o[8];
+          pfx_levels(x[j].x, o[0], o[1]);
+          pfx_levels(x[j].y, o[2], o[3]);
+          pfx_levels(x[j].z, o[4], o[5]);
+          pfx_levels(x[j].w, o[6], o[7]);
+          if (tok < RV_PFX_N) {
+            uint8_t *d = dst + (ch >> 3) * (RV_PFX_N * 128);
+            *(uint4 *)(d + tc_sw_off(tok, ch & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *(uint4 *)(d + tc_sw_off(tok, (ch & 7) + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[slot]);
+      }
+      if (!ok) *s_fail = 1;
     }
-  } else if (warp >= 4 && warp < 12) {
+  } else {
     // --------------------------------------------------------- softmax
     const int s = (warp - 4) >> 2, quad = warp & 3, row = 32 * quad + lane;
     const uint32_t tl = tmem + ((uint32_t)(32 * quad) << 16), tS = tl + 128 * s, tO = tl + RV_PFX_O + 128 * s;
     const bool neg = a.scale_log2 < 0;  // the sign of the scale goes to the queries
     const float scale = fabsf(a.scale_log2);
-    bool ok = true;
-    int ns = 0, no = 0;
-    int gt = 0;  // tiles of earlier pieces
-    while (ok && !*s_fail && pfx_next(a, w, walk, p)) {
-      const int step = p.pair ? 1 : 2, t_first = p.pair ? 0 : s;
-      const int rr = (p.pair ? RV_PFX_M * s : 0) + row;
-      const bool on = rr < p.nrows;
-      const bool warp_on = __any_sync(RV_FULL, on);
-      const PfxRow pr = pfx_row(a, p.suffix, p.b, p.kvh, p.row0 + (on ? rr : 0));
-      int seen = p.keys;  // keys of the segment that this row sees
-      if (p.suffix) seen = min(max(p.keys - (int)a.n_q + 1 + pr.i, 0), p.keys);
-      if (!on) seen = 0;
-      pfx_load_q<D, T>(a, p, p.row0 + (p.pair ? RV_PFX_M * s : 0), min(RV_PFX_M, p.nrows - (p.pair ? RV_PFX_M * s : 0)),
-                       w.q_aligned, neg, row, sm + (p.pair && s ? TILE : 0), sm + TILE, s_up + RV_PFX_M * s,
-                       p.pair || s == 0);
-      if (p.pair || s == 0) {
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_ready[s]);
+    uint8_t *q_dst = sm + s * C::QS;
+    const PfxPiece *mytab = tab[pair ? 0 : s];
+    const int mycount = pair ? count[0] : s ? count[1] : count[0];
+    // Queries of a piece into shared memory, for the products.
+    auto give_q = [&](const PfxPiece &x, int which) {
+      const int r0 = x.row0 + (pair ? RV_PFX_M * s : 0);
+      const int rows = x.head & 1 ? w.rows_s : w.rows_p;
+      pfx_load_q<D, T, C::SR>(a, x, r0, min(C::SR, rows - r0), w.q_aligned, neg, row, q_dst,
+                              s_up + (2 * s + (which & 1)) * C::SR);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[s]);
+    };
+    int at = 0, left;
+    pfx_entry(mytab, mycount, at, left);
+    if (left) give_q(mytab[at], piece);
+    while (ok && left && !*s_fail) {
+      const PfxPiece p = mytab[at];
+      const bool suffix = p.head & 1;
+      const int r = p.row0 + (pair ? RV_PFX_M * s : 0) + row;  // this thread's query row
+      const bool on = row < C::SR && r < (suffix ? w.rows_s : w.rows_p), warp_on = __any_sync(RV_FULL, on);
+      int seen = on ? p.keys : 0;  // keys of the segment that this row sees
+      if (suffix && on) {
+        const PfxRow pr = pfx_row(a, true, p.b, p.head >> 1, r);
+        seen = min(max(p.keys - (int)a.n_q + 1 + pr.i, 0), p.keys);
       }
-      float up = 1.0f;
+      // Scores times c are in units of log2 (8-bit keys: their scales hold
+      // the attention scale).  At least 2^-126, so that -infinity stays one.
+      float c = Q8 ? 1.0f : scale;
       if constexpr (PRECISE) {
         asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory");  // the stream's four warps
-        if (on) up = s_up[RV_PFX_M * s + row];
-        // The next piece's are written once every warp has read these: a
-        // stream with tiles waits for its O, which needs all four warps' P.
-        if (t_first >= p.n) asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory");
+        if (on) c *= __uint_as_float((uint32_t)(s_up[(2 * s + (piece & 1)) * C::SR + row] + 127) << 23);
       }
-      const float c = Q8 ? up : up * scale;
+      c = fmaxf(c, 0x1p-126f);
       float m_ref = -INFINITY, l = 0.0f;
-      for (int t = t_first; ok && t < p.n; t += step) {
-        const int tile = p.tile0 + t, valid = min(RV_PFX_N, p.keys - tile * RV_PFX_N), nch = (valid + 31) >> 5;
+      for (int t = 0; t < p.n; t++, unit++) {
+        const int tile = p.tile0 + t, valid = min(RV_PFX_N, p.keys - tile * RV_PFX_N);
         const int lim = min(max(seen - tile * RV_PFX_N, 0), RV_PFX_N);
-        const float *sc = s_scale + (size_t)((gt + t) % RV_PFX_SCALE_SLOTS) * 3 * RV_PFX_N;
-        if (Q8) ok = pfx_wait(&sc_full[(gt + t) % RV_PFX_SCALE_SLOTS], (uint32_t)((gt + t) / RV_PFX_SCALE_SLOTS) & 1);
-        ok = ok && pfx_wait(&s_full[s], ns & 1);
-        ns++;
+        const int slot = (pair ? 0 : s) * SLOTS + unit % SLOTS;
+        const float *sc = s_scale + (size_t)slot * 3 * RV_PFX_N;
+        if (Q8) ok = pfx_wait(&sc_full[slot], (uint32_t)(unit / SLOTS) & 1);
+        ok = ok && pfx_wait(&s_full[s], unit & 1);
         if (!ok) break;
         tc_fence_after();
         if (warp_on) {
+          // The scores are read twice, for the maximum and for P: a row's 128
+          // do not fit the registers beside the rest.
+          const int halves = valid > 64 ? 2 : 1;
           const bool full = __all_sync(RV_FULL, lim == RV_PFX_N || !on);
-          float mx = -INFINITY;
-          for (int ch = 0; ch < nch; ch++) {
-            uint32_t v[32];
-            float x[32];
-            tc_ld32(tS + 32 * ch, v);
-            pfx_scores<PRECISE, Q8>(v, c, sc + 32 * ch, sc + RV_PFX_N + 32 * ch, x);
-            if (full) {
+          auto scores = [&](int h, uint32_t (&v)[64]) {
+            tc_ld_wait(tS + 64 * h, v);
+            if constexpr (Q8) {
+              const float2 c2 = make_float2(c, c), zero = make_float2(0, 0);
 #pragma unroll
-              for (int j = 0; j < 32; j++) mx = fmaxf(mx, x[j]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; j++) mx = fmaxf(mx, 32 * ch + j < lim ? x[j] : -INFINITY);
+              for (int j = 0; j < 64; j += 4) {
+                const float4 k4 = *(const float4 *)(sc + 64 * h + j), l4 = *(const float4 *)(sc + RV_PFX_N + 64 * h + j);
+                float2 x0 = make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                float2 x1 = make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
+                if (PRECISE) {
+                  x0 = fma_f32x2(x0, c2, zero);
+                  x1 = fma_f32x2(x1, c2, zero);
+                }
+                x0 = fma_f32x2(x0, make_float2(k4.x, k4.y), make_float2(l4.x, l4.y));
+                x1 = fma_f32x2(x1, make_float2(k4.z, k4.w), make_float2(l4.z, l4.w));
+                v[j] = __float_as_uint(x0.x);
+                v[j + 1] = __float_as_uint(x0.y);
+                v[j + 2] = __float_as_uint(x1.x);
+                v[j + 3] = __float_as_uint(x1.y);
+              }
             }
+            if (!full) {
+#pragma unroll
+              for (int j = 0; j < 64; j++) v[j] = 64 * h + j < lim ? v[j] : 0xFF800000u;
+            }
+          };
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int h = 0; h < halves; h++) {
+            uint32_t v[64];
+            scores(h, v);
+#pragma unroll
+            for (int j = 0; j < 64; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
           }
-          if (!on) mx = -INFINITY;
-          if (t == t_first) {
-            m_ref = mx;
-          } else if (const bool move = mx > m_ref + RV_PFX_LAG; __any_sync(RV_FULL, move)) {
+          float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if constexpr (!Q8) top *= c;
+          if (!on) top = -INFINITY;
+          if (t == 0) {
+            m_ref = top;
+          } else if (const bool move = top > m_ref + RV_PFX_LAG; __any_sync(RV_FULL, move)) {
             // Every product issued so far is done (S came after them).
-            const float f = move ? ex2(m_ref - mx) : 1.0f;
-            if (move) m_ref = mx;
+            const float f = move ? ex2(m_ref - top) : 1.0f;
+            if (move) m_ref = top;
             l *= f;
             for (int ch = 0; ch < D / 32; ch++) {
-              uint32_t v[32];
-              tc_ld32(tO + 32 * ch, v);
+              uint32_t o[32];
+              tc_ld_wait(tO + 32 * ch, o);
 #pragma unroll
-              for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
-              tc_st16(tO + 32 * ch, v);
-              tc_st16(tO + 32 * ch + 16, v + 16);
+              for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tc_st32(tO + 32 * ch, o);
             }
           }
           const float m_use = m_ref == -INFINITY ? 0.0f : m_ref - RV_PFX_LIFT;
-          float l0 = 0, l1 = 0;
-          for (int ch = 0; ch < nch; ch++) {
-            uint32_t v[32];
-            float x[32];
-            tc_ld32(tS + 32 * ch, v);
-            pfx_scores<PRECISE, Q8>(v, c, sc + 32 * ch, sc + RV_PFX_N + 32 * ch, x);
+          const float2 c2 = make_float2(c, c), m2 = make_float2(-m_use, -m_use);
+          float2 l2[2] = {make_float2(0, 0), make_float2(0, 0)};
+          for (int h = 0; h < halves; h++) {
+            uint32_t v[64];
+            scores(h, v);
 #pragma unroll
-            for (int j = 0; j < 32; j++) x[j] = ex2(x[j] - m_use);
-            if (!full) {
+            for (int ch = 0; ch < 2; ch++) {
+              uint32_t o[32];
 #pragma unroll
-              for (int j = 0; j < 32; j++) x[j] = 32 * ch + j < lim ? x[j] : 0.0f;
-            }
-            if constexpr (Q8) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 r4 = *(const float4 *)(sc + 2 * RV_PFX_N + 32 * ch + j);
-                const float rs[4] = {r4.x, r4.y, r4.z, r4.w};
-                // A hidden token's 1 / scale may be NaN: its weight is 0 all the same.
-#pragma unroll
-                for (int y = 0; y < 4; y++) {
-                  const float add = full || 32 * ch + j + y < lim ? x[j + y] * rs[y] : 0.0f;
-                  if (y & 1) l1 += add;
-                  else l0 += add;
+              for (int j = 0; j < 16; j++) {
+                const int e = 32 * ch + 2 * j;
+                float2 x = make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+                x = Q8 ? add_f32x2(x, m2) : fma_f32x2(x, c2, m2);
+                x.x = ex2(x.x);
+                x.y = ex2(x.y);
+                if constexpr (Q8)
+                  l2[j & 1] = fma_f32x2(x, *(const float2 *)(sc + 2 * RV_PFX_N + 64 * h + e), l2[j & 1]);
+                else
+                  l2[j & 1] = add_f32x2(l2[j & 1], x);
+                o[j] = pack_f16(x.x, x.y);
+                if constexpr (PRECISE) {
+                  const float2 f = __half22float2(*(const __half2 *)&o[j]);
+                  o[16 + j] = pack_f16(x.x - f.x, x.y - f.y);
                 }
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                l0 += x[j];
-                l1 += x[j + 1];
-              }
+              // P takes the columns its scores came from: 16 of hi, then lo.
+              if constexpr (PRECISE) tc_st32(tS + 64 * h + 32 * ch, o);
+              else tc_st16(tS + 64 * h + 32 * ch, o);
             }
-            uint32_t o[16], r[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-              o[j] = pack_f16(x[2 * j], x[2 * j + 1]);
-              if constexpr (PRECISE) {
-                const float2 f = __half22float2(*(const __half2 *)&o[j]);
-                r[j] = pack_f16(x[2 * j] - f.x, x[2 * j + 1] - f.y);
-              }
-            }
-            // P takes the columns its scores came from.
-            tc_st16(tS + 32 * ch, o);
-            if constexpr (PRECISE) tc_st16(tS + 32 * ch + 16, r);
           }
-          l += l0 + l1;
+          l += (l2[0].x + l2[1].x) + (l2[0].y + l2[1].y);
           tc_wait_st();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[s]);
       }
-      gt += p.n;
+      if (!ok) break;
+      // The products have read this piece's queries (S came after them): give
+      // them the next piece's, under the last P V.
+      at++;
+      pfx_entry(mytab, mycount, at, left);
+      if (left) give_q(mytab[at], piece + 1);
       // ------------------------------------------- the piece's (m, l, O)
-      const int rw = p.suffix ? w.rw_s : RV_PFX_M;
-      const size_t part = (size_t)p.slot * 2 + s;
-      float4 *po = (p.suffix ? w.o_s : w.o_p) + part * (D / 4) * rw + row;
-      float2 *pm = (p.suffix ? w.ml_s : w.ml_p) + part * rw + row;
-      if (ok && t_first < p.n) {
-        ok = pfx_wait(&o_full[s], no & 1);
-        no++;
-        if (!ok) break;
-        tc_fence_after();
-        if (warp_on) {
-          for (int ch = 0; ch < D / 32; ch++) {
-            uint32_t v[32];
-            tc_ld32(tO + 32 * ch, v);
-            if (on) {
-#pragma unroll
-              for (int j = 0; j < 8; j++)
-                po[(size_t)(8 * ch + j) * rw] =
-                    make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
-                                __uint_as_float(v[4 * j + 3]));
-            }
-          }
-          tc_fence_before();
-        }
-      }
+      const int rw = suffix ? w.rw_s : w.rw_p;
+      const size_t part = (size_t)p.part + (pair ? s : 0);
+      float4 *po = (suffix ? w.o_s : w.o_p) + part * (D / 4) * rw + row;
+      float2 *pm = (suffix ? w.ml_s : w.ml_p) + part * rw + row;
       if (on) *pm = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref - RV_PFX_LIFT, l);
-    }
-    if (!ok) *s_fail = 1;
-  } else if (Q8 && warp >= 12) {
-    // ------------------------------------ 8-bit rows into f16 operands
-    // 16 levels a thread and load: D / 16 threads a token.  The next tile's
-    // levels are in registers before its stage is free.
-    constexpr int TPT = D / 16, TOK = 128 / TPT, IT = RV_PFX_N / TOK;
-    const int ct = threadIdx.x - 384, tok0 = ct / TPT, e = (ct % TPT) * 16;
-    bool ok = true;
-    int n0 = 0, gt = 0;
-    while (ok && !*s_fail && pfx_next(a, w, walk, p)) {
-      const size_t first = (p.suffix ? (size_t)p.b * a.cap : 0) + (size_t)p.tile0 * RV_PFX_N;
-      const int left = p.keys - p.tile0 * RV_PFX_N;  // keys from the piece's first tile on
-      for (int i = 0; ok && i < 2 * p.n; i++) {
-        bool is_k;
-        int t;
-        pfx_load_at(p.pair, i, p.n, is_k, t);
-        const int n = n0 + i, slot = n % R, valid = min(RV_PFX_N, left - t * RV_PFX_N);
-        const int8_t *src = (const int8_t *)(is_k ? (p.suffix ? a.sk : a.pk) : (p.suffix ? a.sv : a.pv));
-        uint4 x[IT];
+      ok = pfx_wait(&o_full[s], piece & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (warp_on) {
 #pragma unroll
-        for (int j = 0; j < IT; j++) {
-          const int tok = tok0 + j * TOK;
-          x[j] = tok < valid
-                     ? __ldcs((const uint4 *)(src + ((first + (size_t)t * RV_PFX_N + tok) * a.n_kv + p.kvh) * D + e))
-                     : make_uint4(0, 0, 0, 0);
-        }
-        float ks = 0, vs = 0;
-        if (is_k && ct < valid) {
-          const size_t at = (first + (size_t)t * RV_PFX_N + ct) * a.n_kv + p.kvh;
-          ks = (p.suffix ? a.sks : a.pks)[at];
-          vs = (p.suffix ? a.svs : a.pvs)[at];
-        }
-        ok = pfx_wait(&kv_empty[slot], ((n / R) & 1) ^ 1);
-        if (!ok) break;
-        if (is_k) {
-          float *sc = s_scale + (size_t)((gt + t) % RV_PFX_SCALE_SLOTS) * 3 * RV_PFX_N;
-          // A scale of 0 stands for a row of zeros: any scale does.  NaN and
-          // infinity pass on.
-          const float v1 = vs < 0x1p-60f ? 0x1p-60f : vs;
-          sc[ct] = ks * fabsf(a.scale_log2);
-          sc[RV_PFX_N + ct] = log2f(v1);
-          sc[2 * RV_PFX_N + ct] = __frcp_rn(v1);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sc_full[(gt + t) % RV_PFX_SCALE_SLOTS]);
-        }
-        uint8_t *dst = ring + (size_t)slot * TILE + (e >> 6) * (RV_PFX_N * 128);
+        for (int h = 0; h < D / 64; h++) {
+          uint32_t v[64];
+          tc_ld_wait(tO + 64 * h, v);
+          if (on) {
 #pragma unroll
-        for (int j = 0; j < IT; j++) {
-          const int tok = tok0 + j * TOK, ch = (e & 63) >> 3;
-          uint32_t o[8];
-          pfx_levels(x[j].x, o[0], o[1]);
-          pfx_levels(x[j].y, o[2], o[3]);
-          pfx_levels(x[j].z, o[4], o[5]);
-          pfx_levels(x[j].w, o[6], o[7]);
-          *(uint4 *)(dst + tc_sw_off(tok, ch)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *(uint4 *)(dst + tc_sw_off(tok, ch + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+            for (int j = 0; j < 16; j++)
+              po[(16 * h + j) * rw] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                                  __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+          }
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[slot]);
+        tc_fence_before();
       }
-      n0 += 2 * p.n;
-      gt += p.n;
+      piece++;
     }
     if (!ok) *s_fail = 1;
   }
   tc_fence_before();
-  __syncthreads();
+  __syncthreads();  // the table may be written again
+  if (*s_fail) break;
+  }
   if (warp == 0) {
     tc_fence_after();
     tc_dealloc(tmem, 512);
@@ -866,9 +1055,10 @@ __global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) 
   const int r = min((int)blockIdx.x * RV_PFX_JOIN_ROWS + (lane & 7), w.rows_p - 1);
   const bool on = (int)blockIdx.x * RV_PFX_JOIN_ROWS + (lane & 7) < w.rows_p;
   const PfxRow pr = pfx_row(a, false, 0, kvh, r);
-  const int segs = (int)a.n_kv * w.nrt_s, wp = (int)a.n_kv * w.nrt_p * w.tp;
+  const int segs = (int)a.n_kv * w.nrt_s;
   pdl_wait();  // cum and the parts are k_prefix_tc's
-  const int W = wp + w.cum[a.n_seqs] * segs, per = max(1, (W + w.grid - 1) / w.grid);
+  const int *fcum = w.cum + a.n_seqs + 1;
+  const PfxLine line = pfx_line(a, w, w.cum[a.n_seqs], fcum[a.n_seqs]);
   // The row's parts: those of its prefix segment, then of its sequence's
   // suffix segment; each a run with a constant step.
   const float2 *ml[2];
@@ -876,16 +1066,18 @@ __global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) 
   int n[2], step[2], rw[2];
 #pragma unroll
   for (int s = 0; s < 2; s++) {
-    const int rows = s ? w.rows_s : w.rows_p, x = s ? r - pr.b * w.rows_s : r, in = x % w.sr;
-    const int c0 = s ? w.cum[pr.b] : 0, tiles = s ? w.cum[pr.b + 1] - c0 : w.tp;
-    const int local = kvh * (s ? w.nrt_s : w.nrt_p) + x / w.sr, seg = s ? pr.b * segs + local : local;
-    const int u0 = s ? wp + c0 * segs + local * tiles : seg * tiles;
-    const bool pair = min(w.sr, rows - (x - in)) > RV_PFX_M;
+    const bool pair = !s && w.pair;
+    const int sr = s ? w.sr_s : w.sr_p, x = s ? r - pr.b * w.rows_s : r, in = x % sr;
+    const int c0 = s ? w.cum[pr.b] : 0, tiles = s ? w.cum[pr.b + 1] - c0 : w.tp, ov = pair ? 0 : RV_PFX_OV;
+    const int local = kvh * (s ? w.nrt_s : w.nrt_p) + x / sr, seg = s ? pr.b * segs + local : local;
+    // The places of the segment's tiles on its line.
+    const int u0 = (s ? line.solo_p + (c0 + fcum[pr.b] * RV_PFX_OV) * segs : 0) + local * (tiles + ov) + ov;
+    const int per = pair ? line.per_p : line.per;
     const int first = u0 / per, last = (u0 + tiles - 1) / per;
-    const size_t part = (size_t)(seg + first) * 2 + (pair ? in / RV_PFX_M : 0);
-    rw[s] = s ? w.rw_s : RV_PFX_M;
+    const size_t part = (size_t)(seg + first) * (pair ? 2 : 1) + (pair ? in / RV_PFX_M : 0);
+    rw[s] = s ? w.rw_s : w.rw_p;
     step[s] = pair ? 2 : 1;
-    n[s] = tiles == 0 ? 0 : (last - first + 1) * (pair ? 1 : 2);
+    n[s] = tiles == 0 ? 0 : last - first + 1;
     ml[s] = (s ? w.ml_s : w.ml_p) + part * rw[s] + in % RV_PFX_M;
     po[s] = (s ? w.o_s : w.o_p) + (part * (D / 4) + d4) * rw[s] + in % RV_PFX_M;
   }
@@ -899,7 +1091,7 @@ __global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) 
   float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
   for (int s = 0; s < 2; s++)
-#pragma unroll 4
+#pragma unroll 2
     for (int i = pl; i < n[s]; i += 4) {
       const float2 x = ml[s][(size_t)i * step[s] * rw[s]];
       const float4 *q = po[s] + (size_t)i * step[s] * (D / 4) * rw[s];
