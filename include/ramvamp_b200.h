@@ -731,13 +731,13 @@ RV_API int rv_prefix_attention(const rv_kv_cache *prefix, size_t prefix_len, con
                                const int32_t *lens, int dtype, const void *q, size_t q_seq_stride,
                                size_t q_token_stride, size_t n_q, size_t n_heads, float scale, void *out,
                                void *scratch, size_t scratch_len, rv_stream stream);
-/* Bytes of scratch rv_prefix_attention needs for this geometry on the current
- * device, whatever the lengths. */
+/* Bytes of scratch rv_prefix_attention needs for this geometry, whatever the
+ * lengths, formats and types. */
 RV_API int rv_prefix_attention_scratch(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv_heads, size_t head_dim,
                                        size_t *bytes_out);
 
 /* Draws one token of each of n_rows rows of logits (device f32, row r at
- * r*row_stride, n of them, n < 2^23).  Per row, with l the logits (NaN as
+ * r*row_stride, n of them, n < 2^22).  Per row, with l the logits (NaN as
  * -infinity): z = (l - max l) / temperature, weights exp(z); in descending
  * order of l, equal values by ascending index, top_k keeps the first k tokens
  * (k <= 0 or >= n: all), top_p < 1 of those the tokens whose preceding weight

@@ -32,6 +32,7 @@ import ctypes
 import os
 from dataclasses import dataclass
 from enum import IntEnum
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import torch
@@ -732,6 +733,14 @@ def rmsnorm_quantize(x: torch.Tensor, w: torch.Tensor, eps: float, q8k_out: torc
 
 # ------------------------------------------- continuations of one prompt
 KV_F16, KV_Q8 = 0, 1  # rv_kv_format
+
+
+def _stream_now() -> int:
+    """``_stream()`` without building a Stream object: these calls are short,
+    and the object alone takes 3 us."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # rv_dtype
 
 
@@ -834,7 +843,7 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[t
     if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
         raise KernelError(5, "LengthMismatch: k and v must be alike in shape, strides and type")
     _check(lib().rv_kv_append(cache._ref, _dtype(k), k.data_ptr(), v.data_ptr(), seq, token, n,
-                              _i32(lens, cache.n_seqs, "lens"), position, _stream()))
+                              _i32(lens, cache.n_seqs, "lens"), position, _stream_now()))
 
 
 def kv_read(cache: KvCache, n: int, lens: Optional[torch.Tensor] = None, position: int = 0,
@@ -844,7 +853,7 @@ def kv_read(cache: KvCache, n: int, lens: Optional[torch.Tensor] = None, positio
     k = torch.empty((cache.n_seqs, n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
     _check(lib().rv_kv_read(cache._ref, _dtype(k), n, _i32(lens, cache.n_seqs, "lens"), position, k.data_ptr(),
-                            v.data_ptr(), _stream()))
+                            v.data_ptr(), _stream_now()))
     return k, v
 
 
@@ -874,12 +883,13 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
     _check(lib().rv_prefix_attention(prefix._ref if prefix is not None else None, prefix_len, suffix._ref,
                                      _i32(lens, n, "lens"), _dtype(q), q.data_ptr(), s[0], s[1], n_q, H,
                                      D ** -0.5 if scale is None else scale, out.data_ptr(), scratch.data_ptr(),
-                                     _nbytes(scratch), _stream()))
+                                     _nbytes(scratch), _stream_now()))
     return out
 
 
+@lru_cache(maxsize=256)
 def prefix_attention_scratch(n_seqs: int, n_q: int, n_heads: int, n_kv_heads: int, head_dim: int) -> int:
-    """Bytes of scratch ``prefix_attention`` needs on the current device."""
+    """Bytes of scratch ``prefix_attention`` needs for this geometry."""
     n = ctypes.c_size_t()
     _check(lib().rv_prefix_attention_scratch(n_seqs, n_q, n_heads, n_kv_heads, head_dim, ctypes.byref(n)))
     return n.value
@@ -904,7 +914,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     _check(lib().rv_sample(logits.data_ptr(), logits.stride(0), rows, n, _f32(u, rows, "u"),
                            _f32(temperature, rows, "temperature"), _i32(top_k, rows, "top_k"),
                            _f32(top_p, rows, "top_p"), _f32(min_p, rows, "min_p"), _i32(tokens, rows, "tokens"),
-                           _f32(logprobs, rows, "logprobs"), _stream()))
+                           _f32(logprobs, rows, "logprobs"), _stream_now()))
     return tokens, logprobs
 
 
