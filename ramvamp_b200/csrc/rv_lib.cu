@@ -174,8 +174,10 @@ static int ensure_device(int dev) {
   cudaFuncSetAttribute(k_router_logits, cudaFuncAttributeMaxDynamicSharedMemorySize, big);
   prefix_tc_smem<64>();
   prefix_tc_smem<128>();
-  cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RV_SMEM_PER_CTA);
-  cudaFuncSetAttribute(k_sample, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaFuncSetAttribute(k_sample<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RV_SMEM_PER_CTA);
+  cudaFuncSetAttribute(k_sample<512>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaFuncSetAttribute(k_sample<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RV_SMEM_PER_CTA);
+  cudaFuncSetAttribute(k_sample<1024>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   cudaError_t e3 = cudaGetLastError();
   cudaSetDevice(prev);
   if (e1 != cudaSuccess || e2 != cudaSuccess || e3 != cudaSuccess)
@@ -2957,7 +2959,7 @@ extern "C" int rv_sample(const float *logits, size_t row_stride, size_t n_rows, 
                          int32_t *tokens, float *logprobs, rv_stream stream) {
   if (n_rows == 0) return RV_OK;
   if (n == 0) RV_FAIL(RV_ERR_EMPTY, "sample: no logits");
-  if (n >= (1u << 22)) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu logits a row (< 2^22)", n);
+  if (n > RV_SAMPLE_MOST) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu logits a row (<= %d)", n, RV_SAMPLE_MOST);
   if (n_rows >= (1ull << 27)) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu rows (< 2^27)", n_rows);
   if (row_stride < n && n_rows > 1) RV_FAIL(RV_ERR_LENGTH_MISMATCH, "sample: row stride %zu below %zu logits", row_stride, n);
   if (!logits || !u || !tokens ||
@@ -2977,23 +2979,22 @@ extern "C" int rv_sample(const float *logits, size_t row_stride, size_t n_rows, 
   a.top_k = top_k;
   a.tokens = tokens;
   a.logprobs = logprobs;
-  // CTAs of a row's cluster: as many as keep about two CTAs an SM busy, at
-  // least enough for a slice to fit two CTAs into an SM's shared memory (up to
-  // 8; 16 where one row would leave SMs idle or the slice bound asks for it).
+  // CTAs of a row's cluster: enough for a slice to fit two CTAs into an SM's
+  // shared memory (up to 8; 16 where the row asks for it), and more while the
+  // rows alone leave SMs idle and a slice stays worth a CTA.  1,024 threads
+  // where a CTA has its SM to itself.
   const size_t fixed = (sizeof(SampleShared) + 15) / 16 * 16;
   const size_t half = 113 * 1024 - fixed, whole = RV_SMEM_PER_CTA - fixed;
   const auto slice = [&](size_t c) { return ((n + c - 1) / c + 3) / 4 * 4; };
   size_t c = 1;
-  while (c < 16 && ((c < 8 && slice(c) * 4 > half) || (n_rows * c * 2 <= 2 * RV_PFX_CTAS && slice(c) > 1024) ||
-                    slice(c) > RV_SAMPLE_SLICE))
-    c *= 2;
+  while (c < 16 && (slice(c) * 4 > (c < 8 ? half : whole) || (n_rows * c * 2 <= RV_PFX_CTAS && slice(c) > 1024))) c *= 2;
   a.size = (uint32_t)c;
   a.slice = (uint32_t)slice(c);
-  a.in_smem = a.slice * 4 <= whole;
+  const bool alone = n_rows * c <= RV_PFX_CTAS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_rows * c));
-  cfg.blockDim = dim3(RV_SAMPLE_THREADS);
-  cfg.dynamicSmemBytes = fixed + (a.in_smem ? (size_t)a.slice * 4 : 0);
+  cfg.blockDim = dim3(alone ? 1024 : 512);
+  cfg.dynamicSmemBytes = fixed + (size_t)a.slice * 4;
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -3001,7 +3002,7 @@ extern "C" int rv_sample(const float *logits, size_t row_stride, size_t n_rows, 
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  RV_CUDA(cudaLaunchKernelEx(&cfg, k_sample, a));
+  RV_CUDA(cudaLaunchKernelEx(&cfg, alone ? k_sample<1024> : k_sample<512>, a));
   RV_LAUNCH_CHECK();
   return RV_OK;
 }

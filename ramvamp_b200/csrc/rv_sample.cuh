@@ -11,7 +11,7 @@
 //   kept one in index order whose running weight passes the target
 //   logprob = z_token - ln(W 2^-40)
 // The weights' step of 2^-40 loses less than 2^-40 of the largest weight a
-// token; n < 2^22 keeps every sum below 2^63.
+// token; every sum stays below 2^60.
 //
 // One cluster of CTAs a row: each CTA reads its slice of the row once into
 // shared memory (as values with NaN and -0 folded) and every later step works
@@ -23,16 +23,15 @@
 // ranks them against each other.  Bins with more tokens than the list holds
 // (many equal logits) are searched eight bits of the order's key at a time
 // instead.  Weights enter the histogram as three words of 14 bits each, which
-// shared memory adds as 32-bit integers: 2^18 tokens of a slice cannot overflow
-// one.
+// shared memory adds as 32-bit integers: the tokens of a slice (fewer than
+// 2^18) cannot overflow one.
 #pragma once
 #include "rv_internal.cuh"
 
-#define RV_SAMPLE_ONE 0x1p40f
-#define RV_SAMPLE_THREADS 512
+#define RV_SAMPLE_WARPS 32  // at most
 #define RV_SAMPLE_BINS 1024
 #define RV_SAMPLE_LIST 1024    // tokens of one bin that are ranked directly
-#define RV_SAMPLE_SLICE (1u << 18)
+#define RV_SAMPLE_MOST 720896  // logits a row: 16 slices of 176 KB
 #define RV_SAMPLE_K_BINS 32.0f  // top-k's bins per unit of logit
 #define RV_SAMPLE_P_BINS 64.0f  // top-p's per unit of z
 
@@ -42,7 +41,6 @@ struct SampleArgs {
   const float *logits;
   size_t row_stride;
   uint32_t n, slice, size;  // logits of a row, of a CTA; CTAs of a cluster
-  int in_smem;        // the slice is kept in shared memory
   const float *u, *temperature, *top_p, *min_p;
   const int32_t *top_k;
   int32_t *tokens;
@@ -62,16 +60,24 @@ RV_DEVFN float sample_key_value(u64 key) {
 RV_DEVFN float sample_z(float l, float top, float inv_t) {
   return l == top ? 0.0f : __fmul_rn(__fsub_rn(l, top), inv_t);
 }
-RV_DEVFN u64 sample_weight(float e) { return (u64)__fmul_rn(e, RV_SAMPLE_ONE); }
+// floor(e * 2^40) for 0 <= e <= 1, from the bits: conversions to 64-bit
+// integers are a tenth of the rate of shifts.
+RV_DEVFN u64 sample_weight(float e) {
+  const uint32_t b = __float_as_uint(e), m = (b & 0x7FFFFFu) | 0x800000u;
+  const int up = (int)(b >> 23) - 110;  // e = m * 2^(up - 40), up <= 17
+  return up >= 0 ? (u64)m * (1u << up) : (u64)(m >> min(-up, 31));
+}
 
+static_assert(RV_SAMPLE_BINS <= RV_SAMPLE_LIST, "sums of the bins in the list's space");
 // Shared memory of a CTA besides its slice.
 struct SampleShared {
-  u64 red[RV_SAMPLE_THREADS / 32];
+  u64 red[RV_SAMPLE_WARPS];
   u64 best, sum;          // this CTA's, for the cluster
   u64 pick[4];            // results one thread hands to the others
-  u64 list_key[RV_SAMPLE_LIST];
+  u64 list_key[RV_SAMPLE_LIST];      // also the [CTA][bin] sums of a share of the bins, before the list is filled
   u64 list_w[RV_SAMPLE_LIST];
   uint32_t list_n;
+  u64 part_bin;           // the found bin's total
   uint32_t hist[3][RV_SAMPLE_BINS];  // counts, or words of weights, the lowest first
   u64 part[RV_SAMPLE_BINS];          // cluster sums of this CTA's share of the bins
 };
@@ -102,28 +108,45 @@ RV_DEVFN uint32_t atom_add_cluster(uint32_t a, uint32_t v) {
 }
 
 struct SampleRow {
-  const float *x;  // this CTA's slice (shared memory, or global where it does not fit)
-  uint32_t i0, n;  // its first index and length
-  uint32_t rank, size;  // the CTA in the cluster
+  const float *x;        // this CTA's slice, padded with -infinity to a multiple of 4
+  uint32_t i0, n;        // its first index and length
+  uint32_t rank, size;   // the CTA in the cluster
   float top, inv_t, bin_scale;
-  bool raw;        // x is as given: NaN and -0 are not folded yet
-  RV_DEVFN float at(uint32_t i) const { return raw ? sample_value(x[i]) : x[i]; }
+  float fv;              // kept: values above fv, and equal ones up to index fi
+  uint32_t fi;
   RV_DEVFN float e(float l) const { return expf(sample_z(l, top, inv_t)); }
   RV_DEVFN u64 w(float l) const { return sample_weight(e(l)); }
+  RV_DEVFN bool keeps(float l, uint32_t i) const { return l > fv || (l == fv && i0 + i <= fi); }
   RV_DEVFN int bin(float l) const {  // monotone: a larger value has no larger bin
     return min((int)fminf((top - l) * bin_scale, (float)RV_SAMPLE_BINS), RV_SAMPLE_BINS - 1);
+  }
+  RV_DEVFN void keep_from(u64 key) {
+    fv = sample_key_value(key);
+    fi = ~(uint32_t)key;
+  }
+  // f(value, index) for every token of the slice; the padding comes as tokens
+  // of -infinity with indexes from n on.
+  template <int THREADS, typename F>
+  RV_DEVFN void each(F f) const {
+    for (uint32_t i = threadIdx.x; i < (n + 3) / 4; i += THREADS) {
+      const float4 v = ((const float4 *)x)[i];
+      f(v.x, 4 * i);
+      f(v.y, 4 * i + 1);
+      f(v.z, 4 * i + 2);
+      f(v.w, 4 * i + 3);
+    }
   }
 };
 
 // Sum (or maximum) over the CTA; every thread gets it.
-template <typename F>
+template <int THREADS, typename F>
 RV_DEVFN u64 sample_reduce(u64 v, SampleShared &sh, F f) {
   for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(RV_FULL, v, o));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) sh.red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = sh.red[threadIdx.x & (RV_SAMPLE_THREADS / 32 - 1)];
-  for (int o = RV_SAMPLE_THREADS / 64; o; o >>= 1) v = f(v, __shfl_xor_sync(RV_FULL, v, o));
+  v = sh.red[threadIdx.x & (THREADS / 32 - 1)];
+  for (int o = THREADS / 64; o; o >>= 1) v = f(v, __shfl_xor_sync(RV_FULL, v, o));
   return v;
 }
 // Sum (or maximum) over the cluster.  `slot` of every CTA is written before and
@@ -140,24 +163,30 @@ RV_DEVFN u64 sample_cluster_reduce(u64 v, u64 *slot, const SampleRow &r, F f) {
 
 // The bin where the running total (counts or weights, from bin 0 on) reaches
 // `goal`, and the total before it.  Every CTA gets both.
+template <int THREADS>
 RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights, u64 goal, u64 &before) {
   const uint32_t t = threadIdx.x;
   cluster_sync_all();  // the histograms are complete
-  // Each CTA sums its share of the bins over the cluster; then every CTA reads
-  // all the sums.
-  const uint32_t share = RV_SAMPLE_BINS / r.size, f0 = r.rank * share;
-  for (uint32_t b = f0 + t; b < f0 + share; b += RV_SAMPLE_THREADS) {
+  // Each CTA sums its share of the bins over the cluster (a warp reads
+  // consecutive bins of one CTA); then every CTA reads all the sums.
+  const uint32_t share = RV_SAMPLE_BINS / r.size;
+#pragma unroll
+  for (int j = 0; j < RV_SAMPLE_BINS / THREADS; j++) {
+    const uint32_t id = t + j * THREADS, c = id / share, b = r.rank * share + id % share;
+    u64 s = ld_cluster_u32(dsmem_addr(&sh.hist[0][b], c));
+    if (weights)
+      s += ((u64)ld_cluster_u32(dsmem_addr(&sh.hist[1][b], c)) << 14) +
+           ((u64)ld_cluster_u32(dsmem_addr(&sh.hist[2][b], c)) << 28);
+    sh.list_key[id] = s;
+  }
+  __syncthreads();
+  for (uint32_t b = t; b < share; b += THREADS) {
     u64 s = 0;
-    for (uint32_t c = 0; c < r.size; c++) {
-      s += ld_cluster_u32(dsmem_addr(&sh.hist[0][b], c));
-      if (weights)
-        s += ((u64)ld_cluster_u32(dsmem_addr(&sh.hist[1][b], c)) << 14) +
-             ((u64)ld_cluster_u32(dsmem_addr(&sh.hist[2][b], c)) << 28);
-    }
-    sh.part[b] = s;
+    for (uint32_t c = 0; c < r.size; c++) s += sh.list_key[c * share + b];
+    sh.part[r.rank * share + b] = s;
   }
   cluster_sync_all();
-  constexpr int PER = RV_SAMPLE_BINS / RV_SAMPLE_THREADS;
+  constexpr int PER = RV_SAMPLE_BINS / THREADS;
   u64 v[PER], mine = 0;
 #pragma unroll
   for (int j = 0; j < PER; j++) {
@@ -173,14 +202,17 @@ RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights,
   __syncthreads();
   if ((t & 31) == 31) sh.red[t >> 5] = run;
   __syncthreads();
-  for (uint32_t w = 0; w < t >> 5; w++) run += sh.red[w];
-  run -= mine;
+  // Warp sums: lane w holds warp w's; the sum of those before this warp.
+  u64 lower = (t & 31) < t >> 5 ? sh.red[t & 31] : 0;
+  for (int o = 16; o; o >>= 1) lower += __shfl_xor_sync(RV_FULL, lower, o);
+  run += lower - mine;
   if (run < goal && goal <= run + mine) {
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       if (run < goal && goal <= run + v[j]) {
         sh.pick[0] = t * PER + j;
         sh.pick[1] = run;
+        sh.part_bin = v[j];
       }
       run += v[j];
     }
@@ -190,62 +222,69 @@ RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights,
   return (int)sh.pick[0];
 }
 
-// The key of the last token kept when tokens from the largest on are kept until
-// their number (weights: their weight) reaches `goal`; only tokens at or above
-// `from` count.  1 <= goal <= the total.  Every CTA of the cluster gets it.
-RV_DEVFN u64 sample_cutoff(SampleShared &sh, const SampleRow &r, u64 from, u64 goal, bool weights, u64 least) {
+// Tokens from the largest on are kept until their number (weights: their weight)
+// reaches `goal`; of the tokens that the row keeps so far, 1 <= goal <= the
+// total.  Every CTA of the cluster gets the last one's key -- or 0 when counts
+// left no more candidates than the list holds: then all of them, `cnt`, are in
+// every CTA's list with their weights.
+template <int THREADS>
+RV_DEVFN u64 sample_cutoff(SampleShared &sh, const SampleRow &r, u64 goal, bool weights, u64 least, uint32_t &cnt) {
   const uint32_t t = threadIdx.x;
   cluster_sync_all();  // nobody still reads the histograms of an earlier cutoff
-  for (uint32_t b = t; b < RV_SAMPLE_BINS; b += RV_SAMPLE_THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
+  for (uint32_t b = t; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
   if (t == 0) sh.list_n = 0;
   __syncthreads();
-  // Tokens of less than `least` weight cannot lie at or above the cutoff.
-  for (uint32_t i = t; i < r.n; i += RV_SAMPLE_THREADS) {
-    const float l = r.at(i);
-    if (!weights) {
-      const int b = r.bin(l);
-      // The last bin holds the far tail, which k seldom reaches: its count
-      // is what the others leave.
-      if (b < RV_SAMPLE_BINS - 1) atomicAdd(&sh.hist[0][b], 1u);
-    } else if (sample_key(l, r.i0 + i) >= from) {
-      const u64 w = r.w(l);
-      if (w >= least) sample_add(sh, r.bin(l), w);
-    }
-  }
   if (!weights) {
+    // The last bin holds the far tail, which k seldom reaches: its count is
+    // what the others leave.
+    r.each<THREADS>([&](float l, uint32_t) {
+      const int b = r.bin(l);
+      if (b < RV_SAMPLE_BINS - 1) atomicAdd(&sh.hist[0][b], 1u);
+    });
     __syncthreads();
     u64 s = 0;
-    for (uint32_t b = t; b < RV_SAMPLE_BINS - 1; b += RV_SAMPLE_THREADS) s += sh.hist[0][b];
-    s = sample_reduce(s, sh, [](u64 p, u64 q) { return p + q; });
+    for (uint32_t b = t; b < RV_SAMPLE_BINS - 1; b += THREADS) s += sh.hist[0][b];
+    s = sample_reduce<THREADS>(s, sh, [](u64 p, u64 q) { return p + q; });
     if (t == 0) sh.hist[0][RV_SAMPLE_BINS - 1] = r.n - (uint32_t)s;
+  } else {
+    // Tokens of less than `least` weight do not lie at or above the cutoff.
+    r.each<THREADS>([&](float l, uint32_t i) {
+      if (!r.keeps(l, i)) return;
+      const u64 w = r.w(l);
+      if (w >= least) sample_add(sh, r.bin(l), w);
+    });
   }
   u64 before;
-  const int bin = sample_find_bin(sh, r, weights, goal, before);
-  // The bin's tokens go to CTA 0 of the cluster.
+  const int bin = sample_find_bin<THREADS>(sh, r, weights, goal, before);
+  // The bin's tokens -- all up to it, where they are known to fit -- go to the
+  // list of every CTA.
+  const bool all = !weights && before + sh.part_bin <= RV_SAMPLE_LIST;
   const uint32_t list_n = dsmem_addr(&sh.list_n, 0);
-  for (uint32_t i = t; i < r.n; i += RV_SAMPLE_THREADS) {
-    const float l = r.at(i);
-    if (r.bin(l) != bin) continue;
-    const u64 key = sample_key(l, r.i0 + i);
-    if (key < from) continue;
+  r.each<THREADS>([&](float l, uint32_t i) {
+    const int b = r.bin(l);
+    if (!(b == bin || (all && b < bin)) || i >= r.n || !r.keeps(l, i)) return;
     const uint32_t at = atom_add_cluster(list_n, 1u);
     if (at < RV_SAMPLE_LIST) {
-      st_cluster_u64(dsmem_addr(&sh.list_key[at], 0), key);
-      st_cluster_u64(dsmem_addr(&sh.list_w[at], 0), weights ? r.w(l) : 1ull);
-    }
-  }
-  cluster_sync_all();
-  const uint32_t cnt = ld_cluster_u32(list_n);
-  if (cnt <= RV_SAMPLE_LIST) {
-    // Each thread of CTA 0 places its tokens among the list's.
-    if (r.rank == 0) {
-      for (uint32_t i = t; i < cnt; i += RV_SAMPLE_THREADS) {
-        const u64 key = sh.list_key[i];
-        u64 sum = before;
-        for (uint32_t j = 0; j < cnt; j++) sum += sh.list_key[j] > key ? sh.list_w[j] : 0;
-        if (sum < goal && goal <= sum + sh.list_w[i])
-          for (uint32_t c = 0; c < r.size; c++) st_cluster_u64(dsmem_addr(&sh.pick[2], c), key);
+      const u64 key = sample_key(l, r.i0 + i), w = weights || all ? r.w(l) : 1ull;
+      for (uint32_t c = 0; c < r.size; c++) {
+        st_cluster_u64(dsmem_addr(&sh.list_key[at], c), key);
+        st_cluster_u64(dsmem_addr(&sh.list_w[at], c), w);
       }
+    }
+  });
+  cluster_sync_all();
+  cnt = ld_cluster_u32(list_n);
+  if (all) return 0;
+  if (cnt <= RV_SAMPLE_LIST) {
+    // A warp places a token among the list's; the CTAs share the tokens.
+    for (uint32_t i = (t >> 5) * r.size + r.rank; i < cnt; i += THREADS / 32 * r.size) {
+      const u64 key = sh.list_key[i];
+      u64 sum = 0;
+      for (uint32_t j = t & 31; j < cnt; j += 32) sum += sh.list_key[j] > key ? sh.list_w[j] : 0;
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(RV_FULL, sum, o);
+      sum += before;
+      if (sum < goal && goal <= sum + sh.list_w[i] && (t & 31) < r.size)
+        st_cluster_u64(dsmem_addr(&sh.pick[2], t & 31), key);
     }
     cluster_sync_all();
     return sh.pick[2];
@@ -254,26 +293,80 @@ RV_DEVFN u64 sample_cutoff(SampleShared &sh, const SampleRow &r, u64 from, u64 g
   u64 prefix = 0, above = before;
   for (int shift = 56; shift >= 0; shift -= 8) {
     cluster_sync_all();
-    for (uint32_t b = t; b < RV_SAMPLE_BINS; b += RV_SAMPLE_THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
+    for (uint32_t b = t; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
     __syncthreads();
-    for (uint32_t i = t; i < r.n; i += RV_SAMPLE_THREADS) {
-      const float l = r.at(i);
-      if (r.bin(l) != bin) continue;
+    r.each<THREADS>([&](float l, uint32_t i) {
+      if (r.bin(l) != bin || i >= r.n || !r.keeps(l, i)) return;
       const u64 key = sample_key(l, r.i0 + i);
-      if (key < from || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
+      if (shift < 56 && (key >> (shift + 8)) != prefix) return;
       const int d = 255 - (int)((key >> shift) & 255);  // descending
       if (weights) sample_add(sh, d, r.w(l));
       else atomicAdd(&sh.hist[0][d], 1u);
-    }
+    });
     u64 sum;
-    const int d = sample_find_bin(sh, r, weights, goal - above, sum);
+    const int d = sample_find_bin<THREADS>(sh, r, weights, goal - above, sum);
     prefix = prefix << 8 | (u64)(255 - d);
     above += sum;
   }
   return prefix;
 }
 
-__global__ void __launch_bounds__(RV_SAMPLE_THREADS) k_sample(SampleArgs a) {
+// The draw from a list of all candidates (`cnt` of them, more than k only by the
+// last bin's), in one CTA: a warp a token, every filter by sums over the list.
+template <int THREADS>
+RV_DEVFN void sample_from_list(SampleShared &sh, const SampleRow &r, uint32_t cnt, uint32_t k, float p, float mp,
+                               float u, int32_t *token, float *logprob) {
+  const uint32_t t = threadIdx.x, lane = t & 31;
+  const auto add = [](u64 x, u64 y) { return x + y; };
+  // sh.part: the weight before each token in the order, or ~0 past the first k.
+  u64 mine = 0;
+  for (uint32_t i = t >> 5; i < cnt; i += THREADS / 32) {
+    const u64 key = sh.list_key[i];
+    u64 sum = 0;
+    uint32_t rank = 0;
+    for (uint32_t j = lane; j < cnt; j += 32) {
+      const bool ahead = sh.list_key[j] > key;
+      rank += ahead;
+      sum += ahead ? sh.list_w[j] : 0;
+    }
+    rank = __reduce_add_sync(RV_FULL, rank);
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(RV_FULL, sum, o);
+    if (lane == 0) {
+      sh.part[i] = rank < k ? sum : ~0ull;
+      if (rank < k) mine += sh.list_w[i];
+    }
+  }
+  const u64 total = sample_reduce<THREADS>(mine, sh, add);
+  const u64 goal = p < 1.0f ? (u64)fmax(__dmul_rn((double)p, (double)total), 0.0) : ~0ull;
+  mine = 0;
+  for (uint32_t i = t; i < cnt; i += THREADS) {
+    const u64 key = sh.list_key[i], before = sh.part[i];
+    const float l = sample_key_value(key);
+    const bool keep = before != ~0ull && (before < goal || before == 0) && (r.e(l) >= mp || l == r.top);
+    sh.list_w[i] = keep ? sh.list_w[i] : 0;
+    mine += sh.list_w[i];
+  }
+  const u64 W = sample_reduce<THREADS>(mine, sh, add);
+  u64 target = u > 0.0f ? (u64)__dmul_rn((double)u, (double)W) : 0;  // NaN is 0
+  if (target >= W) target = W - 1;
+  for (uint32_t i = t >> 5; i < cnt; i += THREADS / 32) {
+    const uint32_t id = ~(uint32_t)sh.list_key[i];
+    const u64 w = sh.list_w[i];
+    if (w == 0) continue;
+    u64 sum = 0;  // the kept weight of smaller indexes
+    for (uint32_t j = lane; j < cnt; j += 32) sum += ~(uint32_t)sh.list_key[j] < id ? sh.list_w[j] : 0;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(RV_FULL, sum, o);
+    if (lane == 0 && sum <= target && target < sum + w) {
+      *token = (int32_t)id;
+      if (logprob)
+        *logprob = __fsub_rn(sample_z(sample_key_value(sh.list_key[i]), r.top, r.inv_t),
+                             (float)log((double)W * 0x1p-40));
+    }
+  }
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t s_raw[];
   SampleShared &sh = *(SampleShared *)s_raw;
   float *s_slice = (float *)(s_raw + (sizeof(SampleShared) + 15) / 16 * 16);
@@ -285,118 +378,146 @@ __global__ void __launch_bounds__(RV_SAMPLE_THREADS) k_sample(SampleArgs a) {
   r.size = a.size;
   r.i0 = min(a.n, r.rank * a.slice);
   r.n = min(a.n - r.i0, a.slice);
+  r.x = s_slice;
   const float *x = a.logits + (size_t)row * a.row_stride + r.i0;
-  r.x = a.in_smem ? s_slice : x;
-  r.raw = !a.in_smem;
-  u64 best = 0;
-  const bool wide = a.in_smem && (((uintptr_t)x) & 15) == 0;
-  const uint32_t n4 = wide ? r.n / 4 : 0;
+  float top = -INFINITY;
+  const uint32_t n4 = ((uintptr_t)x & 15) == 0 ? r.n / 4 : 0;
 #pragma unroll 4
-  for (uint32_t i = t; i < n4; i += RV_SAMPLE_THREADS) {
+  for (uint32_t i = t; i < n4; i += THREADS) {
     const float4 v = __ldcs((const float4 *)x + i);
     const float4 y = make_float4(sample_value(v.x), sample_value(v.y), sample_value(v.z), sample_value(v.w));
     ((float4 *)s_slice)[i] = y;
-    best = mx(best, mx(mx(sample_key(y.x, r.i0 + 4 * i), sample_key(y.y, r.i0 + 4 * i + 1)),
-                       mx(sample_key(y.z, r.i0 + 4 * i + 2), sample_key(y.w, r.i0 + 4 * i + 3))));
+    top = fmaxf(top, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
   }
 #pragma unroll 8
-  for (uint32_t i = 4 * n4 + t; i < r.n; i += RV_SAMPLE_THREADS) {
+  for (uint32_t i = 4 * n4 + t; i < r.n; i += THREADS) {
     const float l = sample_value(__ldcs(x + i));
-    if (a.in_smem) s_slice[i] = l;
-    best = mx(best, sample_key(l, r.i0 + i));
+    s_slice[i] = l;
+    top = fmaxf(top, l);
   }
-  best = sample_cluster_reduce(sample_reduce(best, sh, mx), &sh.best, r, mx);
+  if (t < 3 && r.n + t < (r.n + 3) / 4 * 4) s_slice[r.n + t] = -INFINITY;
+  // The maximum as the key of index 0: only its value is used.
+  u64 best = sample_cluster_reduce(sample_reduce<THREADS>(sample_key(top, 0), sh, mx), &sh.best, r, mx);
   r.top = sample_key_value(best);
-  const float temp = a.temperature ? a.temperature[row] : 1.0f;
-  if (r.top == -INFINITY || !(temp > 0.0f)) {  // nothing to draw from, or greedy
+  r.fv = -INFINITY;  // everything
+  r.fi = 0xFFFFFFFFu;
+  const float temp = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f;
+  const int k = a.top_k ? a.top_k[row] : 0;
+  const bool none = r.top == -INFINITY, greedy = !(temp > 0.0f);
+  // The first of the largest, where only that can be drawn.
+  const auto first = [&]() {
+    u64 b = 0;
+    r.each<THREADS>([&](float l, uint32_t i) {
+      if (l == r.top && i < r.n) b = mx(b, sample_key(l, r.i0 + i));
+    });
+    return sample_cluster_reduce(sample_reduce<THREADS>(b, sh, mx), &sh.sum, r, mx);
+  };
+  if (none || greedy) {
+    if (!none) best = first();
     if (t == 0 && r.rank == 0) {
-      a.tokens[row] = r.top == -INFINITY ? 0 : (int32_t)~(uint32_t)best;
-      if (a.logprobs) a.logprobs[row] = r.top == -INFINITY ? -INFINITY : 0.0f;
+      a.tokens[row] = none ? 0 : (int32_t)~(uint32_t)best;
+      if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.0f;
     }
-    if (r.size > 1) cluster_sync_all();  // the others may still read this CTA's maximum
+    cluster_sync_all();  // the others may still read this CTA's maximum
     return;
   }
-  r.inv_t = __fdiv_rn(1.0f, temp);
+  r.inv_t = fmaxf(__fdiv_rn(1.0f, temp), 0x1p-126f);  // so that -infinity times it stays one
   r.bin_scale = RV_SAMPLE_K_BINS;
-  u64 from = 0;
-  const int k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && (uint32_t)k < a.n) from = sample_cutoff(sh, r, 0, (u64)k, false, 0);
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
+  const float mp = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+  uint32_t cnt;
+  if (k > 0 && (uint32_t)k < a.n) {
+    const u64 key = sample_cutoff<THREADS>(sh, r, (u64)k, false, 0, cnt);
+    if (key == 0) {  // no key is: the sign bit of the smallest value is flipped
+      if (r.rank == 0)
+        sample_from_list<THREADS>(sh, r, cnt, (uint32_t)k, p, mp, u, a.tokens + row,
+                                  a.logprobs ? a.logprobs + row : nullptr);
+      cluster_sync_all();  // the others may still read this CTA's shared memory
+      return;
+    }
+    r.keep_from(key);
+  }
   if (p < 1.0f) {
     u64 s = 0;
-    for (uint32_t i = t; i < r.n; i += RV_SAMPLE_THREADS) {
-      const float l = r.at(i);
-      if (sample_key(l, r.i0 + i) >= from) s += r.w(l);
-    }
-    const u64 total = sample_cluster_reduce(sample_reduce(s, sh, add), &sh.sum, r, add);
+    r.each<THREADS>([&](float l, uint32_t i) {
+      if (r.keeps(l, i)) s += r.w(l);
+    });
+    const u64 total = sample_cluster_reduce(sample_reduce<THREADS>(s, sh, add), &sh.sum, r, add);
     const double goal = __dmul_rn((double)p, (double)total);
     if (goal >= 1.0) {
       // The tokens of less than (total - goal) / n each do not amount to what
       // lies beyond the cutoff, so they lie beyond it.
       const u64 g = (u64)goal;
       r.bin_scale = RV_SAMPLE_P_BINS * fminf(r.inv_t, 0x1p40f);
-      from = sample_cutoff(sh, r, from, g, true, (total - g) / a.n);
+      r.keep_from(sample_cutoff<THREADS>(sh, r, g, true, (total - g) / a.n, cnt));
     } else {
-      from = best;
+      cluster_sync_all();  // sh.sum is read by all
+      r.keep_from(first());
     }
   }
-  const float mp = a.min_p ? a.min_p[row] : 0.0f;
   const auto kept = [&](float l, uint32_t i) -> u64 {
-    if (sample_key(l, r.i0 + i) < from) return 0;
+    if (!r.keeps(l, i)) return 0;
     const float e = r.e(l);
     return e >= mp || l == r.top ? sample_weight(e) : 0;
   };
-  // Each warp owns a run of the slice, 32 consecutive tokens at a time.
-  const uint32_t lane = t & 31, warps = RV_SAMPLE_THREADS / 32, per = ((r.n + warps * 32 - 1) / (warps * 32)) * 32,
+  // Each warp owns a run of the slice, 128 consecutive tokens at a time.
+  const uint32_t lane = t & 31, warps = THREADS / 32, per = (r.n + warps * 128 - 1) / (warps * 128) * 128,
                  w0 = min(r.n, (t >> 5) * per), w1 = min(r.n, w0 + per);
   u64 mine = 0;
-  for (uint32_t i = w0 + lane; i < w1; i += 32) mine += kept(r.at(i), i);
+  for (uint32_t i = w0 + 4 * lane; i < w1; i += 128) {
+    const float4 v = *(const float4 *)(s_slice + i);  // the padding weighs nothing
+    mine += kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3);
+  }
   u64 warp_sum = mine;
   for (int o = 16; o; o >>= 1) warp_sum += __shfl_xor_sync(RV_FULL, warp_sum, o);
   __syncthreads();
   if (lane == 0) sh.red[t >> 5] = warp_sum;
   __syncthreads();
-  u64 cta = 0, before = 0;
-  for (uint32_t w = 0; w < warps; w++) {
-    before += w < t >> 5 ? sh.red[w] : 0;
-    cta += sh.red[w];
+  u64 cta = lane < warps ? sh.red[lane] : 0, before = lane < t >> 5 ? cta : 0;
+  for (int o = 16; o; o >>= 1) {
+    cta += __shfl_xor_sync(RV_FULL, cta, o);
+    before += __shfl_xor_sync(RV_FULL, before, o);
   }
-  u64 W = cta;
-  if (r.size > 1) {
-    if (t == 0) sh.pick[3] = cta;
-    cluster_sync_all();
-    u64 c = lane < r.size ? ld_cluster_u64(dsmem_addr(&sh.pick[3], lane)) : 0, lower = lane < r.rank ? c : 0;
-    for (int o = 16; o; o >>= 1) {
-      c += __shfl_xor_sync(RV_FULL, c, o);
-      lower += __shfl_xor_sync(RV_FULL, lower, o);
-    }
-    W = c;
-    before += lower;
+  if (t == 0) sh.pick[3] = cta;
+  cluster_sync_all();
+  u64 W = lane < r.size ? ld_cluster_u64(dsmem_addr(&sh.pick[3], lane)) : 0, lower = lane < r.rank ? W : 0;
+  for (int o = 16; o; o >>= 1) {
+    W += __shfl_xor_sync(RV_FULL, W, o);
+    lower += __shfl_xor_sync(RV_FULL, lower, o);
   }
-  const float u = a.u[row];
+  before += lower;
   u64 target = u > 0.0f ? (u64)__dmul_rn((double)u, (double)W) : 0;  // NaN is 0
   if (target >= W) target = W - 1;
   if (before <= target && target < before + warp_sum) {
-    for (uint32_t b = w0; b < w1; b += 32) {
-      const float l = b + lane < w1 ? r.at(b + lane) : -INFINITY;
-      const u64 w = b + lane < w1 ? kept(l, b + lane) : 0;
-      u64 run = w;
+    // The warp that holds the target: each lane sums a run of the warp's, then
+    // the run that holds it is walked 32 tokens at a time.
+    const auto scan = [&](u64 v) {
       for (int o = 1; o < 32; o <<= 1) {
-        const u64 v = __shfl_up_sync(RV_FULL, run, o);
-        if (lane >= (uint32_t)o) run += v;
+        const u64 x = __shfl_up_sync(RV_FULL, v, o);
+        if (lane >= (uint32_t)o) v += x;
       }
-      const u64 all = __shfl_sync(RV_FULL, run, 31);
-      if (target < before + all) {
-        const int hit = __ffs(__ballot_sync(RV_FULL, target < before + run)) - 1;
-        if ((int)lane == hit) {
+      return v;
+    };
+    const uint32_t run = per / 32, l0 = min(w1, w0 + lane * run), l1 = min(w1, l0 + run);
+    mine = 0;
+    for (uint32_t i = l0; i < l1; i++) mine += kept(s_slice[i], i);
+    u64 upto = before + scan(mine);
+    const int which = __ffs(__ballot_sync(RV_FULL, target < upto)) - 1;
+    before = __shfl_sync(RV_FULL, upto - mine, which);
+    const uint32_t b0 = w0 + which * run, b1 = min(w1, b0 + run);
+    for (uint32_t b = b0; b < b1; b += 32) {
+      const float l = b + lane < b1 ? s_slice[b + lane] : -INFINITY;
+      upto = before + scan(b + lane < b1 ? kept(l, b + lane) : 0);
+      const uint32_t hits = __ballot_sync(RV_FULL, target < upto);
+      if (hits) {
+        if ((int)lane == __ffs(hits) - 1) {
           a.tokens[row] = (int32_t)(r.i0 + b + lane);
           if (a.logprobs)
             a.logprobs[row] = __fsub_rn(sample_z(l, r.top, r.inv_t), (float)log((double)W * 0x1p-40));
         }
         break;
       }
-      before += all;
+      before = __shfl_sync(RV_FULL, upto, 31);
     }
   }
-  if (r.size > 1) cluster_sync_all();  // the others may still read this CTA's sums
+  cluster_sync_all();  // the others may still read this CTA's sums
 }

@@ -89,7 +89,7 @@ def test_sample_refusals(rv, name):
     def call(logits=0x1000, stride=100, rows=2, n=100, u=0x1000, t=None, k=None, p=None, mp=None, tokens=0x1000, lp=None):
         return rv.lib().rv_sample(logits, stride, rows, n, u, t, k, p, mp, tokens, lp, None)
 
-    for bad, kind in ((dict(n=0), "Empty"), (dict(n=1 << 22, stride=1 << 22), "Unimplemented"), (dict(rows=1 << 31), "Unimplemented"),
+    for bad, kind in ((dict(n=0), "Empty"), (dict(n=720897, stride=1 << 22), "Unimplemented"), (dict(rows=1 << 31), "Unimplemented"),
                       (dict(stride=99), "LengthMismatch"), (dict(logits=None), "InvalidArgument"), (dict(u=None), "InvalidArgument"),
                       (dict(tokens=None), "InvalidArgument"), (dict(t=0x1001), "InvalidArgument"), (dict(k=0x1002), "InvalidArgument"),
                       (dict(lp=0x1003), "InvalidArgument")):
