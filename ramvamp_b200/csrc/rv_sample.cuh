@@ -120,6 +120,11 @@ struct SampleRow {
   RV_DEVFN int bin(float l) const {  // monotone: a larger value has no larger bin
     return min((int)fminf((top - l) * bin_scale, (float)RV_SAMPLE_BINS), RV_SAMPLE_BINS - 1);
   }
+  // bin(l) == b, without the conversion.
+  RV_DEVFN bool in_bin(float l, int b) const {
+    const float d = (top - l) * bin_scale;
+    return b == RV_SAMPLE_BINS - 1 ? !(d < (float)b) : d >= (float)b && d < (float)(b + 1);
+  }
   RV_DEVFN void keep_from(u64 key) {
     fv = sample_key_value(key);
     fi = ~(uint32_t)key;
@@ -162,9 +167,11 @@ RV_DEVFN u64 sample_cluster_reduce(u64 v, u64 *slot, const SampleRow &r, F f) {
 }
 
 // The bin where the running total (counts or weights, from bin 0 on) reaches
-// `goal`, and the total before it.  Every CTA gets both.
+// `goal`, and the total before it.  With p >= 0 the goal is first formed: p of
+// all the weight, the bins' and every CTA's sh.sum (what its histogram left
+// out), at least 1.  Every CTA gets all three.
 template <int THREADS>
-RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights, u64 goal, u64 &before) {
+RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights, float p, u64 &goal, u64 &before) {
   const uint32_t t = threadIdx.x;
   cluster_sync_all();  // the histograms are complete
   // Each CTA sums its share of the bins over the cluster (a warp reads
@@ -203,8 +210,13 @@ RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights,
   if ((t & 31) == 31) sh.red[t >> 5] = run;
   __syncthreads();
   // Warp sums: lane w holds warp w's; the sum of those before this warp.
-  u64 lower = (t & 31) < t >> 5 ? sh.red[t & 31] : 0;
-  for (int o = 16; o; o >>= 1) lower += __shfl_xor_sync(RV_FULL, lower, o);
+  u64 total = (t & 31) < THREADS / 32 ? sh.red[t & 31] : 0, lower = (t & 31) < t >> 5 ? total : 0;
+  if (p >= 0.0f && (t & 31) < r.size) total += ld_cluster_u64(dsmem_addr(&sh.sum, t & 31));
+  for (int o = 16; o; o >>= 1) {
+    lower += __shfl_xor_sync(RV_FULL, lower, o);
+    total += __shfl_xor_sync(RV_FULL, total, o);
+  }
+  if (p >= 0.0f) goal = max((u64)__dmul_rn((double)p, (double)total), 1ull);
   run += lower - mine;
   if (run < goal && goal <= run + mine) {
 #pragma unroll
@@ -222,14 +234,21 @@ RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights,
   return (int)sh.pick[0];
 }
 
-// Tokens from the largest on are kept until their number (weights: their weight)
-// reaches `goal`; of the tokens that the row keeps so far, 1 <= goal <= the
-// total.  Every CTA of the cluster gets the last one's key -- or 0 when counts
-// left no more candidates than the list holds: then all of them, `cnt`, are in
-// every CTA's list with their weights.
+// What a cutoff leaves.
+struct SampleCut {
+  u64 key;       // of the last token kept; 0: counts left so few candidates that all are in every CTA's list
+  uint32_t cnt;  // tokens in the list
+  bool sums;     // W and own are known (weights, and the list held its bin)
+  u64 W, own;    // the weight kept, by all CTAs and by this one
+};
+// Tokens from the largest on are kept until their number reaches k (p < 0) or
+// their weight p of the total, of the tokens that the row keeps so far.  Every
+// CTA of the cluster gets the result.
 template <int THREADS>
-RV_DEVFN u64 sample_cutoff(SampleShared &sh, const SampleRow &r, u64 goal, bool weights, u64 least, uint32_t &cnt) {
+RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t k, float p, uint32_t n) {
   const uint32_t t = threadIdx.x;
+  const bool weights = p >= 0.0f;
+  const auto add = [](u64 x, u64 y) { return x + y; };
   cluster_sync_all();  // nobody still reads the histograms of an earlier cutoff
   for (uint32_t b = t; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
   if (t == 0) sh.list_n = 0;
@@ -244,50 +263,76 @@ RV_DEVFN u64 sample_cutoff(SampleShared &sh, const SampleRow &r, u64 goal, bool 
     __syncthreads();
     u64 s = 0;
     for (uint32_t b = t; b < RV_SAMPLE_BINS - 1; b += THREADS) s += sh.hist[0][b];
-    s = sample_reduce<THREADS>(s, sh, [](u64 p, u64 q) { return p + q; });
+    s = sample_reduce<THREADS>(s, sh, add);
     if (t == 0) sh.hist[0][RV_SAMPLE_BINS - 1] = r.n - (uint32_t)s;
   } else {
-    // Tokens of less than `least` weight do not lie at or above the cutoff.
+    // The total is at least 2^40, so the tokens of less than (1 - p) 2^40 / n
+    // each do not amount to what lies beyond the cutoff: they lie beyond it,
+    // and only the total needs them.
+    const u64 least = (u64)(fmax(0.999 - (double)p, 0.0) * 0x1p40 / (double)n);
+    u64 rest = 0;
     r.each<THREADS>([&](float l, uint32_t i) {
       if (!r.keeps(l, i)) return;
       const u64 w = r.w(l);
       if (w >= least) sample_add(sh, r.bin(l), w);
+      else rest += w;
     });
+    rest = sample_reduce<THREADS>(rest, sh, add);
+    if (t == 0) sh.sum = rest;
   }
-  u64 before;
-  const int bin = sample_find_bin<THREADS>(sh, r, weights, goal, before);
+  SampleCut c;
+  u64 goal = k, before;
+  const int bin = sample_find_bin<THREADS>(sh, r, weights, p, goal, before);
   // The bin's tokens -- all up to it, where they are known to fit -- go to the
   // list of every CTA.
   const bool all = !weights && before + sh.part_bin <= RV_SAMPLE_LIST;
   const uint32_t list_n = dsmem_addr(&sh.list_n, 0);
   r.each<THREADS>([&](float l, uint32_t i) {
-    const int b = r.bin(l);
-    if (!(b == bin || (all && b < bin)) || i >= r.n || !r.keeps(l, i)) return;
+    if (!(all ? r.bin(l) <= bin : r.in_bin(l, bin)) || i >= r.n || !r.keeps(l, i)) return;
     const uint32_t at = atom_add_cluster(list_n, 1u);
     if (at < RV_SAMPLE_LIST) {
       const u64 key = sample_key(l, r.i0 + i), w = weights || all ? r.w(l) : 1ull;
-      for (uint32_t c = 0; c < r.size; c++) {
-        st_cluster_u64(dsmem_addr(&sh.list_key[at], c), key);
-        st_cluster_u64(dsmem_addr(&sh.list_w[at], c), w);
+      for (uint32_t cta = 0; cta < r.size; cta++) {
+        st_cluster_u64(dsmem_addr(&sh.list_key[at], cta), key);
+        st_cluster_u64(dsmem_addr(&sh.list_w[at], cta), w);
       }
     }
   });
   cluster_sync_all();
-  cnt = ld_cluster_u32(list_n);
-  if (all) return 0;
-  if (cnt <= RV_SAMPLE_LIST) {
+  c.cnt = ld_cluster_u32(list_n);
+  c.key = 0;
+  c.sums = false;
+  if (all) return c;
+  if (c.cnt <= RV_SAMPLE_LIST) {
     // A warp places a token among the list's; the CTAs share the tokens.
-    for (uint32_t i = (t >> 5) * r.size + r.rank; i < cnt; i += THREADS / 32 * r.size) {
+    for (uint32_t i = (t >> 5) * r.size + r.rank; i < c.cnt; i += THREADS / 32 * r.size) {
       const u64 key = sh.list_key[i];
       u64 sum = 0;
-      for (uint32_t j = t & 31; j < cnt; j += 32) sum += sh.list_key[j] > key ? sh.list_w[j] : 0;
+      for (uint32_t j = t & 31; j < c.cnt; j += 32) sum += sh.list_key[j] > key ? sh.list_w[j] : 0;
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(RV_FULL, sum, o);
       sum += before;
-      if (sum < goal && goal <= sum + sh.list_w[i] && (t & 31) < r.size)
+      if (sum < goal && goal <= sum + sh.list_w[i] && (t & 31) < r.size) {
         st_cluster_u64(dsmem_addr(&sh.pick[2], t & 31), key);
+        st_cluster_u64(dsmem_addr(&sh.pick[3], t & 31), sum + sh.list_w[i]);
+      }
     }
+    // Meanwhile, what this CTA keeps of the bins before.
+    u64 own = 0;
+    if (weights)
+      for (int b = (int)t; b < bin; b += THREADS)
+        own += sh.hist[0][b] + ((u64)sh.hist[1][b] << 14) + ((u64)sh.hist[2][b] << 28);
     cluster_sync_all();
-    return sh.pick[2];
+    c.key = sh.pick[2];
+    c.W = sh.pick[3];
+    c.sums = weights;
+    if (weights) {
+      for (uint32_t i = t; i < c.cnt; i += THREADS) {
+        const uint32_t id = ~(uint32_t)sh.list_key[i];
+        if (sh.list_key[i] >= c.key && id - r.i0 < r.n) own += sh.list_w[i];
+      }
+      c.own = sample_reduce<THREADS>(own, sh, add);
+    }
+    return c;
   }
   // Too many for the list: eight bits of the key at a time, within the bin.
   u64 prefix = 0, above = before;
@@ -296,19 +341,20 @@ RV_DEVFN u64 sample_cutoff(SampleShared &sh, const SampleRow &r, u64 goal, bool 
     for (uint32_t b = t; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
     __syncthreads();
     r.each<THREADS>([&](float l, uint32_t i) {
-      if (r.bin(l) != bin || i >= r.n || !r.keeps(l, i)) return;
+      if (!r.in_bin(l, bin) || i >= r.n || !r.keeps(l, i)) return;
       const u64 key = sample_key(l, r.i0 + i);
       if (shift < 56 && (key >> (shift + 8)) != prefix) return;
       const int d = 255 - (int)((key >> shift) & 255);  // descending
       if (weights) sample_add(sh, d, r.w(l));
       else atomicAdd(&sh.hist[0][d], 1u);
     });
-    u64 sum;
-    const int d = sample_find_bin<THREADS>(sh, r, weights, goal - above, sum);
+    u64 sum, left = goal - above;
+    const int d = sample_find_bin<THREADS>(sh, r, weights, -1.0f, left, sum);
     prefix = prefix << 8 | (u64)(255 - d);
     above += sum;
   }
-  return prefix;
+  c.key = prefix;
+  return c;
 }
 
 // The draw from a list of all candidates (`cnt` of them, more than k only by the
@@ -424,99 +470,101 @@ __global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
   r.inv_t = fmaxf(__fdiv_rn(1.0f, temp), 0x1p-126f);  // so that -infinity times it stays one
   r.bin_scale = RV_SAMPLE_K_BINS;
   const float mp = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-  uint32_t cnt;
+  SampleCut cut;
+  cut.sums = false;
   if (k > 0 && (uint32_t)k < a.n) {
-    const u64 key = sample_cutoff<THREADS>(sh, r, (u64)k, false, 0, cnt);
-    if (key == 0) {  // no key is: the sign bit of the smallest value is flipped
+    cut = sample_cutoff<THREADS>(sh, r, (uint32_t)k, -1.0f, a.n);
+    if (cut.key == 0) {
       if (r.rank == 0)
-        sample_from_list<THREADS>(sh, r, cnt, (uint32_t)k, p, mp, u, a.tokens + row,
+        sample_from_list<THREADS>(sh, r, cut.cnt, (uint32_t)k, p, mp, u, a.tokens + row,
                                   a.logprobs ? a.logprobs + row : nullptr);
       cluster_sync_all();  // the others may still read this CTA's shared memory
       return;
     }
-    r.keep_from(key);
+    r.keep_from(cut.key);
   }
   if (p < 1.0f) {
-    u64 s = 0;
-    r.each<THREADS>([&](float l, uint32_t i) {
-      if (r.keeps(l, i)) s += r.w(l);
-    });
-    const u64 total = sample_cluster_reduce(sample_reduce<THREADS>(s, sh, add), &sh.sum, r, add);
-    const double goal = __dmul_rn((double)p, (double)total);
-    if (goal >= 1.0) {
-      // The tokens of less than (total - goal) / n each do not amount to what
-      // lies beyond the cutoff, so they lie beyond it.
-      const u64 g = (u64)goal;
-      r.bin_scale = RV_SAMPLE_P_BINS * fminf(r.inv_t, 0x1p40f);
-      r.keep_from(sample_cutoff<THREADS>(sh, r, g, true, (total - g) / a.n, cnt));
-    } else {
-      cluster_sync_all();  // sh.sum is read by all
-      r.keep_from(first());
-    }
+    r.bin_scale = RV_SAMPLE_P_BINS * fminf(r.inv_t, 0x1p40f);
+    cut = sample_cutoff<THREADS>(sh, r, 0, fmaxf(p, 0.0f), a.n);
+    r.keep_from(cut.key);
   }
   const auto kept = [&](float l, uint32_t i) -> u64 {
     if (!r.keeps(l, i)) return 0;
     const float e = r.e(l);
     return e >= mp || l == r.top ? sample_weight(e) : 0;
   };
-  // Each warp owns a run of the slice, 128 consecutive tokens at a time.
-  const uint32_t lane = t & 31, warps = THREADS / 32, per = (r.n + warps * 128 - 1) / (warps * 128) * 128,
-                 w0 = min(r.n, (t >> 5) * per), w1 = min(r.n, w0 + per);
-  u64 mine = 0;
-  for (uint32_t i = w0 + 4 * lane; i < w1; i += 128) {
-    const float4 v = *(const float4 *)(s_slice + i);  // the padding weighs nothing
-    mine += kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3);
+  // The kept weight of each block of 128 consecutive tokens, into sh.part.
+  const uint32_t lane = t & 31, blocks = (r.n + 127) / 128;
+  const auto weigh = [&]() {
+    u64 own = 0;
+    for (uint32_t b = t >> 5; b < blocks; b += THREADS / 32) {
+      const uint32_t i = 128 * b + 4 * lane;
+      u64 w = 0;
+      if (i < r.n) {
+        const float4 v = *(const float4 *)(s_slice + i);  // the padding weighs nothing
+        w = kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3);
+      }
+      for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(RV_FULL, w, o);
+      if (lane == 0) sh.part[b] = w;
+      own += w;
+    }
+    return own;  // the warp's blocks
+  };
+  // Without min-p the cutoff by weight knows what each CTA keeps, and only the
+  // CTA that holds the target has to weigh its tokens.
+  const bool known = cut.sums && !(mp > 0.0f);
+  u64 own = cut.own;
+  if (!known) {
+    cluster_sync_all();  // sh.part is read by all in the cutoffs
+    own = weigh();
+    own = sample_reduce<THREADS>(lane == 0 ? own : 0, sh, add);
   }
-  u64 warp_sum = mine;
-  for (int o = 16; o; o >>= 1) warp_sum += __shfl_xor_sync(RV_FULL, warp_sum, o);
-  __syncthreads();
-  if (lane == 0) sh.red[t >> 5] = warp_sum;
-  __syncthreads();
-  u64 cta = lane < warps ? sh.red[lane] : 0, before = lane < t >> 5 ? cta : 0;
-  for (int o = 16; o; o >>= 1) {
-    cta += __shfl_xor_sync(RV_FULL, cta, o);
-    before += __shfl_xor_sync(RV_FULL, before, o);
-  }
-  if (t == 0) sh.pick[3] = cta;
+  if (t == 0) sh.best = own;
   cluster_sync_all();
-  u64 W = lane < r.size ? ld_cluster_u64(dsmem_addr(&sh.pick[3], lane)) : 0, lower = lane < r.rank ? W : 0;
+  u64 W = lane < r.size ? ld_cluster_u64(dsmem_addr(&sh.best, lane)) : 0, before = lane < r.rank ? W : 0;
   for (int o = 16; o; o >>= 1) {
     W += __shfl_xor_sync(RV_FULL, W, o);
-    lower += __shfl_xor_sync(RV_FULL, lower, o);
+    before += __shfl_xor_sync(RV_FULL, before, o);
   }
-  before += lower;
   u64 target = u > 0.0f ? (u64)__dmul_rn((double)u, (double)W) : 0;  // NaN is 0
   if (target >= W) target = W - 1;
-  if (before <= target && target < before + warp_sum) {
-    // The warp that holds the target: each lane sums a run of the warp's, then
-    // the run that holds it is walked 32 tokens at a time.
-    const auto scan = [&](u64 v) {
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 x = __shfl_up_sync(RV_FULL, v, o);
-        if (lane >= (uint32_t)o) v += x;
-      }
-      return v;
-    };
-    const uint32_t run = per / 32, l0 = min(w1, w0 + lane * run), l1 = min(w1, l0 + run);
-    mine = 0;
-    for (uint32_t i = l0; i < l1; i++) mine += kept(s_slice[i], i);
-    u64 upto = before + scan(mine);
-    const int which = __ffs(__ballot_sync(RV_FULL, target < upto)) - 1;
-    before = __shfl_sync(RV_FULL, upto - mine, which);
-    const uint32_t b0 = w0 + which * run, b1 = min(w1, b0 + run);
-    for (uint32_t b = b0; b < b1; b += 32) {
-      const float l = b + lane < b1 ? s_slice[b + lane] : -INFINITY;
-      upto = before + scan(b + lane < b1 ? kept(l, b + lane) : 0);
-      const uint32_t hits = __ballot_sync(RV_FULL, target < upto);
-      if (hits) {
-        if ((int)lane == __ffs(hits) - 1) {
-          a.tokens[row] = (int32_t)(r.i0 + b + lane);
-          if (a.logprobs)
-            a.logprobs[row] = __fsub_rn(sample_z(l, r.top, r.inv_t), (float)log((double)W * 0x1p-40));
+  if (before <= target && target < before + own) {
+    if (known) {
+      weigh();
+      __syncthreads();
+    }
+    if (t < 32) {
+      const auto scan = [&](u64 v) {
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 x = __shfl_up_sync(RV_FULL, v, o);
+          if (lane >= (uint32_t)o) v += x;
+        }
+        return v;
+      };
+      // The block that holds the target, then its tokens four a lane.
+      for (uint32_t b0 = 0; b0 < blocks; b0 += 32) {
+        const u64 v = b0 + lane < blocks ? sh.part[b0 + lane] : 0, upto = before + scan(v);
+        const uint32_t hits = __ballot_sync(RV_FULL, target < upto);
+        if (!hits) {
+          before = __shfl_sync(RV_FULL, upto, 31);
+          continue;
+        }
+        const int which = __ffs(hits) - 1;
+        before = __shfl_sync(RV_FULL, upto - v, which);
+        const uint32_t i = 128 * (b0 + which) + 4 * lane;
+        u64 w[4], sum = 0;
+        for (int j = 0; j < 4; j++) sum += w[j] = i + j < r.n ? kept(s_slice[i + j], i + j) : 0;
+        before += scan(sum) - sum;
+        for (int j = 0; j < 4; j++) {
+          if (before <= target && target < before + w[j]) {
+            a.tokens[row] = (int32_t)(r.i0 + i + j);
+            if (a.logprobs)
+              a.logprobs[row] = __fsub_rn(sample_z(s_slice[i + j], r.top, r.inv_t), (float)log((double)W * 0x1p-40));
+          }
+          before += w[j];
         }
         break;
       }
-      before = __shfl_sync(RV_FULL, upto, 31);
     }
   }
   cluster_sync_all();  // the others may still read this CTA's sums
