@@ -31,7 +31,7 @@
 #define RV_SAMPLE_WARPS 32  // at most
 #define RV_SAMPLE_BINS 1024
 #define RV_SAMPLE_LIST 1024    // tokens of one bin that are ranked directly
-#define RV_SAMPLE_MOST 720896  // logits a row: 16 slices of 176 KB
+#define RV_SAMPLE_MOST 720896  // logits a row: 16 slices of 45,056 (16-bit places)
 #define RV_SAMPLE_K_BINS 32.0f  // top-k's bins per unit of logit
 #define RV_SAMPLE_P_BINS 64.0f  // top-p's per unit of z
 
@@ -76,7 +76,8 @@ struct SampleShared {
   u64 pick[4];            // results one thread hands to the others
   u64 list_key[RV_SAMPLE_LIST];      // also the [CTA][bin] sums of a share of the bins, before the list is filled
   u64 list_w[RV_SAMPLE_LIST];
-  uint32_t list_n;
+  uint32_t list_n, found_n, found_at;  // found: this CTA's tokens for the list
+  uint16_t found[RV_SAMPLE_LIST];
   u64 part_bin;           // the found bin's total
   uint32_t hist[3][RV_SAMPLE_BINS];  // counts, or words of weights, the lowest first
   u64 part[RV_SAMPLE_BINS];          // cluster sums of this CTA's share of the bins
@@ -85,7 +86,7 @@ struct SampleShared {
 RV_DEVFN void sample_add(SampleShared &sh, int b, u64 w) {
   atomicAdd(&sh.hist[0][b], (uint32_t)w & 0x3FFFu);
   atomicAdd(&sh.hist[1][b], (uint32_t)(w >> 14) & 0x3FFFu);
-  atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 28));
+  if (w >> 28) atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 28));  // most weights are below 2^-12
 }
 
 RV_DEVFN u64 ld_cluster_u64(uint32_t a) {
@@ -128,6 +129,27 @@ struct SampleRow {
   RV_DEVFN void keep_from(u64 key) {
     fv = sample_key_value(key);
     fi = ~(uint32_t)key;
+  }
+  // f(value, index) for every token that is kept: 32 tokens a thread are looked
+  // at first, so a warp works on kept tokens only, however few there are.
+  template <int THREADS, typename F>
+  RV_DEVFN void each_kept(F f) const {
+    for (uint32_t base = 0; base < (n + 3) / 4; base += 8 * THREADS) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const uint32_t i = base + j * THREADS + threadIdx.x;
+        if (i < (n + 3) / 4) {
+          const float4 v = ((const float4 *)x)[i];
+          m |= (uint32_t)keeps(v.x, 4 * i) << (4 * j) | (uint32_t)keeps(v.y, 4 * i + 1) << (4 * j + 1) |
+               (uint32_t)keeps(v.z, 4 * i + 2) << (4 * j + 2) | (uint32_t)keeps(v.w, 4 * i + 3) << (4 * j + 3);
+        }
+      }
+      for (; m; m &= m - 1) {
+        const uint32_t b = __ffs(m) - 1, i = 4 * (base + (b >> 2) * THREADS + threadIdx.x) + (b & 3);
+        if (i < n) f(x[i], i);
+      }
+    }
   }
   // f(value, index) for every token of the slice; the padding comes as tokens
   // of -infinity with indexes from n on.
@@ -234,6 +256,12 @@ RV_DEVFN int sample_find_bin(SampleShared &sh, const SampleRow &r, bool weights,
   return (int)sh.pick[0];
 }
 
+template <int THREADS>
+RV_DEVFN void sample_clear(SampleShared &sh) {
+  for (uint32_t b = threadIdx.x; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
+  if (threadIdx.x == 0) sh.list_n = sh.found_n = 0;
+}
+
 // What a cutoff leaves.
 struct SampleCut {
   u64 key;       // of the last token kept; 0: counts left so few candidates that all are in every CTA's list
@@ -243,16 +271,18 @@ struct SampleCut {
 };
 // Tokens from the largest on are kept until their number reaches k (p < 0) or
 // their weight p of the total, of the tokens that the row keeps so far.  Every
-// CTA of the cluster gets the result.
+// CTA of the cluster gets the result.  fresh: the row's first cutoff (the
+// histogram is zero and everything is kept).
 template <int THREADS>
-RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t k, float p, uint32_t n) {
+RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t k, float p, uint32_t n, bool fresh) {
   const uint32_t t = threadIdx.x;
   const bool weights = p >= 0.0f;
   const auto add = [](u64 x, u64 y) { return x + y; };
-  cluster_sync_all();  // nobody still reads the histograms of an earlier cutoff
-  for (uint32_t b = t; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
-  if (t == 0) sh.list_n = 0;
-  __syncthreads();
+  if (!fresh) {
+    cluster_sync_all();  // nobody still reads the histograms of the earlier cutoff
+    sample_clear<THREADS>(sh);
+    __syncthreads();
+  }
   if (!weights) {
     // The last bin holds the far tail, which k seldom reaches: its count is
     // what the others leave.
@@ -271,12 +301,13 @@ RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t 
     // and only the total needs them.
     const u64 least = (u64)(fmax(0.999 - (double)p, 0.0) * 0x1p40 / (double)n);
     u64 rest = 0;
-    r.each<THREADS>([&](float l, uint32_t i) {
-      if (!r.keeps(l, i)) return;
+    const auto put = [&](float l, uint32_t) {
       const u64 w = r.w(l);
       if (w >= least) sample_add(sh, r.bin(l), w);
       else rest += w;
-    });
+    };
+    if (fresh) r.each<THREADS>(put);  // everything is kept; the padding weighs nothing
+    else r.each_kept<THREADS>(put);
     rest = sample_reduce<THREADS>(rest, sh, add);
     if (t == 0) sh.sum = rest;
   }
@@ -284,20 +315,28 @@ RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t 
   u64 goal = k, before;
   const int bin = sample_find_bin<THREADS>(sh, r, weights, p, goal, before);
   // The bin's tokens -- all up to it, where they are known to fit -- go to the
-  // list of every CTA.
+  // list of every CTA: first this CTA's, then one place in the list for all.
   const bool all = !weights && before + sh.part_bin <= RV_SAMPLE_LIST;
   const uint32_t list_n = dsmem_addr(&sh.list_n, 0);
   r.each<THREADS>([&](float l, uint32_t i) {
     if (!(all ? r.bin(l) <= bin : r.in_bin(l, bin)) || i >= r.n || !r.keeps(l, i)) return;
-    const uint32_t at = atom_add_cluster(list_n, 1u);
-    if (at < RV_SAMPLE_LIST) {
-      const u64 key = sample_key(l, r.i0 + i), w = weights || all ? r.w(l) : 1ull;
-      for (uint32_t cta = 0; cta < r.size; cta++) {
-        st_cluster_u64(dsmem_addr(&sh.list_key[at], cta), key);
-        st_cluster_u64(dsmem_addr(&sh.list_w[at], cta), w);
-      }
-    }
+    const uint32_t at = atomicAdd(&sh.found_n, 1u);
+    if (at < RV_SAMPLE_LIST) sh.found[at] = (uint16_t)i;
   });
+  __syncthreads();
+  const uint32_t found = sh.found_n;
+  if (t == 0) sh.found_at = atom_add_cluster(list_n, found);
+  __syncthreads();
+  for (uint32_t j = t; j < min(found, RV_SAMPLE_LIST); j += THREADS) {
+    const uint32_t at = sh.found_at + j, i = sh.found[j];
+    if (at >= RV_SAMPLE_LIST) break;
+    const float l = r.x[i];
+    const u64 key = sample_key(l, r.i0 + i), w = weights || all ? r.w(l) : 1ull;
+    for (uint32_t cta = 0; cta < r.size; cta++) {
+      st_cluster_u64(dsmem_addr(&sh.list_key[at], cta), key);
+      st_cluster_u64(dsmem_addr(&sh.list_w[at], cta), w);
+    }
+  }
   cluster_sync_all();
   c.cnt = ld_cluster_u32(list_n);
   c.key = 0;
@@ -338,7 +377,7 @@ RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t 
   u64 prefix = 0, above = before;
   for (int shift = 56; shift >= 0; shift -= 8) {
     cluster_sync_all();
-    for (uint32_t b = t; b < RV_SAMPLE_BINS; b += THREADS) sh.hist[0][b] = sh.hist[1][b] = sh.hist[2][b] = 0;
+    sample_clear<THREADS>(sh);
     __syncthreads();
     r.each<THREADS>([&](float l, uint32_t i) {
       if (!r.in_bin(l, bin) || i >= r.n || !r.keeps(l, i)) return;
@@ -426,6 +465,7 @@ __global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
   r.n = min(a.n - r.i0, a.slice);
   r.x = s_slice;
   const float *x = a.logits + (size_t)row * a.row_stride + r.i0;
+  sample_clear<THREADS>(sh);
   float top = -INFINITY;
   const uint32_t n4 = ((uintptr_t)x & 15) == 0 ? r.n / 4 : 0;
 #pragma unroll 4
@@ -470,10 +510,11 @@ __global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
   r.inv_t = fmaxf(__fdiv_rn(1.0f, temp), 0x1p-126f);  // so that -infinity times it stays one
   r.bin_scale = RV_SAMPLE_K_BINS;
   const float mp = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+  bool fresh = true;
   SampleCut cut;
   cut.sums = false;
   if (k > 0 && (uint32_t)k < a.n) {
-    cut = sample_cutoff<THREADS>(sh, r, (uint32_t)k, -1.0f, a.n);
+    cut = sample_cutoff<THREADS>(sh, r, (uint32_t)k, -1.0f, a.n, true);
     if (cut.key == 0) {
       if (r.rank == 0)
         sample_from_list<THREADS>(sh, r, cut.cnt, (uint32_t)k, p, mp, u, a.tokens + row,
@@ -482,10 +523,11 @@ __global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
       return;
     }
     r.keep_from(cut.key);
+    fresh = false;
   }
   if (p < 1.0f) {
     r.bin_scale = RV_SAMPLE_P_BINS * fminf(r.inv_t, 0x1p40f);
-    cut = sample_cutoff<THREADS>(sh, r, 0, fmaxf(p, 0.0f), a.n);
+    cut = sample_cutoff<THREADS>(sh, r, 0, fmaxf(p, 0.0f), a.n, fresh);
     r.keep_from(cut.key);
   }
   const auto kept = [&](float l, uint32_t i) -> u64 {
@@ -493,46 +535,63 @@ __global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
     const float e = r.e(l);
     return e >= mp || l == r.top ? sample_weight(e) : 0;
   };
-  // The kept weight of each block of 128 consecutive tokens, into sh.part.
-  const uint32_t lane = t & 31, blocks = (r.n + 127) / 128;
-  const auto weigh = [&]() {
-    u64 own = 0;
-    for (uint32_t b = t >> 5; b < blocks; b += THREADS / 32) {
-      const uint32_t i = 128 * b + 4 * lane;
-      u64 w = 0;
-      if (i < r.n) {
-        const float4 v = *(const float4 *)(s_slice + i);  // the padding weighs nothing
-        w = kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3);
-      }
-      for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(RV_FULL, w, o);
-      if (lane == 0) sh.part[b] = w;
-      own += w;
+  const uint32_t lane = t & 31;
+  // The kept weight of block b of 128 consecutive tokens of CTA c, whose first
+  // index is i0 and length n (its slice is read over the cluster).
+  const auto weigh = [&](uint32_t slice, uint32_t b, uint32_t i0, uint32_t n) {
+    const uint32_t i = 128 * b + 4 * lane;
+    u64 w = 0;
+    if (i < n) {
+      float4 v;
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                   : "r"(slice + 4 * i)
+                   : "memory");
+      const uint32_t at = i0 + i - r.i0;  // kept() adds this CTA's first index
+      w = kept(v.x, at) + kept(v.y, at + 1) + kept(v.z, at + 2) + kept(v.w, at + 3);  // the padding weighs nothing
     }
-    return own;  // the warp's blocks
+    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(RV_FULL, w, o);
+    return w;
   };
   // Without min-p the cutoff by weight knows what each CTA keeps, and only the
-  // CTA that holds the target has to weigh its tokens.
+  // slice that holds the target is weighed, by all CTAs of the cluster.
   const bool known = cut.sums && !(mp > 0.0f);
   u64 own = cut.own;
   if (!known) {
     cluster_sync_all();  // sh.part is read by all in the cutoffs
-    own = weigh();
-    own = sample_reduce<THREADS>(lane == 0 ? own : 0, sh, add);
+    own = 0;
+    for (uint32_t b = t >> 5; b < (r.n + 127) / 128; b += THREADS / 32) {
+      const u64 w = weigh(smem_addr(s_slice), b, r.i0, r.n);
+      if (lane == 0) {
+        sh.part[b] = w;
+        own += w;
+      }
+    }
+    own = sample_reduce<THREADS>(own, sh, add);
   }
   if (t == 0) sh.best = own;
   cluster_sync_all();
-  u64 W = lane < r.size ? ld_cluster_u64(dsmem_addr(&sh.best, lane)) : 0, before = lane < r.rank ? W : 0;
-  for (int o = 16; o; o >>= 1) {
-    W += __shfl_xor_sync(RV_FULL, W, o);
-    before += __shfl_xor_sync(RV_FULL, before, o);
+  const u64 mine = lane < r.size ? ld_cluster_u64(dsmem_addr(&sh.best, lane)) : 0;
+  u64 upto = mine;  // the kept weight up to each CTA's end
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 v = __shfl_up_sync(RV_FULL, upto, o);
+    if (lane >= (uint32_t)o) upto += v;
   }
+  const u64 W = __shfl_sync(RV_FULL, upto, 31);
   u64 target = u > 0.0f ? (u64)__dmul_rn((double)u, (double)W) : 0;  // NaN is 0
   if (target >= W) target = W - 1;
-  if (before <= target && target < before + own) {
-    if (known) {
-      weigh();
-      __syncthreads();
+  const int where = __ffs(__ballot_sync(RV_FULL, target < upto)) - 1;
+  u64 before = __shfl_sync(RV_FULL, upto - mine, where);
+  const uint32_t i0 = min(a.n, (uint32_t)where * a.slice), blocks = (min(a.n - i0, a.slice) + 127) / 128;
+  if (known) {
+    const uint32_t slice = dsmem_addr(s_slice, where), part = dsmem_addr(sh.part, where);
+    for (uint32_t b = (t >> 5) * r.size + r.rank; b < blocks; b += THREADS / 32 * r.size) {
+      const u64 w = weigh(slice, b, i0, min(a.n - i0, a.slice));
+      if (lane == 0) st_cluster_u64(part + 8 * b, w);
     }
+    cluster_sync_all();
+  }
+  if ((uint32_t)where == r.rank) {
     if (t < 32) {
       const auto scan = [&](u64 v) {
         for (int o = 1; o < 32; o <<= 1) {
@@ -543,14 +602,14 @@ __global__ void __launch_bounds__(THREADS) k_sample(SampleArgs a) {
       };
       // The block that holds the target, then its tokens four a lane.
       for (uint32_t b0 = 0; b0 < blocks; b0 += 32) {
-        const u64 v = b0 + lane < blocks ? sh.part[b0 + lane] : 0, upto = before + scan(v);
-        const uint32_t hits = __ballot_sync(RV_FULL, target < upto);
+        const u64 v = b0 + lane < blocks ? sh.part[b0 + lane] : 0, end = before + scan(v);
+        const uint32_t hits = __ballot_sync(RV_FULL, target < end);
         if (!hits) {
-          before = __shfl_sync(RV_FULL, upto, 31);
+          before = __shfl_sync(RV_FULL, end, 31);
           continue;
         }
         const int which = __ffs(hits) - 1;
-        before = __shfl_sync(RV_FULL, upto - v, which);
+        before = __shfl_sync(RV_FULL, end - v, which);
         const uint32_t i = 128 * (b0 + which) + 4 * lane;
         u64 w[4], sum = 0;
         for (int j = 0; j < 4; j++) sum += w[j] = i + j < r.n ? kept(s_slice[i + j], i + j) : 0;
