@@ -689,42 +689,108 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       const uint32_t idesc_s = tc_idesc(RV_PFX_N), idesc_o = tc_idesc(D) | (1u << 16);  // B of P V: keys down the rows
       auto mk = [](uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; };
       int at[2] = {0, 0}, j[2] = {0, 0}, len[2], nk = 0, nv = 0;
-      // One batch of products: S = Q K^T of a stream.
+      // One batch of products, by one thread: S = Q K^T of stream s from the
+      // ring's slot.
       auto issue_qk = [&](int s, int slot) {
-        const uint32_t qa = q_lo + s * (C::QS >> 4), kb = ring_lo + (uint32_t)(slot * (TILE >> 4));
+        const uint32_t qa = q_lo + s * (C::QS >> 4), kb = ring_lo + (uint32_t)(slot * (TILE >> 4)), d = tmem + 128 * s;
 #pragma unroll
         for (int kk = 0; kk < D / 16; kk++) {
           const uint32_t oq = (uint32_t)(kk >> 2) * (C::SR * 128 >> 4) + 2 * (kk & 3),
                          okk = (uint32_t)(kk >> 2) * (RV_PFX_N * 128 >> 4) + 2 * (kk & 3);
-          tc_mma_f16(tmem + 128 * s, mk(lbo_k | (qa + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, kk != 0);
+          tc_mma_f16(d, mk(lbo_k | (qa + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, kk != 0);
           if (PRECISE)
-            tc_mma_f16(tmem + 128 * s, mk(lbo_k | (qa + (C::QT >> 4) + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw),
-                       idesc_s, 1u);
+            tc_mma_f16(d, mk(lbo_k | (qa + (C::QT >> 4) + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, 1u);
         }
         tc_commit(&s_full[s]);
-        if (!pair || s) tc_commit(&kv_empty[slot]);  // released by its last reader
       };
+      // O (+)= P V of stream s over `steps` times 16 keys.
+      auto issue_pv = [&](int s, int slot, int steps, bool add) {
+        const uint32_t vb = ring_lo + (uint32_t)(slot * (TILE >> 4)), p0 = tmem + 128 * s, d = p0 + RV_PFX_O;
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++) {
+          if (kk < steps) {
+            const uint32_t pa = p0 + 32 * (kk >> 1) + 8 * (kk & 1);
+            const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
+            tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || add);
+            if (PRECISE) tc_mma_f16_ta(d, pa + 16, bd, idesc_o, 1u);
+          }
+        }
+      };
+      if (pair) {
+        // One thread runs the whole role: the streams are in step, so there is
+        // one count of everything, and few instructions stand between the
+        // batches (this warp shares its scheduler with two softmax warps).
+        if (elect_one()) {
+          const auto full = [&](int i) { return mbar_wait_bounded(&kv_full[i % R], (i / R) & 1); };
+          for (int e = 0; ok && e < count[0]; e++) {
+            const PfxPiece *p = &tab[0][e];
+            const int units = p->n;
+            const int last = min(RV_PFX_N, p->keys - (p->tile0 + units - 1) * RV_PFX_N);
+            ok = mbar_wait_bounded(&q_ready[0], nq[0] & 1) && mbar_wait_bounded(&q_ready[1], nq[0] & 1);
+            nq[0]++;
+            nk = n++;
+            ok = ok && full(nk);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int s = 0; s < 2; s++) issue_qk(s, nk % R);
+            tc_commit(&kv_empty[nk % R]);
+            for (int u = 0; ok && u < units; u++) {
+              const bool more = u + 1 < units;
+              const int steps = more ? 8 : (last + 15) >> 4;
+              nv = n++;
+              ok = full(nv);
+              if (more) {
+                nk = n++;
+                ok = ok && full(nk);
+              }
+#pragma unroll 1
+              for (int s = 0; ok && s < 2; s++) {
+                ok = mbar_wait_bounded(&p_ready[s], np[0] & 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(s, nv % R, steps, u != 0);
+                if (more) issue_qk(s, nk % R);
+                else tc_commit(&o_full[s]);
+              }
+              np[0]++;
+              tc_commit(&kv_empty[nv % R]);
+              if (more) tc_commit(&kv_empty[nk % R]);
+            }
+          }
+          if (!ok) *s_fail = 1;
+        }
+        __syncwarp();
+        // The counts go on with the other lanes too, should another lane be
+        // elected in the next plan.
+        n = __reduce_max_sync(RV_FULL, n);
+        np[0] = __reduce_max_sync(RV_FULL, np[0]);
+        nq[0] = __reduce_max_sync(RV_FULL, nq[0]);
+      } else {
       auto wait_full = [&](int i) { return pfx_wait(&kv_full[i % R], (i / R) & 1); };
       // A new piece's first S.
       auto start = [&](int s) {
-        pfx_entry(tab[pair ? 0 : s], count[pair ? 0 : s], at[s], len[s]);
+        pfx_entry(tab[s], count[s], at[s], len[s]);
         j[s] = 0;
         if (!len[s]) return;
         ok = pfx_wait(&q_ready[s], nq[s] & 1);
         nq[s]++;
-        if (!(pair && s)) nk = n++;
+        nk = n++;
         ok = ok && wait_full(nk);
         tc_fence_after();
-        if (ok && elect_one()) issue_qk(s, nk % R);
+        if (ok && elect_one()) {
+          issue_qk(s, nk % R);
+          tc_commit(&kv_empty[nk % R]);
+        }
         __syncwarp();
       };
       // O += P V of a stream's unit and the next S of the same piece, in one go.
       auto turn = [&](int s) {
         if (!ok || !len[s]) return;
-        const PfxPiece &p = tab[pair ? 0 : s][at[s]];
+        const PfxPiece &p = tab[s][at[s]];
         const int valid = min(RV_PFX_N, p.keys - (p.tile0 + j[s]) * RV_PFX_N), steps = (valid + 15) >> 4;
         const bool more = j[s] + 1 < len[s];
-        if (!(pair && s)) nv = n++;
+        nv = n++;
         ok = wait_full(nv);
         if (!Q8 && (p.head & 1) && (valid & 15)) {
           // Rows past the sequence's end hold whatever the cache held: zero
@@ -738,7 +804,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
           __syncwarp();
         }
         if (more) {
-          if (!(pair && s)) nk = n++;
+          nk = n++;
           ok = ok && wait_full(nk);
         }
         ok = ok && pfx_wait(&p_ready[s], np[s] & 1);
@@ -746,19 +812,11 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t vb = ring_lo + (uint32_t)(nv % R * (TILE >> 4)), d = tmem + RV_PFX_O + 128 * s;
-#pragma unroll
-          for (int kk = 0; kk < 8; kk++) {
-            if (kk < steps) {
-              const uint32_t pa = tmem + 128 * s + 32 * (kk >> 1) + 8 * (kk & 1);
-              const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
-              tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || j[s] != 0);
-              if (PRECISE) tc_mma_f16_ta(d, pa + 16, bd, idesc_o, 1u);
-            }
-          }
+          issue_pv(s, nv % R, steps, j[s] != 0);
           if (more) issue_qk(s, nk % R);
           else tc_commit(&o_full[s]);
-          if (!pair || s) tc_commit(&kv_empty[nv % R]);
+          tc_commit(&kv_empty[nv % R]);
+          if (more) tc_commit(&kv_empty[nk % R]);
         }
         __syncwarp();
         j[s]++;
@@ -773,9 +831,10 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         turn(0);
         turn(1);
       }
+      }
       if (!ok) *s_fail = 1;
       if (*s_fail) {  // products in flight end before tensor memory is freed
-        if (lane == 0) {
+        if (elect_one()) {
           tc_commit(drained);
           mbar_wait_bounded(drained, 0);
         }
