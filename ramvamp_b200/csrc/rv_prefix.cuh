@@ -135,9 +135,10 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 // the reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
 // normal f16 down to 2^-21 of the largest.
 //
-// 8-bit cache: levels are exact in f16, so the products run on levels.  With
-// sk and sv the tokens' scales, t = s * sk + log2(sv): P = 2^(t - m) already
-// holds sv, and l adds P / sv.
+// 8-bit cache: levels are exact in f16, so the products run on levels; a token's
+// key scale multiplies its score and its value scale its weight, both in f32.
+// With 2^ev above the tile's largest value scale the reference is m + ev, so
+// that P, which holds the value scale, stays in the range above.
 #define RV_PFX_CTAS 148       // CTAs at most: one per SM of a B200
 #define RV_PFX_THREADS 384    // loads, products and conversion; two softmax warpgroups
 #define RV_PFX_CONV 96        // threads that turn 8-bit rows into f16 (warps 0, 2, 3)
@@ -147,6 +148,7 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 #define RV_PFX_LAG 8.0f       // the reference maximum may lag by this (log2)
 #define RV_PFX_LIFT 7.0f      // P is lifted by 2^7
 #define RV_PFX_SCALE_SLOTS 8  // tiles a stream whose token scales are in shared memory
+#define RV_PFX_SCALE (2 * RV_PFX_N + 4)  // floats of a tile's scales: keys', values', the values' largest by warp
 #define RV_PFX_TABLE 32       // pieces a stream works through between plans
 #define RV_PFX_O 256          // first tensor-memory column of O (S and P: 0..255)
 
@@ -179,10 +181,11 @@ RV_DEVFN PfxLine pfx_line(const PrefixArgs &a, const PfxWork &w, int tiles, int 
   l.solo_p = w.pair || w.tp == 0 ? 0 : seg_p * (w.tp + RV_PFX_OV);
   l.wp = w.pair ? seg_p * w.tp : 0;
   l.w = l.solo_p + suffix;
-  // A paired unit costs a CTA about what two solo units (one a stream) do.
+  // A paired unit costs a CTA about 1.5 solo places (measured: 5.1 and 3.4
+  // thousand cycles).
   l.gp = 0;
   if (l.wp) {
-    const long long cost = 2ll * l.wp, both = cost + l.w;
+    const long long cost = 3ll * l.wp, both = cost + 2ll * l.w;
     l.gp = min(max((int)((cost * w.grid + both / 2) / both), 1), l.w ? w.grid - 1 : w.grid);
   }
   l.per_p = l.gp ? (l.wp + l.gp - 1) / l.gp : 1;
@@ -215,10 +218,11 @@ struct PfxCfg {
   static constexpr int QT = SR * D * 2;                         // bytes of one query operand
   static constexpr int QS = QT * (PRECISE ? 2 : 1);             // of a stream's
   static constexpr int TILE = RV_PFX_N * D * 2;                 // of a K or V tile
-  static constexpr int R = D == 64 ? 8 : Q8 ? 4 : 5;            // K/V ring stages
-  static constexpr int SCALES = Q8 ? 2 * RV_PFX_SCALE_SLOTS * 3 * RV_PFX_N * 4 : 0;
+  static constexpr int R = D == 64 ? (Q8 ? 6 : 8) : Q8 ? 3 : 5;  // K/V ring stages
+  static constexpr int RAW = Q8 ? 2 * RV_PFX_N * D : 0;         // two tiles of levels on their way
+  static constexpr int SCALES = Q8 ? 2 * RV_PFX_SCALE_SLOTS * RV_PFX_SCALE * 4 : 0;
   static constexpr int NBARS = 2 * R + 8 + 2 * RV_PFX_SCALE_SLOTS + 1;
-  static constexpr size_t ring = 2 * QS, scales = ring + (size_t)R * TILE, table = scales + SCALES,
+  static constexpr size_t ring = 2 * QS, raw = ring + (size_t)R * TILE, scales = raw + RAW, table = scales + SCALES,
                           ups = table + 2 * RV_PFX_TABLE * sizeof(PfxPiece), bars = ups + (PRECISE ? 4 * SR : 0);
   static constexpr size_t total = bars + NBARS * 8 + 48 * 4;
   static_assert(total <= 227 * 1024, "shared memory of a CTA");
@@ -228,7 +232,9 @@ struct PfxCfg {
 // them in: K of each stream's first unit, then in turn for each stream V of its
 // unit and K of its next.  Paired streams use the same tiles: one stream here.
 struct PfxFeed {
-  int i[2], j[2], n[2], unit[2];  // entry, tile of it, its tiles (0: the stream has ended), units so far
+  // Per stream: table entry, tile of it, its tiles (0: the stream has ended),
+  // units so far.  Indexed by constants, so they stay in registers.
+  int i[2], j[2], n[2], unit[2];
   int boot, turn;
   bool want_k;
   // The current load.
@@ -239,45 +245,55 @@ RV_DEVFN void pfx_entry(const PfxPiece *tab, int count, int &i, int &n) {
   for (n = 0; i < count; i++)
     if ((n = tab[i].n) > 0) return;
 }
+RV_DEVFN void pfx_feed_start(PfxFeed &f) {
+  f.boot = f.turn = 0;
+  f.want_k = false;
+  f.n[0] = f.n[1] = 0;
+}
 RV_DEVFN bool pfx_feed(const PfxPiece (*tab)[RV_PFX_TABLE], const int (&count)[2], int ns, PfxFeed &f) {
-  for (;;) {
-    int s;
-    if (f.boot < ns) {
-      s = f.boot++;
-      f.i[s] = f.j[s] = 0;
-      pfx_entry(tab[s], count[s], f.i[s], f.n[s]);
-      if (!f.n[s]) continue;
-      f.is_k = true;
-    } else if (f.want_k) {
-      f.want_k = false;
-      s = f.turn;
-      f.turn = ns == 2 ? s ^ 1 : 0;
-      if (!f.n[s]) continue;
-      f.is_k = true;
-    } else {
-      if (!f.n[0] && !f.n[1]) return false;
-      s = f.turn;
-      if (!f.n[s]) {
-        f.turn = s ^ 1;
-        continue;
+  int s = -1;
+  if (f.boot < ns) {  // K of the streams' first units
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+      if (s < 0 && k >= f.boot && k < ns) {
+        f.boot = k + 1;
+        f.i[k] = f.j[k] = 0;
+        pfx_entry(tab[k], count[k], f.i[k], f.n[k]);
+        if (f.n[k]) s = k;
       }
-      f.is_k = false;
-      f.want_k = true;
-    }
-    f.s = s;
-    f.entry = f.i[s];
-    f.tile = tab[s][f.i[s]].tile0 + f.j[s];
-    f.u = f.unit[s];
-    if (!f.is_k) {
-      f.unit[s]++;
-      if (++f.j[s] == f.n[s]) {
-        f.j[s] = 0;
-        f.i[s]++;
-        pfx_entry(tab[s], count[s], f.i[s], f.n[s]);
-      }
-    }
-    return true;
+    f.is_k = true;
   }
+  if (s < 0 && f.want_k) {  // K of the unit after the V just loaded
+    f.want_k = false;
+    f.is_k = true;
+    const int k = f.turn;
+    f.turn = ns == 2 ? k ^ 1 : 0;
+    if (k ? f.n[1] : f.n[0]) s = k;
+  }
+  if (s < 0) {  // V of the next stream in turn that goes on
+    if (!f.n[0] && !f.n[1]) return false;
+    if (!(f.turn ? f.n[1] : f.n[0])) f.turn ^= 1;
+    s = f.turn;
+    f.is_k = false;
+    f.want_k = true;
+  }
+  f.s = s;
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+    if (s == k) {
+      f.entry = f.i[k];
+      f.tile = tab[k][f.i[k]].tile0 + f.j[k];
+      f.u = f.unit[k];
+      if (!f.is_k) {
+        f.unit[k]++;
+        if (++f.j[k] == f.n[k]) {
+          f.j[k] = 0;
+          f.i[k]++;
+          pfx_entry(tab[k], count[k], f.i[k], f.n[k]);
+        }
+      }
+    }
+  return true;
 }
 
 RV_DEVFN float ex2(float x) {
@@ -320,15 +336,13 @@ RV_DEVFN void tc_ld_wait(uint32_t taddr, uint32_t (&v)[64]) {
       : "r"(taddr)
       : "memory");
 }
-RV_DEVFN void tc_ld_wait(uint32_t taddr, uint32_t (&v)[32]) {
+RV_DEVFN void tc_ld_wait(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n"
       " tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr)
       : "memory");
 }
@@ -479,7 +493,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
   constexpr int R = C::R, TILE = C::TILE, SLOTS = RV_PFX_SCALE_SLOTS;
   extern __shared__ __align__(1024) uint8_t sm[];  // the operand tiles are whole swizzle atoms
   uint8_t *ring = sm + C::ring;
-  float *s_scale = (float *)(sm + C::scales);  // [stream][slot][ck, lv, 1 / sv][128]
+  float *s_scale = (float *)(sm + C::scales);  // [stream][slot][RV_PFX_SCALE]
   PfxPiece(*tab)[RV_PFX_TABLE] = (PfxPiece(*)[RV_PFX_TABLE])(sm + C::table);
   int8_t *s_up = (int8_t *)(sm + C::ups);  // [stream][piece & 1][SR] exponents of f32 query rows
   uint64_t *bars = (uint64_t *)(sm + C::bars);
@@ -493,15 +507,6 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
   if (smem_addr(sm) & 1023) {
     rv_dev_fail(RV_ERR_CUDA);
     return;
-  }
-  // Tiles of a run of sequences, and how many have any.
-  const int run = ((int)a.n_seqs + RV_PFX_THREADS - 1) / RV_PFX_THREADS;
-  const int b0 = min((int)threadIdx.x * run, (int)a.n_seqs), b1 = min(b0 + run, (int)a.n_seqs);
-  int mine = 0, filled = 0;
-  for (int b = b0; b < b1; b++) {
-    const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
-    mine += t;
-    filled += t != 0;
   }
   if (threadIdx.x == 32) {
     for (int i = 0; i < R; i++) {
@@ -518,11 +523,27 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       for (int i = 0; i < 2 * SLOTS; i++) mbar_init(&sc_full[i], RV_PFX_CONV / 32);
     mbar_init(drained, 1);
     *s_fail = 0;
-    for (int i = 32; i < 36; i++) s_scan[i] = i & 1 ? -1 : 0;
   }
   if (warp == 0) {
     tc_alloc(s_tmem, 512);
     tc_relinquish();
+  }
+  // Counters that run on over the plans (each role uses its own).
+  int n = 0, np[2] = {0, 0}, nq[2] = {0, 0}, unit = 0, piece = 0;
+  bool ok = true;
+  PfxFeed feed{};
+  for (int base = 0;; base += RV_PFX_TABLE) {
+  // ------------------------------------------------ the next pieces
+  // (Planned from the lengths each time, so that nothing of it stays in
+  // registers while the roles run.)
+  // Tiles of a run of sequences, and how many have any.
+  const int run = ((int)a.n_seqs + RV_PFX_THREADS - 1) / RV_PFX_THREADS;
+  const int b0 = min((int)threadIdx.x * run, (int)a.n_seqs), b1 = min(b0 + run, (int)a.n_seqs);
+  int mine = 0, filled = 0;
+  for (int b = b0; b < b1; b++) {
+    const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
+    mine += t;
+    filled += t != 0;
   }
   int before = mine, fbefore = filled;
   for (int o = 1; o < 32; o <<= 1) {
@@ -536,10 +557,10 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     s_scan[warp] = before;
     s_scan[16 + warp] = fbefore;
   }
+  if (threadIdx.x < 4) s_scan[32 + threadIdx.x] = threadIdx.x & 1 ? -1 : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *s_tmem;
   int all = 0, fall = 0;
 #pragma unroll
   for (int i = 0; i < RV_PFX_THREADS / 32; i++) {
@@ -568,7 +589,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     k.u = min(end, k.v * per);
     k.end = min(end, k.u + per);
   }
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && base == 0) {
     int x = before, f = fbefore;
     for (int b = b0; b < b1; b++) {
       w.cum[b] = x;
@@ -604,12 +625,6 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     k.g0 = k.u < lim ? k.u / len_p : s_scan[32 + 2 * s];
     k.g1 = k.u >= k.end ? k.g0 - 1 : k.end - 1 < lim ? (k.end - 1) / len_p : s_scan[33 + 2 * s];
   }
-  // Counters that run on over the plans (each role uses its own).
-  int n = 0, np[2] = {0, 0}, nq[2] = {0, 0}, unit = 0, piece = 0;
-  bool ok = true;
-  PfxFeed feed{};
-  for (int base = 0;; base += RV_PFX_TABLE) {
-  // ------------------------------------------------ the next pieces
   int count[2];
 #pragma unroll
   for (int s = 0; s < 2; s++) count[s] = min(max(str[s].g1 - str[s].g0 + 1 - base, 0), RV_PFX_TABLE);
@@ -637,7 +652,8 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         const PfxStretch &k = str[s];
-        const int g = seg_p + b * segs, lo = max(0, k.g0 + base - g), hi = min(segs - 1, min(k.g1, k.g0 + base + RV_PFX_TABLE - 1) - g);
+        const int g = seg_p + b * segs, lo = max(0, k.g0 + base - g),
+                  hi = min(segs - 1, min(k.g1, k.g0 + base + RV_PFX_TABLE - 1) - g);
         if (t)
           for (int local = lo; local <= hi; local++) {
             PfxPiece p{};
@@ -656,13 +672,12 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     __syncthreads();
   }
 
+  const uint32_t tmem = *s_tmem;
   if (warp < 4) {
     if (!Q8 && warp == 0 && lane == 0) {
       // ---------------------------------------------------------- loads
       PfxFeed &f = feed;
-      f.boot = f.turn = 0;
-      f.want_k = false;
-      f.n[0] = f.n[1] = 0;
+      pfx_feed_start(f);
       for (; ok && !*s_fail && pfx_feed(tab, count, pair ? 1 : 2, f); n++) {
         const int slot = n % R;
         if (!mbar_wait_bounded(&kv_empty[slot], ((n / R) & 1) ^ 1)) {
@@ -842,69 +857,89 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       }
     } else if (Q8) {
       // ---------------------------------- 8-bit rows into f16 operands
-      // 16 levels a load, D / 16 loads a token.  The next tile's levels are in
-      // registers before its stage is free.
+      // 16 levels a load, D / 16 loads a token.  The next tile's levels are
+      // copied to shared memory while this one's are converted; every thread
+      // converts what it copied.
       constexpr int TPT = D / 16, LOADS = RV_PFX_N * TPT, IT = (LOADS + RV_PFX_CONV - 1) / RV_PFX_CONV;
       const int ct = (warp == 0 ? 0 : 32 * (warp - 1)) + lane;
       PfxFeed &f = feed;
-      f.boot = f.turn = 0;
-      f.want_k = false;
-      f.n[0] = f.n[1] = 0;
-      for (; ok && !*s_fail && pfx_feed(tab, count, pair ? 1 : 2, f); n++) {
+      pfx_feed_start(f);
+      // A tile on its way: its scales in registers.
+      struct Load {
+        float ks[2], vs[2];
+        int at;  // scale slot of a K tile, -1: a V tile
+      } cur, nxt;
+      uint8_t *raw = sm + C::raw;
+      const auto fetch = [&](Load &o, int half) {
+        if (!pfx_feed(tab, count, pair ? 1 : 2, f)) return false;
         const PfxPiece &p = tab[f.s][f.entry];
         const bool suffix = p.head & 1;
-        const int kvh = p.head >> 1, slot = n % R, valid = min(RV_PFX_N, p.keys - f.tile * RV_PFX_N);
+        const int kvh = p.head >> 1, valid = min(RV_PFX_N, p.keys - f.tile * RV_PFX_N);
         const size_t first = (size_t)p.b * a.cap * suffix + (size_t)f.tile * RV_PFX_N;
-        const int8_t *src = (const int8_t *)(f.is_k ? (suffix ? a.sk : a.pk) : (suffix ? a.sv : a.pv));
-        uint4 x[IT];
+        const int8_t *src = (const int8_t *)(f.is_k ? (suffix ? a.sk : a.pk) : (suffix ? a.sv : a.pv)) +
+                            (first * a.n_kv + kvh) * D;
+        const size_t pitch = (size_t)a.n_kv * D;
 #pragma unroll
         for (int j = 0; j < IT; j++) {
           const int id = j * RV_PFX_CONV + ct, tok = id / TPT;
-          x[j] = tok < valid ? __ldg((const uint4 *)(src + ((first + tok) * a.n_kv + kvh) * D + (id % TPT) * 16))
-                             : make_uint4(0, 0, 0, 0);
+          if (tok < RV_PFX_N)  // tokens past the end read as zeros
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(raw + half + 16 * id)),
+                         "l"(tok < valid ? src + tok * pitch + (id % TPT) * 16 : src), "r"(tok < valid ? 16 : 0)
+                         : "memory");
         }
-        float ks[2] = {0, 0}, vs[2] = {0, 0};
-        if (f.is_k) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        o.at = f.is_k ? f.s * SLOTS + f.u % SLOTS : -1;
 #pragma unroll
-          for (int j = 0; j < 2; j++)
-            if (ct + j * RV_PFX_CONV < valid) {
-              const size_t at = (first + ct + j * RV_PFX_CONV) * a.n_kv + kvh;
-              ks[j] = (suffix ? a.sks : a.pks)[at];
-              vs[j] = (suffix ? a.svs : a.pvs)[at];
-            }
+        for (int j = 0; j < 2; j++) {
+          o.ks[j] = o.vs[j] = 0;
+          if (f.is_k && ct + j * RV_PFX_CONV < valid) {
+            const size_t at = (first + ct + j * RV_PFX_CONV) * a.n_kv + kvh;
+            o.ks[j] = (suffix ? a.sks : a.pks)[at];
+            o.vs[j] = (suffix ? a.svs : a.pvs)[at];
+          }
         }
+        return true;
+      };
+      int half = 0;
+      bool any = fetch(cur, 0);
+      for (; ok && any && !*s_fail; n++) {
+        any = fetch(nxt, half ^ RV_PFX_N * D);  // in flight while this tile is converted
+        if (any) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        const int slot = n % R;
         ok = pfx_wait(&kv_empty[slot], ((n / R) & 1) ^ 1);
         if (!ok) break;
-        if (f.is_k) {
-          const int at = f.s * SLOTS + f.u % SLOTS;
-          float *sc = s_scale + (size_t)at * 3 * RV_PFX_N;
+        if (cur.at >= 0) {
+          float *sc = s_scale + cur.at * RV_PFX_SCALE, top = 0;
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const int tok = ct + j * RV_PFX_CONV;
-            // A scale of 0 stands for a row of zeros: any scale does.  One
-            // that is not finite makes the weight NaN by itself, and its
-            // reciprocal must not: rows that do not see the token multiply it
-            // by 0.
-            const float v1 = vs[j] < 0x1p-60f ? 0x1p-60f : vs[j], r1 = __frcp_rn(v1);
+            // A value scale that is not finite makes the token's weight NaN
+            // through its key scale; as a factor it is 0, for the rows that do
+            // not see the token.
+            const bool fine = cur.vs[j] < INFINITY;
             if (tok < RV_PFX_N) {
-              sc[tok] = ks[j] * fabsf(a.scale_log2);
-              sc[RV_PFX_N + tok] = log2f(v1);
-              sc[2 * RV_PFX_N + tok] = r1 > 0.0f ? r1 : 1.0f;
+              sc[tok] = fine ? cur.ks[j] * fabsf(a.scale_log2) : __uint_as_float(0x7FC00000u);
+              sc[RV_PFX_N + tok] = fine ? cur.vs[j] : 0.0f;
             }
+            if (fine) top = fmaxf(top, cur.vs[j]);
           }
+          for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(RV_FULL, top, o));
+          if (lane == 0) sc[2 * RV_PFX_N + ct / 32] = top;
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sc_full[at]);
+          if (lane == 0) mbar_arrive(&sc_full[cur.at]);
         }
         uint8_t *dst = ring + (size_t)slot * TILE;
 #pragma unroll
         for (int j = 0; j < IT; j++) {
           const int id = j * RV_PFX_CONV + ct, tok = id / TPT, ch = (id % TPT) * 2;
-          uint32_t o[8];
-          pfx_levels(x[j].x, o[0], o[1]);
-          pfx_levels(x[j].y, o[2], o[3]);
-          pfx_levels(x[j].z, o[4], o[5]);
-          pfx_levels(x[j].w, o[6], o[7]);
           if (tok < RV_PFX_N) {
+            const uint4 x = *(const uint4 *)(raw + half + 16 * id);
+            uint32_t o[8];
+            pfx_levels(x.x, o[0], o[1]);
+            pfx_levels(x.y, o[2], o[3]);
+            pfx_levels(x.z, o[4], o[5]);
+            pfx_levels(x.w, o[6], o[7]);
             uint8_t *d = dst + (ch >> 3) * (RV_PFX_N * 128);
             *(uint4 *)(d + tc_sw_off(tok, ch & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
             *(uint4 *)(d + tc_sw_off(tok, (ch & 7) + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -913,7 +948,10 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kv_full[slot]);
+        cur = nxt;
+        half ^= RV_PFX_N * D;
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       if (!ok) *s_fail = 1;
     }
   } else {
@@ -957,35 +995,43 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       }
       c = fmaxf(c, 0x1p-126f);
       float m_ref = -INFINITY, l = 0.0f;
+      int ev = 0;
       for (int t = 0; t < p.n; t++, unit++) {
         const int tile = p.tile0 + t, valid = min(RV_PFX_N, p.keys - tile * RV_PFX_N);
         const int lim = min(max(seen - tile * RV_PFX_N, 0), RV_PFX_N);
         const int slot = (pair ? 0 : s) * SLOTS + unit % SLOTS;
-        const float *sc = s_scale + (size_t)slot * 3 * RV_PFX_N;
+        const float *sc = s_scale + slot * RV_PFX_SCALE;
         if (Q8) ok = pfx_wait(&sc_full[slot], (uint32_t)(unit / SLOTS) & 1);
         ok = ok && pfx_wait(&s_full[s], unit & 1);
         if (!ok) break;
         tc_fence_after();
         if (warp_on) {
-          // The scores are read twice, for the maximum and for P: a row's 128
-          // do not fit the registers beside the rest.
           const int halves = valid > 64 ? 2 : 1;
           const bool full = __all_sync(RV_FULL, lim == RV_PFX_N || !on);
-          auto scores = [&](int h, uint32_t (&v)[64]) {
+          if constexpr (Q8) {
+            // The tile's values reach 2^ev; P holds the tokens' scales, so the
+            // reference grows with it.
+            const float *vm = sc + 2 * RV_PFX_N;
+            const float vmax = fmaxf(vm[0], fmaxf(vm[1], vm[2]));
+            ev = max((int)(__float_as_uint(vmax) >> 23) - 126, -80);
+          }
+#pragma unroll 1
+          for (int h = 0; h < halves; h++) {
+            uint32_t v[64];
             tc_ld_wait(tS + 64 * h, v);
             if constexpr (Q8) {
               const float2 c2 = make_float2(c, c), zero = make_float2(0, 0);
 #pragma unroll
               for (int j = 0; j < 64; j += 4) {
-                const float4 k4 = *(const float4 *)(sc + 64 * h + j), l4 = *(const float4 *)(sc + RV_PFX_N + 64 * h + j);
+                const float4 k4 = *(const float4 *)(sc + 64 * h + j);
                 float2 x0 = make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                 float2 x1 = make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
                 if (PRECISE) {
                   x0 = fma_f32x2(x0, c2, zero);
                   x1 = fma_f32x2(x1, c2, zero);
                 }
-                x0 = fma_f32x2(x0, make_float2(k4.x, k4.y), make_float2(l4.x, l4.y));
-                x1 = fma_f32x2(x1, make_float2(k4.z, k4.w), make_float2(l4.z, l4.w));
+                x0 = fma_f32x2(x0, make_float2(k4.x, k4.y), zero);
+                x1 = fma_f32x2(x1, make_float2(k4.z, k4.w), zero);
                 v[j] = __float_as_uint(x0.x);
                 v[j + 1] = __float_as_uint(x0.y);
                 v[j + 2] = __float_as_uint(x1.x);
@@ -996,38 +1042,41 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 64; j++) v[j] = 64 * h + j < lim ? v[j] : 0xFF800000u;
             }
-          };
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          for (int h = 0; h < halves; h++) {
-            uint32_t v[64];
-            scores(h, v);
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int j = 0; j < 64; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
-          }
-          float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if constexpr (!Q8) top *= c;
-          if (!on) top = -INFINITY;
-          if (t == 0) {
-            m_ref = top;
-          } else if (const bool move = top > m_ref + RV_PFX_LAG; __any_sync(RV_FULL, move)) {
-            // Every product issued so far is done (S came after them).
-            const float f = move ? ex2(m_ref - top) : 1.0f;
-            if (move) m_ref = top;
-            l *= f;
-            for (int ch = 0; ch < D / 32; ch++) {
-              uint32_t o[32];
-              tc_ld_wait(tO + 32 * ch, o);
+            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if constexpr (!Q8) top *= c;
+            top = on ? ceilf(top) + ev : -INFINITY;
+            if (t == 0 && h == 0) {
+              m_ref = top;
+            } else if (const bool move = top > m_ref + RV_PFX_LAG; __any_sync(RV_FULL, move)) {
+              // A new reference, a whole number of powers of two away: O and P
+              // change their exponents.  Every product issued so far is done
+              // (S came after them).
+              const int d = move && m_ref != -INFINITY ? (int)fmaxf(m_ref - top, -200.0f) : 0;
+              const bool none = move && (m_ref == -INFINITY || d < -126);
+              const float f = none ? 0.0f : __uint_as_float((uint32_t)(127 + d) << 23);
+              if (move) m_ref = top;
+              l *= f;
+              const __half2 f2 = __float2half2_rn(f);
+#pragma unroll 1
+              for (int ch = t > 0 ? 0 : D / 16; ch < D / 16 + 4 * h; ch++) {
+                uint32_t o[16];
+                const bool is_p = ch >= D / 16;  // P of the tile's first half
+                const uint32_t at = is_p ? tS + 16 * (ch - D / 16) : tO + 16 * ch;
+                tc_ld_wait(at, o);
 #pragma unroll
-              for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tc_st32(tO + 32 * ch, o);
+                for (int j = 0; j < 16; j++) {
+                  const __half2 x = __hmul2(*(const __half2 *)&o[j], f2);
+                  o[j] = is_p ? *(const uint32_t *)&x : __float_as_uint(__uint_as_float(o[j]) * f);
+                }
+                tc_st16(at, o);
+              }
             }
-          }
-          const float m_use = m_ref == -INFINITY ? 0.0f : m_ref - RV_PFX_LIFT;
-          const float2 c2 = make_float2(c, c), m2 = make_float2(-m_use, -m_use);
-          float2 l2[2] = {make_float2(0, 0), make_float2(0, 0)};
-          for (int h = 0; h < halves; h++) {
-            uint32_t v[64];
-            scores(h, v);
+            const float m_use = m_ref == -INFINITY ? 0.0f : m_ref - RV_PFX_LIFT;
+            const float2 c2 = make_float2(c, c), m2 = make_float2(-m_use, -m_use);
+            float2 l2[2] = {make_float2(0, 0), make_float2(0, 0)};
 #pragma unroll
             for (int ch = 0; ch < 2; ch++) {
               uint32_t o[32];
@@ -1038,10 +1087,9 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                 x = Q8 ? add_f32x2(x, m2) : fma_f32x2(x, c2, m2);
                 x.x = ex2(x.x);
                 x.y = ex2(x.y);
+                l2[j & 1] = add_f32x2(l2[j & 1], x);
                 if constexpr (Q8)
-                  l2[j & 1] = fma_f32x2(x, *(const float2 *)(sc + 2 * RV_PFX_N + 64 * h + e), l2[j & 1]);
-                else
-                  l2[j & 1] = add_f32x2(l2[j & 1], x);
+                  x = fma_f32x2(x, *(const float2 *)(sc + RV_PFX_N + 64 * h + e), make_float2(0, 0));
                 o[j] = pack_f16(x.x, x.y);
                 if constexpr (PRECISE) {
                   const float2 f = __half22float2(*(const __half2 *)&o[j]);
@@ -1052,8 +1100,8 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
               if constexpr (PRECISE) tc_st32(tS + 64 * h + 32 * ch, o);
               else tc_st16(tS + 64 * h + 32 * ch, o);
             }
+            l += (l2[0].x + l2[1].x) + (l2[0].y + l2[1].y);
           }
-          l += (l2[0].x + l2[1].x) + (l2[0].y + l2[1].y);
           tc_wait_st();
         }
         tc_fence_before();
@@ -1099,7 +1147,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
   }
   if (warp == 0) {
     tc_fence_after();
-    tc_dealloc(tmem, 512);
+    tc_dealloc(*s_tmem, 512);
   }
 }
 
