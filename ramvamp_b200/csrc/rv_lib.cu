@@ -2771,6 +2771,8 @@ static void prefix_shape(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv,
   w->nrt_s = (w->rows_s + w->sr_s - 1) / w->sr_s;
   w->rw_p = w->pair ? RV_PFX_M : std::min((int)sr, w->rows_p);
   w->rw_s = std::min((int)sr, w->rows_s);
+  w->by_g = PfxDiv((uint32_t)G);
+  w->by_row = PfxDiv((uint32_t)w->rows_s);
 }
 static PfxScratch prefix_scratch(size_t n_seqs, size_t n_kv, size_t hd, const PfxWork &w) {
   // A segment has one piece more than cuts, and the cuts of a line are fewer

@@ -152,6 +152,18 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 #define RV_PFX_TABLE 32       // pieces a stream works through between plans
 #define RV_PFX_O 256          // first tensor-memory column of O (S and P: 0..255)
 
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
+struct PfxDiv {
+  uint32_t mul, shift;
+  PfxDiv() = default;
+  __host__ explicit PfxDiv(uint32_t d) {
+    shift = 0;
+    while (shift < 31 && (1u << shift) < d) shift++;
+    mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+  }
+  RV_DEVFN int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+
 struct PfxWork {
   int tp;              // prefix tiles
   int rows_p, rows_s;  // query rows of one kv head: all sequences', one sequence's
@@ -159,6 +171,7 @@ struct PfxWork {
   int nrt_p, nrt_s;    // segments per kv head (per sequence)
   int rw_p, rw_s;      // rows of a part
   int pair;            // the prefix runs on paired streams
+  PfxDiv by_g, by_row; // divisions by the query heads of a kv head, by the query rows of a sequence's
   int grid;
   int q_aligned, out_aligned;  // 16-byte loads and stores
   int *cum;            // [2 n_seqs + 1]: suffix tiles, then suffixes that are not empty, before sequence b
@@ -316,6 +329,24 @@ RV_DEVFN float2 add_f32x2(float2 a, float2 b) {
       : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
   return d;
 }
+// 2^x of two values on the FMA units: x = n + f with n the nearest integer and
+// |f| <= 1/2, 2^f by its degree-4 polynomial of least largest relative error
+// (2.6e-6, fitted for this), n added to the exponent.  x <= 30; below -126 the
+// result is of the order of 2^-126; NaN stays NaN.
+RV_DEVFN float2 ex2_poly(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float big = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
+  const float2 t = add_f32x2(x, make_float2(big, big)), n = add_f32x2(t, make_float2(-big, -big));
+  const float2 f = fma_f32x2(n, make_float2(-1, -1), x);
+  const auto c2 = [](float c) { return make_float2(c, c); };
+  float2 p = fma_f32x2(f, c2(0.009570086f), c2(0.055917852f));
+  p = fma_f32x2(f, p, c2(0.24024744f));
+  p = fma_f32x2(f, p, c2(0.6931218f));
+  p = fma_f32x2(f, p, c2(0.9999993f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
 // Consecutive 32-bit columns of this thread's tensor-memory lane, loaded when
 // it returns (one statement, so no use can be moved before the wait).
 RV_DEVFN void tc_ld_wait(uint32_t taddr, uint32_t (&v)[64]) {
@@ -380,60 +411,61 @@ RV_DEVFN uint32_t pack_f16(float lo, float hi) {  // element order: lo first
 struct PfxRow {
   int b, i, h;
 };
-RV_DEVFN PfxRow pfx_row(const PrefixArgs &a, bool suffix, int b, int kvh, int r) {
-  const int G = (int)(a.n_heads / a.n_kv), per = (int)a.n_q * G;
+RV_DEVFN PfxRow pfx_row(const PfxWork &w, int G, bool suffix, int b, int kvh, int r) {
   PfxRow o;
-  o.b = suffix ? b : r / per;
-  const int x = suffix ? r : r - o.b * per;
-  o.i = x / G;
+  o.b = suffix ? b : w.by_row(r);
+  const int x = suffix ? r : r - o.b * w.rows_s;
+  o.i = w.by_g(x);
   o.h = kvh * G + x - o.i * G;
   return o;
 }
 
 // The query rows of a stream's tile into its A operand(s) (K-major, 128-byte
 // swizzle, 64 values a half tile), by the stream's 128 threads: D / 8 threads a
-// row, so a row's loads are contiguous, and four rows a thread in flight.  f32
-// rows are divided by a power of two first (2^e, e in `up`; the largest value
-// then lies in [1, 2)) and held as hi + lo.  neg: the queries change sign.
+// row, so a row's loads are contiguous, and 64 registers of loads a thread in
+// flight.  f32 rows are divided by a power of two first (2^e, e in `up`; the
+// largest value then lies in [1, 2)) and held as hi + lo.  neg: the queries
+// change sign.
 template <int D, typename T, int SR>
-RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr, bool aligned, bool neg, int tid,
+RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxWork &w, const PfxPiece &p, int r0, int nr, bool neg, int tid,
                          uint8_t *hi, int8_t *up) {
   constexpr int LPR = D / 8, RP = RV_PFX_M / LPR;  // threads a row, rows a pass
   constexpr bool F32 = sizeof(T) == 4;
+  constexpr int W4 = F32 ? 2 : 1, NB = F32 ? 2 : 4;  // 16-byte words; rows a thread in flight
   uint8_t *lo = hi + SR * D * 2;
-  const int c = tid % LPR;
-  for (int b0 = 0; b0 < nr; b0 += 4 * RP) {
-    float x[4][8];
+  const int c = tid % LPR, G = (int)(a.n_heads / a.n_kv);
+  for (int b0 = 0; b0 < nr; b0 += NB * RP) {
+    uint4 x[NB][W4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < NB; k++) {
       const int row = b0 + k * RP + tid / LPR;
       if (row < nr) {
-        const PfxRow pr = pfx_row(a, p.head & 1, p.b, p.head >> 1, r0 + row);
+        const PfxRow pr = pfx_row(w, G, p.head & 1, p.b, p.head >> 1, r0 + row);
         const T *q = (const T *)a.q + (size_t)pr.b * a.q_seq_stride + (size_t)pr.i * a.q_token_stride +
                      (size_t)pr.h * D + 8 * c;
-        if (aligned) {
-          if constexpr (F32) {
-            *(float4 *)x[k] = __ldg((const float4 *)q);
-            *(float4 *)(x[k] + 4) = __ldg((const float4 *)q + 1);
-          } else {
-            *(uint4 *)x[k] = __ldg((const uint4 *)q);  // eight f16 as they are
-          }
-        } else {
+        if (w.q_aligned) {
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            if constexpr (F32) x[k][j] = q[j];
-            else ((T *)x[k])[j] = q[j];
+          for (int i = 0; i < W4; i++) x[k][i] = __ldg((const uint4 *)q + i);
+        } else {
+          __align__(16) T t[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) t[j] = q[j];
+#pragma unroll
+          for (int i = 0; i < W4; i++) x[k][i] = ((const uint4 *)t)[i];
         }
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < NB; k++) {
       const int row = b0 + k * RP + tid / LPR;
       const uint32_t off = (uint32_t)(c >> 3) * (SR * 128) + tc_sw_off(row, c & 7);
       if constexpr (F32) {
+        const float f[8] = {__uint_as_float(x[k][0].x), __uint_as_float(x[k][0].y), __uint_as_float(x[k][0].z),
+                            __uint_as_float(x[k][0].w), __uint_as_float(x[k][1].x), __uint_as_float(x[k][1].y),
+                            __uint_as_float(x[k][1].z), __uint_as_float(x[k][1].w)};
         float m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(x[k][j]));
+        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(f[j]));
         if (row >= nr) m = 0;
 #pragma unroll
         for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(RV_FULL, m, o));
@@ -445,15 +477,15 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxPiece &p, int r0, int nr,
         uint32_t o[4], r[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float x0 = x[k][2 * j] * sg, x1 = x[k][2 * j + 1] * sg;
+          const float x0 = f[2 * j] * sg, x1 = f[2 * j + 1] * sg;
           o[j] = pack_f16(x0, x1);
-          const float2 f = __half22float2(*(const __half2 *)&o[j]);
-          r[j] = pack_f16(x0 - f.x, x1 - f.y);
+          const float2 h = __half22float2(*(const __half2 *)&o[j]);
+          r[j] = pack_f16(x0 - h.x, x1 - h.y);
         }
         *(uint4 *)(hi + off) = make_uint4(o[0], o[1], o[2], o[3]);
         *(uint4 *)(lo + off) = make_uint4(r[0], r[1], r[2], r[3]);
       } else if (row < nr) {
-        uint4 v = *(const uint4 *)x[k];
+        const uint4 v = x[k][0];
         const uint32_t sg = neg ? 0x80008000u : 0;
         *(uint4 *)(hi + off) = make_uint4(v.x ^ sg, v.y ^ sg, v.z ^ sg, v.w ^ sg);
       }
@@ -478,10 +510,23 @@ RV_DEVFN bool elect_one() {
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
   return p != 0;
 }
-// Barrier phases that a whole warp waits for.
-RV_DEVFN bool pfx_wait(uint64_t *bar, uint32_t parity) {
-  return __all_sync(RV_FULL, mbar_wait_bounded(bar, parity));
+// The bounded wait of mbar_wait_bounded in few instructions: this kernel's
+// roles are limited by the instruction cache.
+RV_DEVFN bool pfx_wait1(uint64_t *bar, uint32_t parity) {
+  long long t0 = 0;
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); i++) {
+    if (i & 31) continue;
+    const long long now = clock64();
+    if (i == 32) t0 = now;
+    if (now - t0 > RV_WAIT_CYCLES) {
+      rv_dev_fail(RV_ERR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
 }
+// The same by a whole warp.
+RV_DEVFN bool pfx_wait(uint64_t *bar, uint32_t parity) { return __all_sync(RV_FULL, pfx_wait1(bar, parity)); }
 
 template <int D, typename T, bool Q8>
 __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
@@ -703,150 +748,113 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       const uint32_t q_lo = smem_addr(sm) >> 4, ring_lo = smem_addr(ring) >> 4;
       const uint32_t idesc_s = tc_idesc(RV_PFX_N), idesc_o = tc_idesc(D) | (1u << 16);  // B of P V: keys down the rows
       auto mk = [](uint32_t lo, uint32_t hi) { return ((uint64_t)hi << 32) | lo; };
-      int at[2] = {0, 0}, j[2] = {0, 0}, len[2], nk = 0, nv = 0;
-      // One batch of products, by one thread: S = Q K^T of stream s from the
-      // ring's slot.
-      auto issue_qk = [&](int s, int slot) {
-        const uint32_t qa = q_lo + s * (C::QS >> 4), kb = ring_lo + (uint32_t)(slot * (TILE >> 4)), d = tmem + 128 * s;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; kk++) {
-          const uint32_t oq = (uint32_t)(kk >> 2) * (C::SR * 128 >> 4) + 2 * (kk & 3),
-                         okk = (uint32_t)(kk >> 2) * (RV_PFX_N * 128 >> 4) + 2 * (kk & 3);
-          tc_mma_f16(d, mk(lbo_k | (qa + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, kk != 0);
-          if (PRECISE)
-            tc_mma_f16(d, mk(lbo_k | (qa + (C::QT >> 4) + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, 1u);
-        }
-        tc_commit(&s_full[s]);
-      };
-      // O (+)= P V of stream s over `steps` times 16 keys.
-      auto issue_pv = [&](int s, int slot, int steps, bool add) {
-        const uint32_t vb = ring_lo + (uint32_t)(slot * (TILE >> 4)), p0 = tmem + 128 * s, d = p0 + RV_PFX_O;
-#pragma unroll
-        for (int kk = 0; kk < 8; kk++) {
-          if (kk < steps) {
-            const uint32_t pa = p0 + 32 * (kk >> 1) + 8 * (kk & 1);
-            const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
-            tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || add);
-            if (PRECISE) tc_mma_f16_ta(d, pa + 16, bd, idesc_o, 1u);
-          }
-        }
-      };
-      if (pair) {
-        // One thread runs the whole role: the streams are in step, so there is
-        // one count of everything, and few instructions stand between the
-        // batches (this warp shares its scheduler with two softmax warps).
-        if (elect_one()) {
-          const auto full = [&](int i) { return mbar_wait_bounded(&kv_full[i % R], (i / R) & 1); };
-          for (int e = 0; ok && e < count[0]; e++) {
-            const PfxPiece *p = &tab[0][e];
-            const int units = p->n;
-            const int last = min(RV_PFX_N, p->keys - (p->tile0 + units - 1) * RV_PFX_N);
-            ok = mbar_wait_bounded(&q_ready[0], nq[0] & 1) && mbar_wait_bounded(&q_ready[1], nq[0] & 1);
-            nq[0]++;
-            nk = n++;
-            ok = ok && full(nk);
+      // A stream's place: table entry, its units (0: none left), the next one to
+      // multiply (-1: S of the piece's first is still to come), phases passed.
+      struct Place {
+        int at, len, j, np, nq;
+      } c = {0, 0, -1, np[0], nq[0]}, o = {0, 0, -1, np[1], nq[1]};
+      const auto wait_full = [&](int i) { return pfx_wait(&kv_full[i % R], (i / R) & 1); };
+      int nk = 0, nv = 0;
+      pfx_entry(tab[0], count[0], c.at, c.len);
+      if (pair) o.len = c.len, o.at = c.at;
+      else pfx_entry(tab[1], count[1], o.at, o.len);
+      // The streams in turn: O += P V of a unit and S = Q K^T of the stream's
+      // next one.  Paired streams share tiles: stream 0 takes them from the ring,
+      // stream 1 gives them back.
+      int s = 0;
+#pragma unroll 1
+      for (; ok && (c.len || o.len) && !*s_fail; s ^= 1) {
+        if (c.len) {
+          const bool take = !(pair && s), give = !pair || s;
+          const PfxPiece *p = &tab[pair ? 0 : s][c.at];
+          bool next = c.j + 1 < c.len;  // an S is to come: of this piece, or
+          if (c.j >= 0) {
+            const int valid = min(RV_PFX_N, p->keys - (p->tile0 + c.j) * RV_PFX_N), steps = (valid + 15) >> 4;
+            if (take) {
+              nv = n++;
+              ok = wait_full(nv);
+              if (!Q8 && (p->head & 1) && (valid & 15)) {
+                // Rows past the sequence's end hold whatever the cache held:
+                // zero those the last K step reads (0 * NaN is not 0).
+                for (int i = lane; i < (16 * steps - valid) * (D / 8); i += 32) {
+                  const int r = valid + i / (D / 8), ch = i % (D / 8);
+                  *(uint4 *)(ring + (size_t)(nv % R) * TILE + (ch >> 3) * (RV_PFX_N * 128) + tc_sw_off(r, ch & 7)) =
+                      make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+                __syncwarp();
+              }
+              if (next) {
+                nk = n++;
+                ok = ok && wait_full(nk);
+              }
+            }
+            ok = ok && pfx_wait(&p_ready[s], c.np & 1);
+            c.np++;
             if (!ok) break;
             tc_fence_after();
-#pragma unroll 1
-            for (int s = 0; s < 2; s++) issue_qk(s, nk % R);
-            tc_commit(&kv_empty[nk % R]);
-            for (int u = 0; ok && u < units; u++) {
-              const bool more = u + 1 < units;
-              const int steps = more ? 8 : (last + 15) >> 4;
-              nv = n++;
-              ok = full(nv);
-              if (more) {
-                nk = n++;
-                ok = ok && full(nk);
+            if (elect_one()) {
+              const uint32_t vb = ring_lo + (uint32_t)(nv % R * (TILE >> 4)), p0 = tmem + 128 * s, d = p0 + RV_PFX_O;
+#pragma unroll
+              for (int kk = 0; kk < 8; kk++) {
+                if (kk < steps) {
+                  const uint32_t pa = p0 + 32 * (kk >> 1) + 8 * (kk & 1);
+                  const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
+                  tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || c.j != 0);
+                  if (PRECISE) tc_mma_f16_ta(d, pa + 16, bd, idesc_o, 1u);
+                }
               }
-#pragma unroll 1
-              for (int s = 0; ok && s < 2; s++) {
-                ok = mbar_wait_bounded(&p_ready[s], np[0] & 1);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(s, nv % R, steps, u != 0);
-                if (more) issue_qk(s, nk % R);
-                else tc_commit(&o_full[s]);
-              }
-              np[0]++;
-              tc_commit(&kv_empty[nv % R]);
-              if (more) tc_commit(&kv_empty[nk % R]);
+              if (!next) tc_commit(&o_full[s]);
+              if (give) tc_commit(&kv_empty[nv % R]);
             }
+            __syncwarp();
           }
-          if (!ok) *s_fail = 1;
-        }
-        __syncwarp();
-        // The counts go on with the other lanes too, should another lane be
-        // elected in the next plan.
-        n = __reduce_max_sync(RV_FULL, n);
-        np[0] = __reduce_max_sync(RV_FULL, np[0]);
-        nq[0] = __reduce_max_sync(RV_FULL, nq[0]);
-      } else {
-      auto wait_full = [&](int i) { return pfx_wait(&kv_full[i % R], (i / R) & 1); };
-      // A new piece's first S.
-      auto start = [&](int s) {
-        pfx_entry(tab[s], count[s], at[s], len[s]);
-        j[s] = 0;
-        if (!len[s]) return;
-        ok = pfx_wait(&q_ready[s], nq[s] & 1);
-        nq[s]++;
-        nk = n++;
-        ok = ok && wait_full(nk);
-        tc_fence_after();
-        if (ok && elect_one()) {
-          issue_qk(s, nk % R);
-          tc_commit(&kv_empty[nk % R]);
-        }
-        __syncwarp();
-      };
-      // O += P V of a stream's unit and the next S of the same piece, in one go.
-      auto turn = [&](int s) {
-        if (!ok || !len[s]) return;
-        const PfxPiece &p = tab[s][at[s]];
-        const int valid = min(RV_PFX_N, p.keys - (p.tile0 + j[s]) * RV_PFX_N), steps = (valid + 15) >> 4;
-        const bool more = j[s] + 1 < len[s];
-        nv = n++;
-        ok = wait_full(nv);
-        if (!Q8 && (p.head & 1) && (valid & 15)) {
-          // Rows past the sequence's end hold whatever the cache held: zero
-          // those the last K step reads (0 * NaN is not 0).
-          for (int i = lane; i < (16 * steps - valid) * (D / 8); i += 32) {
-            const int r = valid + i / (D / 8), ch = i % (D / 8);
-            *(uint4 *)(ring + (size_t)(nv % R) * TILE + (ch >> 3) * (RV_PFX_N * 128) + tc_sw_off(r, ch & 7)) =
-                make_uint4(0, 0, 0, 0);
+          c.j++;
+          if (c.j == c.len) {  // of the next piece
+            c.at++;
+            pfx_entry(tab[pair ? 0 : s], count[pair ? 0 : s], c.at, c.len);
+            c.j = 0;
+            next = c.len != 0;
           }
-          fence_proxy_async();
-          __syncwarp();
+          if (next) {
+            if (c.j == 0) {
+              ok = pfx_wait(&q_ready[s], c.nq & 1);
+              c.nq++;
+              if (take) {
+                nk = n++;
+                ok = ok && wait_full(nk);
+              }
+              if (!ok) break;
+              tc_fence_after();
+            }
+            if (elect_one()) {
+              const uint32_t qa = q_lo + s * (C::QS >> 4), kb = ring_lo + (uint32_t)(nk % R * (TILE >> 4)),
+                             d = tmem + 128 * s;
+#pragma unroll
+              for (int kk = 0; kk < D / 16; kk++) {
+                const uint32_t oq = (uint32_t)(kk >> 2) * (C::SR * 128 >> 4) + 2 * (kk & 3),
+                               okk = (uint32_t)(kk >> 2) * (RV_PFX_N * 128 >> 4) + 2 * (kk & 3);
+                tc_mma_f16(d, mk(lbo_k | (qa + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s, kk != 0);
+                if (PRECISE)
+                  tc_mma_f16(d, mk(lbo_k | (qa + (C::QT >> 4) + oq), hi_sw), mk(lbo_k | (kb + okk), hi_sw), idesc_s,
+                             1u);
+              }
+              tc_commit(&s_full[s]);
+              if (give) tc_commit(&kv_empty[nk % R]);
+            }
+            __syncwarp();
+          }
         }
-        if (more) {
-          nk = n++;
-          ok = ok && wait_full(nk);
-        }
-        ok = ok && pfx_wait(&p_ready[s], np[s] & 1);
-        np[s]++;
-        if (!ok) return;
-        tc_fence_after();
-        if (elect_one()) {
-          issue_pv(s, nv % R, steps, j[s] != 0);
-          if (more) issue_qk(s, nk % R);
-          else tc_commit(&o_full[s]);
-          tc_commit(&kv_empty[nv % R]);
-          if (more) tc_commit(&kv_empty[nk % R]);
-        }
-        __syncwarp();
-        j[s]++;
-        if (!more) {
-          at[s]++;
-          start(s);
-        }
-      };
-      start(0);
-      if (ok) start(1);
-      while (ok && !*s_fail && (len[0] || len[1])) {
-        turn(0);
-        turn(1);
+        const Place t = c;
+        c = o;
+        o = t;
       }
+      if (s) {  // an odd number of turns: c is stream 1's
+        const Place t = c;
+        c = o;
+        o = t;
       }
+      np[0] = c.np, nq[0] = c.nq, np[1] = o.np, nq[1] = o.nq;
       if (!ok) *s_fail = 1;
       if (*s_fail) {  // products in flight end before tensor memory is freed
         if (elect_one()) {
@@ -967,7 +975,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     auto give_q = [&](const PfxPiece &x, int which) {
       const int r0 = x.row0 + (pair ? RV_PFX_M * s : 0);
       const int rows = x.head & 1 ? w.rows_s : w.rows_p;
-      pfx_load_q<D, T, C::SR>(a, x, r0, min(C::SR, rows - r0), w.q_aligned, neg, row, q_dst,
+      pfx_load_q<D, T, C::SR>(a, w, x, r0, min(C::SR, rows - r0), neg, row, q_dst,
                               s_up + (2 * s + (which & 1)) * C::SR);
       fence_proxy_async();
       __syncwarp();
@@ -975,17 +983,44 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     };
     int at = 0, left;
     pfx_entry(mytab, mycount, at, left);
-    if (left) give_q(mytab[at], piece);
-    while (ok && left && !*s_fail) {
+    // What the piece before leaves, written while this one's first scores are
+    // on their way.
+    int p_head = 0, p_part = -1;
+    bool p_on = false, p_warp = false;
+    float p_m = 0, p_l = 0;
+#pragma unroll 1
+    while (ok && !*s_fail) {
+      if (left) give_q(mytab[at], piece);
+      if (p_part >= 0) {
+        const int rw = p_head & 1 ? w.rw_s : w.rw_p;
+        const size_t part = (size_t)p_part + (pair ? s : 0);
+        float4 *po = (p_head & 1 ? w.o_s : w.o_p) + part * (D / 4) * rw + row;
+        if (p_on) (p_head & 1 ? w.ml_s : w.ml_p)[part * rw + row] = make_float2(p_m, p_l);
+        ok = pfx_wait(&o_full[s], (piece - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (p_warp) {
+#pragma unroll 1
+          for (int ch = 0; ch < D / 16; ch++) {
+            uint32_t v[16];
+            tc_ld_wait(tO + 16 * ch, v);
+            if (p_on) {
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                po[(4 * ch + j) * rw] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                                    __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+            }
+          }
+          tc_fence_before();
+        }
+      }
+      if (!left) break;
       const PfxPiece p = mytab[at];
       const bool suffix = p.head & 1;
       const int r = p.row0 + (pair ? RV_PFX_M * s : 0) + row;  // this thread's query row
       const bool on = row < C::SR && r < (suffix ? w.rows_s : w.rows_p), warp_on = __any_sync(RV_FULL, on);
       int seen = on ? p.keys : 0;  // keys of the segment that this row sees
-      if (suffix && on) {
-        const PfxRow pr = pfx_row(a, true, p.b, p.head >> 1, r);
-        seen = min(max(p.keys - (int)a.n_q + 1 + pr.i, 0), p.keys);
-      }
+      if (suffix && on) seen = min(max(p.keys - (int)a.n_q + 1 + w.by_g(r), 0), p.keys);
       // Scores times c are in units of log2 (8-bit keys: their scales hold
       // the attention scale).  At least 2^-126, so that -infinity stays one.
       float c = Q8 ? 1.0f : scale;
@@ -1085,8 +1120,14 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                 const int e = 32 * ch + 2 * j;
                 float2 x = make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
                 x = Q8 ? add_f32x2(x, m2) : fma_f32x2(x, c2, m2);
-                x.x = ex2(x.x);
-                x.y = ex2(x.y);
+                // Every fourth pair on the FMA units: the exponentials' own unit
+                // is what bounds a stream (f32 needs its accuracy).
+                if (!PRECISE && (j & 3) == 3) {
+                  x = ex2_poly(x);
+                } else {
+                  x.x = ex2(x.x);
+                  x.y = ex2(x.y);
+                }
                 l2[j & 1] = add_f32x2(l2[j & 1], x);
                 if constexpr (Q8)
                   x = fma_f32x2(x, *(const float2 *)(sc + RV_PFX_N + 64 * h + e), make_float2(0, 0));
@@ -1109,34 +1150,16 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         if (lane == 0) mbar_arrive(&p_ready[s]);
       }
       if (!ok) break;
-      // The products have read this piece's queries (S came after them): give
-      // them the next piece's, under the last P V.
+      // The products have read this piece's queries (S came after them), so the
+      // next piece's may take their place under the last P V.
+      p_head = p.head;
+      p_part = p.part;
+      p_on = on;
+      p_warp = warp_on;
+      p_m = m_ref == -INFINITY ? -INFINITY : m_ref - RV_PFX_LIFT;
+      p_l = l;
       at++;
       pfx_entry(mytab, mycount, at, left);
-      if (left) give_q(mytab[at], piece + 1);
-      // ------------------------------------------- the piece's (m, l, O)
-      const int rw = suffix ? w.rw_s : w.rw_p;
-      const size_t part = (size_t)p.part + (pair ? s : 0);
-      float4 *po = (suffix ? w.o_s : w.o_p) + part * (D / 4) * rw + row;
-      float2 *pm = (suffix ? w.ml_s : w.ml_p) + part * rw + row;
-      if (on) *pm = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref - RV_PFX_LIFT, l);
-      ok = pfx_wait(&o_full[s], piece & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (warp_on) {
-#pragma unroll
-        for (int h = 0; h < D / 64; h++) {
-          uint32_t v[64];
-          tc_ld_wait(tO + 64 * h, v);
-          if (on) {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-              po[(16 * h + j) * rw] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
-                                                  __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
-          }
-        }
-        tc_fence_before();
-      }
       piece++;
     }
     if (!ok) *s_fail = 1;
@@ -1161,7 +1184,7 @@ __global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) 
   const int lane = threadIdx.x & 31, d4 = threadIdx.x >> 5, kvh = blockIdx.y, pl = lane >> 3;
   const int r = min((int)blockIdx.x * RV_PFX_JOIN_ROWS + (lane & 7), w.rows_p - 1);
   const bool on = (int)blockIdx.x * RV_PFX_JOIN_ROWS + (lane & 7) < w.rows_p;
-  const PfxRow pr = pfx_row(a, false, 0, kvh, r);
+  const PfxRow pr = pfx_row(w, (int)(a.n_heads / a.n_kv), false, 0, kvh, r);
   const int segs = (int)a.n_kv * w.nrt_s;
   pdl_wait();  // cum and the parts are k_prefix_tc's
   const int *fcum = w.cum + a.n_seqs + 1;
