@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 #define RV_PFX_LIFT 7.0f      // P is lifted by 2^7
 #define RV_PFX_SCALE_SLOTS 8  // tiles a stream whose token scales are in shared memory
 #define RV_PFX_SCALE (2 * RV_PFX_N + 4)  // floats of a tile's scales: keys', values', the values' largest by warp
-#define RV_PFX_TABLE 32       // pieces a stream works through between plans
+#define RV_PFX_TABLE 32       // pieces a stream works through between plans: one a lane
 #define RV_PFX_O 256          // first tensor-memory column of O (S and P: 0..255)
 
 // n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery, 1994).
@@ -194,12 +194,12 @@ RV_DEVFN PfxLine pfx_line(const PrefixArgs &a, const PfxWork &w, int tiles, int 
   l.solo_p = w.pair || w.tp == 0 ? 0 : seg_p * (w.tp + RV_PFX_OV);
   l.wp = w.pair ? seg_p * w.tp : 0;
   l.w = l.solo_p + suffix;
-  // A paired unit costs a CTA about 1.5 solo places (measured: 5.1 and 3.4
-  // thousand cycles).
+  // A paired unit costs a CTA about two solo places (measured: 5.3 and 2.5
+  // thousand cycles), and a paired segment three units more.
   l.gp = 0;
   if (l.wp) {
-    const long long cost = 3ll * l.wp, both = cost + 2ll * l.w;
-    l.gp = min(max((int)((cost * w.grid + both / 2) / both), 1), l.w ? w.grid - 1 : w.grid);
+    const float cost = __fmul_rn(2.0f, (float)(l.wp + 3 * seg_p)), share = __fdiv_rn(cost, __fadd_rn(cost, (float)l.w));
+    l.gp = min(max(__float2int_rn(__fmul_rn(share, (float)w.grid)), 1), l.w ? w.grid - 1 : w.grid);
   }
   l.per_p = l.gp ? (l.wp + l.gp - 1) / l.gp : 1;
   const int streams = 2 * (w.grid - l.gp);
@@ -212,10 +212,9 @@ struct __align__(16) PfxPiece {
   int b, head, row0, keys;  // head: 2 * kv head + (1: a suffix)
   int tile0, n, part, pad;
 };
-// A stream's stretch of its line: places [u, end), which is stretch v, over
-// the segments g0..g1 (counted along the line, empty ones included).
+// A stream's stretch of its line: places [u, end), which is stretch v.
 struct PfxStretch {
-  int u, end, v, g0, g1;
+  int u, end, v;
 };
 // Segment [at, at + len) of the line (fixed cost ov, then tiles) cut to a stretch.
 RV_DEVFN void pfx_cut(PfxPiece &p, const PfxStretch &k, int at, int tiles, int ov) {
@@ -237,76 +236,82 @@ struct PfxCfg {
   static constexpr int NBARS = 2 * R + 8 + 2 * RV_PFX_SCALE_SLOTS + 1;
   static constexpr size_t ring = 2 * QS, raw = ring + (size_t)R * TILE, scales = raw + RAW, table = scales + SCALES,
                           ups = table + 2 * RV_PFX_TABLE * sizeof(PfxPiece), bars = ups + (PRECISE ? 4 * SR : 0);
-  static constexpr size_t total = bars + NBARS * 8 + 48 * 4;
+  static constexpr size_t total = bars + NBARS * 8 + 4 * 4;
   static_assert(total <= 227 * 1024, "shared memory of a CTA");
 };
 
 // The order in which K and V tiles are first used, for the warps that bring
 // them in: K of each stream's first unit, then in turn for each stream V of its
 // unit and K of its next.  Paired streams use the same tiles: one stream here.
-struct PfxFeed {
-  // Per stream: table entry, tile of it, its tiles (0: the stream has ended),
-  // units so far.  Indexed by constants, so they stay in registers.
-  int i[2], j[2], n[2], unit[2];
-  int boot, turn;
-  bool want_k;
-  // The current load.
-  bool is_k;
-  int s, entry, tile, u;
-};
 RV_DEVFN void pfx_entry(const PfxPiece *tab, int count, int &i, int &n) {
   for (n = 0; i < count; i++)
     if ((n = tab[i].n) > 0) return;
 }
-RV_DEVFN void pfx_feed_start(PfxFeed &f) {
-  f.boot = f.turn = 0;
-  f.want_k = false;
-  f.n[0] = f.n[1] = 0;
-}
-RV_DEVFN bool pfx_feed(const PfxPiece (*tab)[RV_PFX_TABLE], const int (&count)[2], int ns, PfxFeed &f) {
-  int s = -1;
-  if (f.boot < ns) {  // K of the streams' first units
-#pragma unroll
-    for (int k = 0; k < 2; k++)
-      if (s < 0 && k >= f.boot && k < ns) {
-        f.boot = k + 1;
-        f.i[k] = f.j[k] = 0;
-        pfx_entry(tab[k], count[k], f.i[k], f.n[k]);
-        if (f.n[k]) s = k;
-      }
-    f.is_k = true;
-  }
-  if (s < 0 && f.want_k) {  // K of the unit after the V just loaded
-    f.want_k = false;
-    f.is_k = true;
-    const int k = f.turn;
-    f.turn = ns == 2 ? k ^ 1 : 0;
-    if (k ? f.n[1] : f.n[0]) s = k;
-  }
-  if (s < 0) {  // V of the next stream in turn that goes on
-    if (!f.n[0] && !f.n[1]) return false;
-    if (!(f.turn ? f.n[1] : f.n[0])) f.turn ^= 1;
-    s = f.turn;
-    f.is_k = false;
-    f.want_k = true;
-  }
-  f.s = s;
-#pragma unroll
-  for (int k = 0; k < 2; k++)
-    if (s == k) {
-      f.entry = f.i[k];
-      f.tile = tab[k][f.i[k]].tile0 + f.j[k];
-      f.u = f.unit[k];
-      if (!f.is_k) {
-        f.unit[k]++;
-        if (++f.j[k] == f.n[k]) {
-          f.j[k] = 0;
-          f.i[k]++;
-          pfx_entry(tab[k], count[k], f.i[k], f.n[k]);
-        }
-      }
+struct PfxSide {  // a stream
+  int at, left, tile, unit;  // table entry, its units not loaded yet, the next one's tile; units so far
+  int b, head, keys;
+  bool begun;  // K of the next unit is loaded
+  RV_DEVFN void enter(const PfxPiece *tab, int count) {
+    pfx_entry(tab, count, at, left);
+    if (left) {
+      tile = tab[at].tile0;
+      b = tab[at].b;
+      head = tab[at].head;
+      keys = tab[at].keys;
     }
-  return true;
+  }
+};
+struct PfxFeed {
+  PfxSide c, o;  // the stream in turn and the other
+  int s;         // which c is
+  bool v_done;   // of this turn
+  // The current load.
+  bool is_k;
+  int stream, tile, b, head, keys, unit;
+};
+RV_DEVFN void pfx_feed_start(const PfxPiece (*tab)[RV_PFX_TABLE], const int (&count)[2], bool pair, PfxFeed &f) {
+  if (f.s) {
+    const PfxSide t = f.c;
+    f.c = f.o;
+    f.o = t;
+  }
+  f.s = f.c.at = f.o.at = 0;
+  f.c.begun = f.o.begun = f.v_done = false;
+  f.c.enter(tab[0], count[0]);
+  f.o.left = 0;
+  if (!pair) f.o.enter(tab[1], count[1]);
+}
+RV_DEVFN bool pfx_feed(const PfxPiece (*tab)[RV_PFX_TABLE], const int (&count)[2], bool pair, PfxFeed &f) {
+  while (f.c.left || f.o.left) {
+    f.is_k = f.v_done || !f.c.begun;
+    f.stream = f.s;
+    f.tile = f.c.tile;
+    f.b = f.c.b;
+    f.head = f.c.head;
+    f.keys = f.c.keys;
+    f.unit = f.c.unit;
+    if (!f.is_k) {  // V of the unit whose K came last
+      f.v_done = true;
+      f.c.unit++;
+      f.c.tile++;
+      if (--f.c.left == 0) {
+        f.c.at++;
+        f.c.enter(tab[f.s], count[f.s]);
+      }
+      return true;
+    }
+    const bool has = f.c.left != 0;  // K of the next unit; then it is the other's turn
+    f.c.begun = has;
+    f.v_done = false;
+    if (!pair) {
+      const PfxSide t = f.c;
+      f.c = f.o;
+      f.o = t;
+      f.s ^= 1;
+    }
+    if (has) return true;
+  }
+  return false;
 }
 
 RV_DEVFN float ex2(float x) {
@@ -328,24 +333,6 @@ RV_DEVFN float2 add_f32x2(float2 a, float2 b) {
       : "=l"(*(unsigned long long *)&d)
       : "l"(*(unsigned long long *)&a), "l"(*(unsigned long long *)&b));
   return d;
-}
-// 2^x of two values on the FMA units: x = n + f with n the nearest integer and
-// |f| <= 1/2, 2^f by its degree-4 polynomial of least largest relative error
-// (2.6e-6, fitted for this), n added to the exponent.  x <= 30; below -126 the
-// result is of the order of 2^-126; NaN stays NaN.
-RV_DEVFN float2 ex2_poly(float2 x) {
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
-  const float big = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are n
-  const float2 t = add_f32x2(x, make_float2(big, big)), n = add_f32x2(t, make_float2(-big, -big));
-  const float2 f = fma_f32x2(n, make_float2(-1, -1), x);
-  const auto c2 = [](float c) { return make_float2(c, c); };
-  float2 p = fma_f32x2(f, c2(0.009570086f), c2(0.055917852f));
-  p = fma_f32x2(f, p, c2(0.24024744f));
-  p = fma_f32x2(f, p, c2(0.6931218f));
-  p = fma_f32x2(f, p, c2(0.9999993f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 // Consecutive 32-bit columns of this thread's tensor-memory lane, loaded when
 // it returns (one statement, so no use can be moved before the wait).
@@ -431,18 +418,30 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxWork &w, const PfxPiece &
                          uint8_t *hi, int8_t *up) {
   constexpr int LPR = D / 8, RP = RV_PFX_M / LPR;  // threads a row, rows a pass
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int W4 = F32 ? 2 : 1, NB = F32 ? 2 : 4;  // 16-byte words; rows a thread in flight
+  constexpr int W4 = F32 ? 2 : 1, NB = 2;  // 16-byte words; rows a thread in flight
   uint8_t *lo = hi + SR * D * 2;
   const int c = tid % LPR, G = (int)(a.n_heads / a.n_kv);
+  const auto at = [&](int row) {
+    const PfxRow pr = pfx_row(w, G, p.head & 1, p.b, p.head >> 1, r0 + row);
+    return (const T *)a.q + (size_t)pr.b * a.q_seq_stride + (size_t)pr.i * a.q_token_stride + (size_t)pr.h * D + 8 * c;
+  };
+  if (!F32 && w.q_aligned && !neg) {  // as they are: copied past the registers
+#pragma unroll 1
+    for (int row = tid / LPR; row < nr; row += RP)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                       smem_addr(hi + (uint32_t)(c >> 3) * (SR * 128) + tc_sw_off(row, c & 7))),
+                   "l"(at(row))
+                   : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
   for (int b0 = 0; b0 < nr; b0 += NB * RP) {
     uint4 x[NB][W4];
 #pragma unroll
     for (int k = 0; k < NB; k++) {
       const int row = b0 + k * RP + tid / LPR;
       if (row < nr) {
-        const PfxRow pr = pfx_row(w, G, p.head & 1, p.b, p.head >> 1, r0 + row);
-        const T *q = (const T *)a.q + (size_t)pr.b * a.q_seq_stride + (size_t)pr.i * a.q_token_stride +
-                     (size_t)pr.h * D + 8 * c;
+        const T *q = at(row);
         if (w.q_aligned) {
 #pragma unroll
           for (int i = 0; i < W4; i++) x[k][i] = __ldg((const uint4 *)q + i);
@@ -544,9 +543,9 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
   uint64_t *bars = (uint64_t *)(sm + C::bars);
   uint64_t *kv_full = bars, *kv_empty = bars + R, *s_full = bars + 2 * R, *p_ready = s_full + 2, *o_full = p_ready + 2,
            *q_ready = o_full + 2, *sc_full = q_ready + 2, *drained = sc_full + 2 * SLOTS;
-  int *s_scan = (int *)(bars + C::NBARS);  // [32] warp sums, then per stream its first and last segment
-  uint32_t *s_tmem = (uint32_t *)(s_scan + 40);
-  volatile int *s_fail = s_scan + 41;
+  int *s_scan = (int *)(bars + C::NBARS);  // pieces in the streams' tables
+  uint32_t *s_tmem = (uint32_t *)(s_scan + 2);
+  volatile int *s_fail = s_scan + 3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   if (smem_addr(sm) & 1023) {
@@ -580,167 +579,131 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
   for (int base = 0;; base += RV_PFX_TABLE) {
   // ------------------------------------------------ the next pieces
   // (Planned from the lengths each time, so that nothing of it stays in
-  // registers while the roles run.)
-  // Tiles of a run of sequences, and how many have any.
-  const int run = ((int)a.n_seqs + RV_PFX_THREADS - 1) / RV_PFX_THREADS;
-  const int b0 = min((int)threadIdx.x * run, (int)a.n_seqs), b1 = min(b0 + run, (int)a.n_seqs);
-  int mine = 0, filled = 0;
-  for (int b = b0; b < b1; b++) {
-    const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
-    mine += t;
-    filled += t != 0;
-  }
-  int before = mine, fbefore = filled;
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(RV_FULL, before, o), f = __shfl_up_sync(RV_FULL, fbefore, o);
-    if (lane >= o) {
-      before += v;
-      fbefore += f;
+  // registers while the roles run.)  Every warp adds up the lengths for itself;
+  // warps 2 and 3 write the streams' pieces, a sequence a lane.
+  bool pair;
+  {
+    int all = 0, fall = 0;
+    for (uint32_t b = lane; b < ((a.n_seqs + 31) & ~31u); b += 32) {
+      const int t = b < a.n_seqs ? pfx_tiles(prefix_suffix_len(a, b)) : 0;
+      all += t;
+      fall += t != 0;
+    }
+    all = __reduce_add_sync(RV_FULL, all);
+    fall = __reduce_add_sync(RV_FULL, fall);
+    const PfxLine line = pfx_line(a, w, all, fall);
+    pair = (int)blockIdx.x < line.gp;
+    const int segs = (int)a.n_kv * w.nrt_s;
+    const bool cums = blockIdx.x == 0 && base == 0 && warp == 1;
+    if (cums || warp == 2 || warp == 3) {
+      const int s = warp - 2, ov_p = pair ? 0 : RV_PFX_OV, len_p = w.tp + ov_p;
+      const int seg_p = pair || line.solo_p ? (int)a.n_kv * w.nrt_p : 0;  // prefix segments on this CTA's line
+      // Solo streams: first stream 0 of every CTA, then stream 1, so few units
+      // spread over all SMs.
+      PfxStretch k;
+      k.v = pair ? (int)blockIdx.x : (int)blockIdx.x - line.gp + s * (w.grid - line.gp);
+      const int end = pair ? line.wp : line.w, per = pair ? line.per_p : line.per;
+      k.u = min(end, k.v * per);
+      k.end = min(end, k.u + per);
+      // The first and last segment of the stretch, counted along the line.
+      const int lim = seg_p * len_p;
+      int g0 = -1, g1 = -1;
+      if (k.u < min(k.end, lim)) {
+        g0 = k.u / len_p;
+        g1 = (min(k.end, lim) - 1) / len_p;
+      }
+      PfxPiece p{};
+      if (g0 >= 0 && g0 + base + lane <= g1) {
+        const int g = g0 + base + lane, kvh = g / w.nrt_p;
+        p.head = 2 * kvh;
+        p.row0 = (g - kvh * w.nrt_p) * w.sr_p;
+        p.keys = (int)a.prefix_len;
+        p.part = (g + k.v) * (pair ? 2 : 1);
+        pfx_cut(p, k, g * len_p, w.tp, ov_p);
+      }
+      if (!cums) tab[s][lane] = p;
+      __syncwarp();
+      if (cums || (!pair && k.end > lim && k.u < k.end)) {
+        int x0 = line.solo_p, c0 = 0, f0 = 0;  // the place, tiles and filled sequences before the 32
+        for (uint32_t b0 = 0; b0 < a.n_seqs && (cums || x0 < k.end); b0 += 32) {
+          const int b = (int)b0 + lane, keys = b < (int)a.n_seqs ? prefix_suffix_len(a, (uint32_t)b) : 0;
+          const int t = pfx_tiles(keys), len = t ? t + RV_PFX_OV : 0;
+          int upto = t;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(RV_FULL, upto, o);
+            if (lane >= o) upto += v;
+          }
+          const uint32_t some = __ballot_sync(RV_FULL, t != 0);
+          const int c = c0 + upto - t, f = f0 + __popc(some & ((1u << lane) - 1));
+          const int x = line.solo_p + (c + f * RV_PFX_OV) * segs;  // where the sequence's segments begin
+          if (cums) {
+            if (b < (int)a.n_seqs) {
+              w.cum[b] = c;
+              w.cum[a.n_seqs + 1 + b] = f;
+            }
+          } else {
+            const int lo = max(k.u, x), hi = min(k.end, x + len * segs);  // its places on the stretch
+            const uint32_t hit = __ballot_sync(RV_FULL, lo < hi);
+            if (hit) {
+              const int l0 = lo < hi ? (lo - x) / len : 0, l1 = lo < hi ? (hi - 1 - x) / len : -1, g = seg_p + b * segs;
+              if (g0 < 0) g0 = __shfl_sync(RV_FULL, g + l0, __ffs(hit) - 1);
+              g1 = __shfl_sync(RV_FULL, g + l1, 31 - __clz(hit));
+              for (int i = max(l0, g0 + base - g); i <= min(l1, g0 + base + RV_PFX_TABLE - 1 - g); i++) {
+                const int kvh = i / w.nrt_s;
+                p.b = b;
+                p.head = 2 * kvh + 1;
+                p.row0 = (i - kvh * w.nrt_s) * w.sr_s;
+                p.keys = keys;
+                p.part = b * segs + i + k.v;
+                pfx_cut(p, k, x + i * len, t, RV_PFX_OV);
+                tab[s][g + i - g0 - base] = p;
+              }
+            }
+          }
+          c0 = __shfl_sync(RV_FULL, c + t, 31);
+          f0 += __popc(some);
+          x0 = line.solo_p + (c0 + f0 * RV_PFX_OV) * segs;
+        }
+        if (cums && lane == 0) {
+          w.cum[a.n_seqs] = c0;
+          w.cum[2 * a.n_seqs + 1] = f0;
+        }
+      }
+      if (!cums && lane == 0) s_scan[s] = g0 < 0 ? 0 : min(max(g1 - g0 + 1 - base, 0), RV_PFX_TABLE);
     }
   }
-  if (lane == 31) {
-    s_scan[warp] = before;
-    s_scan[16 + warp] = fbefore;
-  }
-  if (threadIdx.x < 4) s_scan[32 + threadIdx.x] = threadIdx.x & 1 ? -1 : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int all = 0, fall = 0;
-#pragma unroll
-  for (int i = 0; i < RV_PFX_THREADS / 32; i++) {
-    const int v = s_scan[i], f = s_scan[16 + i];
-    if (i < warp) {
-      before += v;
-      fbefore += f;
-    }
-    all += v;
-    fall += f;
-  }
-  before -= mine;
-  fbefore -= filled;
-  const PfxLine line = pfx_line(a, w, all, fall);
-  const bool pair = (int)blockIdx.x < line.gp;
-  const int segs = (int)a.n_kv * w.nrt_s, ov_p = pair ? 0 : RV_PFX_OV, len_p = w.tp + ov_p;
-  const int seg_p = pair || line.solo_p ? (int)a.n_kv * w.nrt_p : 0;  // prefix segments on this CTA's line
-  PfxStretch str[2];
-#pragma unroll
-  for (int s = 0; s < 2; s++) {
-    PfxStretch &k = str[s];
-    // Solo streams: first stream 0 of every CTA, then stream 1, so few units
-    // spread over all SMs.
-    k.v = pair ? (int)blockIdx.x : (int)blockIdx.x - line.gp + s * (w.grid - line.gp);
-    const int end = pair ? line.wp : line.w, per = pair ? line.per_p : line.per;
-    k.u = min(end, k.v * per);
-    k.end = min(end, k.u + per);
-  }
-  if (blockIdx.x == 0 && base == 0) {
-    int x = before, f = fbefore;
-    for (int b = b0; b < b1; b++) {
-      w.cum[b] = x;
-      w.cum[a.n_seqs + 1 + b] = f;
-      const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b));
-      x += t;
-      f += t != 0;
-    }
-    if (threadIdx.x == 0) {
-      w.cum[a.n_seqs] = all;
-      w.cum[2 * a.n_seqs + 1] = fall;
-    }
-  }
-  // The segments that hold a stretch's first and last place.
-  if (!pair) {
-    int x = line.solo_p + (before + fbefore * RV_PFX_OV) * segs;
-    for (int b = b0; b < b1; b++) {
-      const int t = pfx_tiles(prefix_suffix_len(a, (uint32_t)b)), len = t ? t + RV_PFX_OV : 0;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const PfxStretch &k = str[i >> 1];
-        const int u = i & 1 ? k.end - 1 : k.u;
-        if (k.u < k.end && u >= x && u < x + len * segs) s_scan[32 + i] = seg_p + b * segs + (u - x) / len;
-      }
-      x += len * segs;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int s = 0; s < 2; s++) {
-    PfxStretch &k = str[s];
-    const int lim = seg_p * len_p;
-    k.g0 = k.u < lim ? k.u / len_p : s_scan[32 + 2 * s];
-    k.g1 = k.u >= k.end ? k.g0 - 1 : k.end - 1 < lim ? (k.end - 1) / len_p : s_scan[33 + 2 * s];
-  }
-  int count[2];
-#pragma unroll
-  for (int s = 0; s < 2; s++) count[s] = min(max(str[s].g1 - str[s].g0 + 1 - base, 0), RV_PFX_TABLE);
+  const int count[2] = {s_scan[0], s_scan[1]};
   if (count[0] + count[1] == 0) break;
-  for (int i = threadIdx.x; i < 2 * RV_PFX_TABLE; i += RV_PFX_THREADS) {
-    const int s = i / RV_PFX_TABLE, idx = i % RV_PFX_TABLE;
-    const PfxStretch &k = s ? str[1] : str[0];
-    const int g = k.g0 + base + idx;
-    PfxPiece p{};
-    if (g < seg_p && g <= k.g1) {
-      const int kvh = g / w.nrt_p;
-      p.head = 2 * kvh;
-      p.row0 = (g - kvh * w.nrt_p) * w.sr_p;
-      p.keys = (int)a.prefix_len;
-      p.part = (g + k.v) * (pair ? 2 : 1);
-      pfx_cut(p, k, g * len_p, w.tp, ov_p);
-    }
-    tab[s][idx] = p;
-  }
-  __syncthreads();
-  if (!pair) {
-    int x = line.solo_p + (before + fbefore * RV_PFX_OV) * segs;
-    for (int b = b0; b < b1; b++) {
-      const int keys = prefix_suffix_len(a, (uint32_t)b), t = pfx_tiles(keys), len = t ? t + RV_PFX_OV : 0;
-#pragma unroll
-      for (int s = 0; s < 2; s++) {
-        const PfxStretch &k = str[s];
-        const int g = seg_p + b * segs, lo = max(0, k.g0 + base - g),
-                  hi = min(segs - 1, min(k.g1, k.g0 + base + RV_PFX_TABLE - 1) - g);
-        if (t)
-          for (int local = lo; local <= hi; local++) {
-            PfxPiece p{};
-            const int kvh = local / w.nrt_s;
-            p.b = b;
-            p.head = 2 * kvh + 1;
-            p.row0 = (local - kvh * w.nrt_s) * w.sr_s;
-            p.keys = keys;
-            p.part = b * segs + local + k.v;
-            pfx_cut(p, k, x + local * len, t, RV_PFX_OV);
-            tab[s][g + local - k.g0 - base] = p;
-          }
-      }
-      x += len * segs;
-    }
-    __syncthreads();
-  }
-
   const uint32_t tmem = *s_tmem;
   if (warp < 4) {
-    if (!Q8 && warp == 0 && lane == 0) {
+    if (!Q8 && warp == 0) {
+    if (elect_one()) {
       // ---------------------------------------------------------- loads
       PfxFeed &f = feed;
-      pfx_feed_start(f);
-      for (; ok && !*s_fail && pfx_feed(tab, count, pair ? 1 : 2, f); n++) {
+      pfx_feed_start(tab, count, pair, f);
+      for (; ok && !*s_fail && pfx_feed(tab, count, pair, f); n++) {
         const int slot = n % R;
         if (!mbar_wait_bounded(&kv_empty[slot], ((n / R) & 1) ^ 1)) {
           ok = false;
           break;
         }
         mbar_arrive_expect_tx(&kv_full[slot], (uint32_t)TILE);
-        const PfxPiece &p = tab[f.s][f.entry];
-        const bool suffix = p.head & 1;
+        const bool suffix = f.head & 1;
         const CUtensorMap *m = suffix ? (f.is_k ? &map_sk : &map_sv) : (f.is_k ? &map_pk : &map_pv);
 #pragma unroll
         for (int h = 0; h < D / 64; h++)
-          tma_load_4d(ring + (size_t)slot * TILE + h * (RV_PFX_N * 128), m, 64 * h, p.head >> 1, f.tile * RV_PFX_N, p.b,
+          tma_load_4d(ring + (size_t)slot * TILE + h * (RV_PFX_N * 128), m, 64 * h, f.head >> 1, f.tile * RV_PFX_N, f.b,
                       &kv_full[slot]);
       }
       if (!ok) *s_fail = 1;
       if (*s_fail)  // let the copies in flight land before the CTA ends
         for (int i = max(0, n - R); i < n; i++) mbar_wait_bounded(&kv_full[i % R], (i / R) & 1);
+    }
+    __syncwarp();
+    n = __reduce_max_sync(RV_FULL, n);  // another lane may be elected in the next plan
     } else if (warp == 1) {
       // ----------------------------------------------------- MMA issue
       const uint32_t hi_sw = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -871,7 +834,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       constexpr int TPT = D / 16, LOADS = RV_PFX_N * TPT, IT = (LOADS + RV_PFX_CONV - 1) / RV_PFX_CONV;
       const int ct = (warp == 0 ? 0 : 32 * (warp - 1)) + lane;
       PfxFeed &f = feed;
-      pfx_feed_start(f);
+      pfx_feed_start(tab, count, pair, f);
       // A tile on its way: its scales in registers.
       struct Load {
         float ks[2], vs[2];
@@ -879,11 +842,10 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       } cur, nxt;
       uint8_t *raw = sm + C::raw;
       const auto fetch = [&](Load &o, int half) {
-        if (!pfx_feed(tab, count, pair ? 1 : 2, f)) return false;
-        const PfxPiece &p = tab[f.s][f.entry];
-        const bool suffix = p.head & 1;
-        const int kvh = p.head >> 1, valid = min(RV_PFX_N, p.keys - f.tile * RV_PFX_N);
-        const size_t first = (size_t)p.b * a.cap * suffix + (size_t)f.tile * RV_PFX_N;
+        if (!pfx_feed(tab, count, pair, f)) return false;
+        const bool suffix = f.head & 1;
+        const int kvh = f.head >> 1, valid = min(RV_PFX_N, f.keys - f.tile * RV_PFX_N);
+        const size_t first = (size_t)f.b * a.cap * suffix + (size_t)f.tile * RV_PFX_N;
         const int8_t *src = (const int8_t *)(f.is_k ? (suffix ? a.sk : a.pk) : (suffix ? a.sv : a.pv)) +
                             (first * a.n_kv + kvh) * D;
         const size_t pitch = (size_t)a.n_kv * D;
@@ -896,7 +858,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                          : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        o.at = f.is_k ? f.s * SLOTS + f.u % SLOTS : -1;
+        o.at = f.is_k ? f.stream * SLOTS + f.unit % SLOTS : -1;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           o.ks[j] = o.vs[j] = 0;
@@ -1120,14 +1082,8 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                 const int e = 32 * ch + 2 * j;
                 float2 x = make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
                 x = Q8 ? add_f32x2(x, m2) : fma_f32x2(x, c2, m2);
-                // Every fourth pair on the FMA units: the exponentials' own unit
-                // is what bounds a stream (f32 needs its accuracy).
-                if (!PRECISE && (j & 3) == 3) {
-                  x = ex2_poly(x);
-                } else {
-                  x.x = ex2(x.x);
-                  x.y = ex2(x.y);
-                }
+                x.x = ex2(x.x);
+                x.y = ex2(x.y);
                 l2[j & 1] = add_f32x2(l2[j & 1], x);
                 if constexpr (Q8)
                   x = fma_f32x2(x, *(const float2 *)(sc + RV_PFX_N + 64 * h + e), make_float2(0, 0));
