@@ -2852,6 +2852,10 @@ static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t 
   w.o_p = (float4 *)(scratch + o.o_p);
   w.o_s = (float4 *)(scratch + o.o_s);
   const size_t eb = sizeof(T);
+  // What a paired unit costs a CTA, in solo places (measured, f16 caches: 5.3
+  // and 2.5 thousand cycles; 8-bit caches, where the conversion of twice the
+  // tiles bounds solo streams: 4.3 and 7).
+  w.pair_cost = Q8 ? 1.3f : 2.0f;
   w.q_aligned = (((uintptr_t)a.q | a.q_seq_stride * eb | a.q_token_stride * eb) & 15) == 0;
   w.out_aligned = ((uintptr_t)a.out & 15) == 0;
   CUtensorMap m[4] = {};

@@ -171,6 +171,7 @@ struct PfxWork {
   int nrt_p, nrt_s;    // segments per kv head (per sequence)
   int rw_p, rw_s;      // rows of a part
   int pair;            // the prefix runs on paired streams
+  float pair_cost;     // a paired unit's cost in solo places
   PfxDiv by_g, by_row; // divisions by the query heads of a kv head, by the query rows of a sequence's
   int grid;
   int q_aligned, out_aligned;  // 16-byte loads and stores
@@ -194,11 +195,10 @@ RV_DEVFN PfxLine pfx_line(const PrefixArgs &a, const PfxWork &w, int tiles, int 
   l.solo_p = w.pair || w.tp == 0 ? 0 : seg_p * (w.tp + RV_PFX_OV);
   l.wp = w.pair ? seg_p * w.tp : 0;
   l.w = l.solo_p + suffix;
-  // A paired unit costs a CTA about two solo places (measured: 5.3 and 2.5
-  // thousand cycles), and a paired segment three units more.
+  // A paired segment costs about three units more than its own.
   l.gp = 0;
   if (l.wp) {
-    const float cost = __fmul_rn(2.0f, (float)(l.wp + 3 * seg_p)), share = __fdiv_rn(cost, __fadd_rn(cost, (float)l.w));
+    const float cost = __fmul_rn(w.pair_cost, (float)(l.wp + 3 * seg_p)), share = __fdiv_rn(cost, __fadd_rn(cost, (float)l.w));
     l.gp = min(max(__float2int_rn(__fmul_rn(share, (float)w.grid)), 1), l.w ? w.grid - 1 : w.grid);
   }
   l.per_p = l.gp ? (l.wp + l.gp - 1) / l.gp : 1;
