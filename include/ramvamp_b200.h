@@ -719,7 +719,10 @@ RV_API int rv_kv_read(const rv_kv_cache *cache, int dtype, size_t n, const int32
  * device int32 [n_seqs], the suffix lengths with the n_q newest tokens (the
  * queries' own) counted.  Token i of sequence b sees the whole prefix and
  * suffix positions 0..lens[b]-n_q+i (none when that is negative); a row that
- * sees nothing is written as zeros.  q: device, dtype RV_F32 or RV_F16,
+ * sees nothing is written as zeros.  Nothing outside what a row sees reaches
+ * it, infinities and NaN included; in an f16 cache a value row of the n_q newest
+ * tokens that is not finite makes the whole output row NaN for the queries that
+ * see it.  q: device, dtype RV_F32 or RV_F16,
  * element (b, i, h, d) at b*q_seq_stride + i*q_token_stride + h*head_dim + d;
  * query head h reads kv head h / (n_heads / n_kv_heads); out: device,
  * [n_seqs][n_q][n_heads][head_dim] contiguous, the same dtype.  scratch:

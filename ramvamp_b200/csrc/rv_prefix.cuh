@@ -9,7 +9,7 @@
 // l = sum exp(s_j - m) and o = sum exp(s_j - m) v_j, and the parts add up as
 // sum_p exp(m_p - M) (l_p, o_p) with M = max m_p.  A row that sees nothing is 0.
 #pragma once
-#include <type_traits>
+#include <limits.h>
 
 #include "rv_kv.cuh"
 #include "rv_tc.cuh"
@@ -198,7 +198,8 @@ RV_DEVFN PfxLine pfx_line(const PrefixArgs &a, const PfxWork &w, int tiles, int 
   // A paired segment costs about three units more than its own.
   l.gp = 0;
   if (l.wp) {
-    const float cost = __fmul_rn(w.pair_cost, (float)(l.wp + 3 * seg_p)), share = __fdiv_rn(cost, __fadd_rn(cost, (float)l.w));
+    const float cost = __fmul_rn(w.pair_cost, (float)(l.wp + 3 * seg_p));
+    const float share = __fdiv_rn(cost, __fadd_rn(cost, (float)l.w));
     l.gp = min(max(__float2int_rn(__fmul_rn(share, (float)w.grid)), 1), l.w ? w.grid - 1 : w.grid);
   }
   l.per_p = l.gp ? (l.wp + l.gp - 1) / l.gp : 1;
@@ -236,7 +237,7 @@ struct PfxCfg {
   static constexpr int NBARS = 2 * R + 8 + 2 * RV_PFX_SCALE_SLOTS + 1;
   static constexpr size_t ring = 2 * QS, raw = ring + (size_t)R * TILE, scales = raw + RAW, table = scales + SCALES,
                           ups = table + 2 * RV_PFX_TABLE * sizeof(PfxPiece), bars = ups + (PRECISE ? 4 * SR : 0);
-  static constexpr size_t total = bars + NBARS * 8 + 4 * 4;
+  static constexpr size_t total = bars + NBARS * 8 + 8 * 4;
   static_assert(total <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
            *q_ready = o_full + 2, *sc_full = q_ready + 2, *drained = sc_full + 2 * SLOTS;
   int *s_scan = (int *)(bars + C::NBARS);  // pieces in the streams' tables
   uint32_t *s_tmem = (uint32_t *)(s_scan + 2);
-  volatile int *s_fail = s_scan + 3;
+  volatile int *s_fail = s_scan + 3, *s_bad = s_scan + 4;  // s_bad: [stream]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   if (smem_addr(sm) & 1023) {
@@ -744,6 +745,30 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                   *(uint4 *)(ring + (size_t)(nv % R) * TILE + (ch >> 3) * (RV_PFX_N * 128) + tc_sw_off(r, ch & 7)) =
                       make_uint4(0, 0, 0, 0);
                 }
+                fence_proxy_async();
+                __syncwarp();
+              }
+              if (!Q8 && a.n_q > 1 && (p->head & 1)) {
+                // Values among the sequence's newest tokens are hidden from some
+                // of its queries, and 0 * NaN is not 0: a row that is not finite
+                // is taken out here, and its first key kept for the queries that
+                // see it, whose outputs become NaN.
+                int bad = c.j == 0 ? INT_MAX : s_bad[s];
+                const int hidden = p->keys - (int)a.n_q + 1 - (p->tile0 + c.j) * RV_PFX_N;
+                for (int r = max(hidden, 0); r < valid; r++) {
+                  uint4 *x = (uint4 *)(ring + (size_t)(nv % R) * TILE + (lane >> 3) * (RV_PFX_N * 128) +
+                                       tc_sw_off(r, lane & 7));
+                  uint4 v = make_uint4(0, 0, 0, 0);
+                  if (lane < D / 8) v = *x;
+                  const auto odd = [](uint32_t u) {
+                    return (u & 0x7C00u) == 0x7C00u || (u & 0x7C000000u) == 0x7C000000u;
+                  };
+                  if (__any_sync(RV_FULL, odd(v.x) || odd(v.y) || odd(v.z) || odd(v.w))) {
+                    if (lane < D / 8) *x = make_uint4(0, 0, 0, 0);
+                    bad = min(bad, (p->tile0 + c.j) * RV_PFX_N + r);
+                  }
+                }
+                if (lane == 0) s_bad[s] = bad;
                 fence_proxy_async();
                 __syncwarp();
               }
@@ -947,7 +972,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     pfx_entry(mytab, mycount, at, left);
     // What the piece before leaves, written while this one's first scores are
     // on their way.
-    int p_head = 0, p_part = -1;
+    int p_head = 0, p_part = -1, p_seen = 0;
     bool p_on = false, p_warp = false;
     float p_m = 0, p_l = 0;
 #pragma unroll 1
@@ -957,10 +982,11 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         const int rw = p_head & 1 ? w.rw_s : w.rw_p;
         const size_t part = (size_t)p_part + (pair ? s : 0);
         float4 *po = (p_head & 1 ? w.o_s : w.o_p) + part * (D / 4) * rw + row;
-        if (p_on) (p_head & 1 ? w.ml_s : w.ml_p)[part * rw + row] = make_float2(p_m, p_l);
         ok = pfx_wait(&o_full[s], (piece - 1) & 1);
         if (!ok) break;
         tc_fence_after();
+        if (!Q8 && a.n_q > 1 && (p_head & 1) && p_seen > s_bad[s]) p_l = __uint_as_float(0x7FC00000u);
+        if (p_on) (p_head & 1 ? w.ml_s : w.ml_p)[part * rw + row] = make_float2(p_m, p_l);
         if (p_warp) {
 #pragma unroll 1
           for (int ch = 0; ch < D / 16; ch++) {
@@ -1111,6 +1137,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       p_head = p.head;
       p_part = p.part;
       p_on = on;
+      p_seen = seen;
       p_warp = warp_on;
       p_m = m_ref == -INFINITY ? -INFINITY : m_ref - RV_PFX_LIFT;
       p_l = l;

@@ -299,6 +299,31 @@ def test_attention_values_that_are_not_finite_reach_their_rows_only(rv):
     assert torch.isfinite(out[:, :, :4]).all() and not torch.isfinite(out[:, :, 4:]).any()
 
 
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_Q8"])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_later_tokens_do_not_reach_earlier_queries(rv, fmt, dim, bad):
+    """Of five new tokens the fourth has a value (then a key) that is not
+    finite: the first three queries are the same bits as without it, the last
+    two are not finite (but for a key of infinite scale, whose scores may be
+    -infinity: then it weighs nothing)."""
+    fmt = getattr(rv, fmt)
+    for length in (5, 126, 131, 260):
+        outs = []
+        for where in (None, "v", "k"):
+            pre, suf = make_caches(rv, 2, 300, 2, dim, 130, fmt, 51)
+            if where:
+                planes = (getattr(suf, where) if fmt == rv.KV_F16 else getattr(suf, where + "_scale"))
+                planes[1, length - 2] = bad
+            q = torch.randn(2, 5, 8, dim, device="cuda", generator=gen(52))
+            outs.append([rv.prefix_attention(q.to(t), pre, 130, suf, i32([300, length])) for t in (torch.float32, torch.float16)])
+        for where, with_bad in zip("vk", outs[1:]):
+            for clean, got in zip(outs[0], with_bad):
+                assert torch.equal(got[0], clean[0]) and torch.equal(got[1, :3], clean[1, :3])
+                if where == "v" or fmt == rv.KV_F16 or math.isnan(bad):
+                    assert not torch.isfinite(got[1, 3:]).all(-1).any()
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_attention_large_scores_and_sinks(rv, dim, dtype):
