@@ -21,6 +21,7 @@
 #include "rv_internal.cuh"
 
 #define RV_KV_THREADS 256
+#define RV_KV_UNROLL 2
 #define RV_KV_TINY 0x1p-50f
 
 struct KvArgs {
@@ -75,43 +76,65 @@ RV_DEVFN long long kv_position(const KvArgs &a, uint32_t b, uint32_t i) {
   return pos < 0 ? -1 : pos;
 }
 
-// Rows into the cache.  grid = (row blocks of one sequence, sequences, 2: keys
-// and values).
+// Both kernels move RV_KV_UNROLL rows a thread (their loads in flight together).
+// grid = (row blocks of one sequence, sequences, 2: keys and values).
+struct KvRow {
+  uint32_t i, h;
+  long long pos;
+  size_t at;  // the row in the cache
+};
+RV_DEVFN KvRow kv_row(const KvArgs &a, uint32_t b, int u) {
+  const uint32_t per = RV_KV_THREADS / a.lanes, row = (blockIdx.x * RV_KV_UNROLL + u) * per + threadIdx.x / a.lanes;
+  KvRow r;
+  r.i = row / a.n_kv;
+  r.h = row - r.i * a.n_kv;
+  r.pos = r.i < a.n ? kv_position(a, b, r.i) : -1;
+  r.at = ((size_t)b * a.capacity + (size_t)(r.pos < 0 ? 0 : r.pos)) * a.n_kv + r.h;
+  return r;
+}
+
+// Rows into the cache.
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(RV_KV_THREADS) k_kv_append(KvArgs a) {
-  const uint32_t per = RV_KV_THREADS / a.lanes, lane = threadIdx.x % a.lanes;
-  const uint32_t row = blockIdx.x * per + threadIdx.x / a.lanes, b = blockIdx.y;
-  const uint32_t i = row / a.n_kv, h = row - i * a.n_kv, e = lane * 8;
+  const uint32_t lane = threadIdx.x % a.lanes, b = blockIdx.y, e = lane * 8;
   const bool val = blockIdx.z != 0;
-  // Every lane of a row's group reaches the shuffles.
-  const long long pos = i < a.n ? kv_position(a, b, i) : -1;
-  const bool on = pos >= 0 && e < a.hd;
-  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (on)
-    kv_load8((const T *)(val ? a.v_io : a.k_io) + b * a.seq_stride + i * a.token_stride + (size_t)h * a.hd + e, a.aligned,
-             x);
-  const size_t at = ((size_t)b * a.capacity + (size_t)(pos < 0 ? 0 : pos)) * a.n_kv + h;
-  if constexpr (!Q8) {
-    if (on) kv_store8((__half *)(val ? a.v : a.k) + at * a.hd + e, true, x);
-  } else {
-    // max |x| as bits: for non-negative floats the integer order is the
-    // float order with NaN above infinity, so a NaN is not lost.
-    uint32_t m = 0;
+  float x[RV_KV_UNROLL][8];
+  KvRow r[RV_KV_UNROLL];
 #pragma unroll
-    for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-    for (uint32_t o = a.lanes / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(RV_FULL, m, o));
-    const float amax = __uint_as_float(m);
-    const bool zero = amax < RV_KV_TINY;
-    const float inv = zero ? 0.0f : __fmul_rn(__frcp_rn(amax), 127.0f);
-    uint32_t w[2] = {0, 0};
+  for (int u = 0; u < RV_KV_UNROLL; u++) {
+    r[u] = kv_row(a, b, u);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int level = __float2int_rn(__fmul_rn(x[j], inv));  // NaN -> 0
-      w[j >> 2] |= (uint32_t)(level & 255) << (8 * (j & 3));
-    }
-    if (on) {
-      *(uint2 *)((int8_t *)(val ? a.v : a.k) + at * a.hd + e) = make_uint2(w[0], w[1]);
-      if (lane == 0) (val ? a.v_scale : a.k_scale)[at] = zero ? 0.0f : __fmul_rn(amax, 1.0f / 127.0f);
+    for (int j = 0; j < 8; j++) x[u][j] = 0;
+    if (r[u].pos >= 0 && e < a.hd)
+      kv_load8((const T *)(val ? a.v_io : a.k_io) + b * a.seq_stride + r[u].i * a.token_stride + (size_t)r[u].h * a.hd + e,
+               a.aligned, x[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < RV_KV_UNROLL; u++) {
+    const bool on = r[u].pos >= 0 && e < a.hd;
+    if constexpr (!Q8) {
+      if (on) kv_store8((__half *)(val ? a.v : a.k) + r[u].at * a.hd + e, true, x[u]);
+    } else {
+      // max |x| as bits: for non-negative floats the integer order is the
+      // float order with NaN above infinity, so a NaN is not lost.  Every lane
+      // of a row's group reaches the shuffles.
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(x[u][j]) & 0x7FFFFFFFu);
+      for (uint32_t o = a.lanes / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(RV_FULL, m, o));
+      const float amax = __uint_as_float(m);
+      const bool zero = amax < RV_KV_TINY;
+      const float inv = zero ? 0.0f : __fmul_rn(__frcp_rn(amax), 127.0f);
+      uint32_t w[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int level = __float2int_rn(__fmul_rn(x[u][j], inv));  // NaN -> 0
+        w[j >> 2] |= (uint32_t)(level & 255) << (8 * (j & 3));
+      }
+      if (on) {
+        *(uint2 *)((int8_t *)(val ? a.v : a.k) + r[u].at * a.hd + e) = make_uint2(w[0], w[1]);
+        if (lane == 0) (val ? a.v_scale : a.k_scale)[r[u].at] = zero ? 0.0f : __fmul_rn(amax, 1.0f / 127.0f);
+      }
     }
   }
 }
@@ -120,24 +143,36 @@ __global__ void __launch_bounds__(RV_KV_THREADS) k_kv_append(KvArgs a) {
 // A row without a position is written as zeros.
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(RV_KV_THREADS) k_kv_read(KvArgs a) {
-  const uint32_t per = RV_KV_THREADS / a.lanes, e = threadIdx.x % a.lanes * 8;
-  const uint32_t row = blockIdx.x * per + threadIdx.x / a.lanes, b = blockIdx.y;
-  const uint32_t i = row / a.n_kv, h = row - i * a.n_kv;
+  const uint32_t b = blockIdx.y, e = threadIdx.x % a.lanes * 8;
   const bool val = blockIdx.z != 0;
-  if (i >= a.n || e >= a.hd) return;
-  const long long pos = kv_position(a, b, i);
-  float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (pos >= 0) {
-    const size_t at = ((size_t)b * a.capacity + (size_t)pos) * a.n_kv + h;
-    if constexpr (Q8) {
-      const uint2 w = *(const uint2 *)((const int8_t *)(val ? a.v : a.k) + at * a.hd + e);
-      const float s = (val ? a.v_scale : a.k_scale)[at];
+  float x[RV_KV_UNROLL][8], s[RV_KV_UNROLL];
+  uint2 w[RV_KV_UNROLL];
+  KvRow r[RV_KV_UNROLL];
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-        x[j] = __fmul_rn((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))), s);
-    } else {
-      kv_load8((const __half *)(val ? a.v : a.k) + at * a.hd + e, true, x);
+  for (int u = 0; u < RV_KV_UNROLL; u++) {
+    r[u] = kv_row(a, b, u);
+    w[u] = make_uint2(0, 0);
+    s[u] = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[u][j] = 0;
+    if (r[u].pos >= 0 && e < a.hd) {
+      if constexpr (Q8) {
+        w[u] = *(const uint2 *)((const int8_t *)(val ? a.v : a.k) + r[u].at * a.hd + e);
+        s[u] = (val ? a.v_scale : a.k_scale)[r[u].at];
+      } else {
+        kv_load8((const __half *)(val ? a.v : a.k) + r[u].at * a.hd + e, true, x[u]);
+      }
     }
   }
-  kv_store8((T *)(val ? a.v_io : a.k_io) + b * a.seq_stride + i * a.token_stride + (size_t)h * a.hd + e, a.aligned, x);
+#pragma unroll
+  for (int u = 0; u < RV_KV_UNROLL; u++) {
+    if constexpr (Q8) {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        x[u][j] = __fmul_rn((float)(int8_t)((j < 4 ? w[u].x : w[u].y) >> (8 * (j & 3))), s[u]);
+    }
+    if (r[u].i < a.n && e < a.hd)
+      kv_store8((T *)(val ? a.v_io : a.k_io) + b * a.seq_stride + r[u].i * a.token_stride + (size_t)r[u].h * a.hd + e,
+                a.aligned, x[u]);
+  }
 }

@@ -2704,7 +2704,7 @@ static int kv_rows_args(const char *what, const rv_kv_cache *c, int dtype, const
   a->lanes = 1;
   while (a->lanes * 8 < c->head_dim) a->lanes *= 2;
   a->aligned = ((((uintptr_t)k | (uintptr_t)v) | token_stride * eb | seq_stride * eb) & 15) == 0;
-  const size_t per = RV_KV_THREADS / a->lanes, rows = n * c->n_kv_heads;
+  const size_t per = RV_KV_THREADS / a->lanes * RV_KV_UNROLL, rows = n * c->n_kv_heads;
   if (rows > 0xFFFFFFFFull - per) RV_FAIL(RV_ERR_UNIMPLEMENTED, "%s: %zu rows of one sequence", what, rows);
   *grid = dim3((unsigned)((rows + per - 1) / per), c->n_seqs, 2);
   return ensure_current_device();
