@@ -874,12 +874,11 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
     if s[3] != 1 or (s[2] != D and H > 1):
         raise KernelError(5, "LengthMismatch: the heads of a query token must be contiguous")
     if out is None:
-        out = torch.empty((n, n_q, H, D), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, n_q, H, D))
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise KernelError(5, "LengthMismatch: out must be contiguous and like q in shape and type")
     if scratch is None:
-        scratch = torch.empty(prefix_attention_scratch(n, n_q, H, suffix.n_kv_heads, D), dtype=torch.uint8,
-                              device=q.device)
+        scratch = q.new_empty(prefix_attention_scratch(n, n_q, H, suffix.n_kv_heads, D), dtype=torch.uint8)
     _check(lib().rv_prefix_attention(prefix._ref if prefix is not None else None, prefix_len, suffix._ref,
                                      _i32(lens, n, "lens"), _dtype(q), q.data_ptr(), s[0], s[1], n_q, H,
                                      D ** -0.5 if scale is None else scale, out.data_ptr(), scratch.data_ptr(),

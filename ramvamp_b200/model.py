@@ -20,9 +20,10 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
-from . import (AttnEngine, ExpertTable, MoeEngine, QuantFormat, QWEN3_Q6K_DOWN_LAYERS, _check, _p, _stream,
-               attn_weights, dequantize_rows, gemv_q8_k, lib, qwen3_layer_layout, quantize_row_q8_0,
-               quantize_weights, rmsnorm_quantize, synth_normal)
+from . import (AttnEngine, ExpertTable, KV_F16, KV_Q8, KvCache, MoeEngine, QuantFormat, QWEN3_Q6K_DOWN_LAYERS, _check,
+               _p, _stream, attn_weights, dequantize_rows, gemv_q8_0_batched, gemv_q8_k, gemv_q8_k_batched, kv_append,
+               kv_read, lib, prefix_attention, prefix_attention_scratch, qwen3_layer_layout, quantize_row_q8_0,
+               quantize_row_q8_k, quantize_weights, rmsnorm, rmsnorm_quantize, rope_neox_heads, sample, synth_normal)
 
 Q = QuantFormat
 
@@ -231,6 +232,111 @@ class Decoder:
         return [int(x) for x in ids[len(prompt) - 1:]]
 
 
+class ParallelDecoder:
+    """n continuations of one prompt, drawn together.  The prompt goes through
+    ``Decoder`` once; its keys and values -- the engine's own f16 caches, or
+    8-bit copies of them (``kv_format``) -- are the prefix that every
+    continuation attends to, each beside its own rows, and a token of each is
+    drawn per step.  No counterpart in the reference, whose generate/mod.rs
+    draws one sequence."""
+
+    def __init__(self, weights: Qwen3Weights, n: int, max_prompt: int = 1024, max_new: int = 1024,
+                 kv_format: int = KV_Q8, device: int = 0):
+        cfg = weights.cfg
+        self.w, self.cfg, self.n, self.device, self.kv_format = weights, cfg, n, device, kv_format
+        self.max_prompt, self.max_new = max_prompt, max_new
+        self.prompt = Decoder(weights, max_prompt, device)
+        self.prompt_len = self.new = 0
+        d = f"cuda:{device}"
+        caches = lambda n, rows: [KvCache(n, rows, cfg.n_kv_heads, cfg.head_dim, kv_format, device)  # noqa: E731
+                                  for _ in range(cfg.n_layers)]
+        self.suffix = caches(n, max_new)
+        self.prefix = caches(1, max_prompt) if kv_format != KV_F16 else \
+            [KvCache.of_engine(self.prompt.attn, l) for l in range(cfg.n_layers)]
+        self.moe = MoeEngine(cfg.hidden, cfg.moe, cfg.n_experts, cfg.top_k, cfg.norm_topk_prob, cfg.eps,
+                             max_tokens=n, device=device)
+        f32 = lambda *shape: torch.zeros(shape, dtype=torch.float32, device=d)  # noqa: E731
+        self.residual, self.normed = f32(n, cfg.hidden), f32(n, cfg.hidden)
+        self.logits = f32(n, cfg.vocab)
+        self.lens = torch.zeros(n, dtype=torch.int32, device=d)
+        self.scratch = torch.empty(prefix_attention_scratch(n, 1, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim),
+                                   dtype=torch.uint8, device=d)
+
+    def prefill(self, prompt: Sequence[int]) -> torch.Tensor:
+        """The prompt's rows into the prefix; the logits of its last token."""
+        if not 0 < len(prompt) <= self.max_prompt:
+            raise ValueError("the prompt must hold 1 to max_prompt tokens")
+        dec = self.prompt
+        dec.reset()
+        ids = torch.tensor(list(prompt), dtype=torch.int32, device=dec.token.device)
+        for i in range(len(prompt)):
+            dec.token.copy_(ids[i:i + 1])
+            dec.step()
+        if self.kv_format != KV_F16:
+            for l, cache in enumerate(self.prefix):
+                k, v = kv_read(KvCache.of_engine(dec.attn, l), len(prompt))
+                kv_append(cache, k, v)
+        self.prompt_len, self.new = len(prompt), 0
+        self.lens.zero_()
+        return dec.logits
+
+    def _rows(self, gemv, *args) -> torch.Tensor:
+        """A batched GEMV's [out_dim][n] result as rows [n, out_dim]."""
+        *head, in_dim, out_dim, acts = args
+        out = torch.empty(out_dim, self.n, dtype=torch.float32, device=self.residual.device)
+        gemv(*head, in_dim, out_dim, acts, self.n, range(out_dim), out)
+        return out.t().contiguous()
+
+    def step(self, tokens: torch.Tensor) -> torch.Tensor:
+        """One token of every continuation (int32 [n], on the device) through
+        the model (model/forward.rs:2548-2780 for each row): logits [n, vocab]."""
+        cfg, w, n = self.cfg, self.w, self.n
+        H, hd, position = cfg.hidden, cfg.head_dim, self.prompt_len + self.new
+        if self.prompt_len == 0 or self.new >= self.max_new:
+            raise ValueError("no prompt yet, or max_new tokens drawn")
+        self.new += 1
+        self.lens.add_(1)
+        dequantize_rows(Q.Q4_K, w.token_embd, H, cfg.vocab, rows=tokens, out=self.residual)
+        for l, lw in enumerate(w.layers):
+            rmsnorm(self.residual, lw.attn_norm, cfg.eps, self.normed)
+            a = quantize_row_q8_k(self.normed)
+            q = self._rows(gemv_q8_k_batched, Q.Q4_K, lw.attn_q, H, cfg.q_dim, a).view(n, 1, cfg.n_heads, hd)
+            k = self._rows(gemv_q8_0_batched, lw.attn_k, H, cfg.kv_dim, quantize_row_q8_0(self.normed))
+            k = k.view(n, 1, cfg.n_kv_heads, hd)
+            v = self._rows(gemv_q8_k_batched, lw.attn_v_format, lw.attn_v, H, cfg.kv_dim, a).view_as(k)
+            rmsnorm(q, lw.attn_q_norm, cfg.eps, q)
+            rmsnorm(k, lw.attn_k_norm, cfg.eps, k)
+            rope_neox_heads(q, n * cfg.n_heads, hd, position, cfg.rope_theta)
+            rope_neox_heads(k, n * cfg.n_kv_heads, hd, position, cfg.rope_theta)
+            kv_append(self.suffix[l], k, v, lens=self.lens)
+            o = prefix_attention(q, self.prefix[l], self.prompt_len, self.suffix[l], self.lens, scratch=self.scratch)
+            self.residual.add_(self._rows(gemv_q8_k_batched, Q.Q5_K, lw.attn_output, cfg.q_dim, H,
+                                          quantize_row_q8_k(o)))
+            self.moe.forward(w.experts, l, lw.ffn_norm, lw.router, self.residual)
+        rmsnorm(self.residual, w.output_norm, cfg.eps, self.normed)
+        self.logits.copy_(self._rows(gemv_q8_k_batched, Q.Q6_K, w.lm_head, H, cfg.vocab, quantize_row_q8_k(self.normed)))
+        return self.logits
+
+    def generate(self, prompt: Sequence[int], n_new: int, seed: int = 0, temperature: float = 1.0, top_k: int = 0,
+                 top_p: float = 1.0, min_p: float = 0.0):
+        """n continuations of `prompt` by n_new tokens: (tokens int32, logprobs
+        f32), both [n, n_new] on the device.  The uniforms come from `seed`."""
+        d = self.residual.device
+        g = torch.Generator(device=d)
+        g.manual_seed(seed)
+        u = torch.rand(n_new, self.n, device=d, generator=g)
+        full = lambda v: torch.full((self.n,), v, dtype=torch.float32, device=d)  # noqa: E731
+        filters = (full(temperature), torch.full((self.n,), top_k, dtype=torch.int32, device=d), full(top_p), full(min_p))
+        tokens = torch.empty(n_new, self.n, dtype=torch.int32, device=d)
+        logprobs = torch.empty(n_new, self.n, dtype=torch.float32, device=d)
+        logits = self.prefill(prompt).expand(self.n, -1).contiguous()
+        for i in range(n_new):
+            sample(logits, u[i], *filters, tokens=tokens[i], logprobs=logprobs[i])
+            if i + 1 < n_new:
+                logits = self.step(tokens[i])
+        return tokens.t().contiguous(), logprobs.t().contiguous()
+
+
 def kl_divergence(ref_logits, logits) -> float:
     """Full-vocab KL(p_ref || p) in f64 from two logit vectors (the
     comparison of scripts/kl_vs_reference.py)."""
@@ -254,14 +360,22 @@ def top1(logits) -> int:
 def _main(argv=None):
     """python -m ramvamp_b200.model [--layers N] [--profile-step K]: build
     the synthetic Qwen3 model, run K eager steps, then one more inside the
-    NVTX range "step" (for a profiler restricted to that range)."""
+    NVTX range "step" (for a profiler restricted to that range).  With
+    --continuations C: draw C continuations of K tokens of a short prompt."""
     import argparse
 
     ap = argparse.ArgumentParser()
     ap.add_argument("--layers", type=int, default=48)
     ap.add_argument("--profile-step", type=int, default=8)
+    ap.add_argument("--continuations", type=int, default=0)
     a = ap.parse_args(argv)
     w = Qwen3Weights.synthetic(ModelConfig(n_layers=a.layers), seed=1)
+    if a.continuations:
+        par = ParallelDecoder(w, a.continuations, max_prompt=16, max_new=a.profile_step)
+        tokens, logprobs = par.generate([5, 17, 290, 4], a.profile_step, seed=1, temperature=0.8, top_k=50, top_p=0.95)
+        for t, lp in zip(tokens.tolist(), logprobs.sum(1).tolist()):
+            print(f"{lp:9.3f}", t)
+        return
     dec = Decoder(w, max_positions=a.profile_step + 8)
     dec.reset()
     dec.token.fill_(5)
