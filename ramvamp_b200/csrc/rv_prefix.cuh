@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 // f16 (or 8-bit) keys and values are exact, so the result carries f32's
 // rounding only; the price is twice the products, and for head_dim 128 query
 // tiles of 64 rows (two operands a stream in shared memory).  f16 queries round
-// P to f16 once, the size of the output's own rounding.  P is lifted by 2^7 and
+// P to f16 once, the size of the output's own rounding: two terms there took
+// 64 sequences over an 8-bit 16K prompt from 58 to 65 us.  P is lifted by 2^7 and
 // the reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
 // normal f16 down to 2^-21 of the largest.
 //
@@ -1042,6 +1043,11 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
           for (int h = 0; h < halves; h++) {
             uint32_t v[64];
             tc_ld_wait(tS + 64 * h, v);
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (!full) {
+#pragma unroll
+              for (int j = 0; j < 64; j++) v[j] = 64 * h + j < lim ? v[j] : 0xFF800000u;
+            }
             if constexpr (Q8) {
               const float2 c2 = make_float2(c, c), zero = make_float2(0, 0);
 #pragma unroll
@@ -1049,25 +1055,25 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                 const float4 k4 = *(const float4 *)(sc + 64 * h + j);
                 float2 x0 = make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                 float2 x1 = make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
-                if (PRECISE) {
+                if constexpr (PRECISE) {  // by a power of two: exact
                   x0 = fma_f32x2(x0, c2, zero);
                   x1 = fma_f32x2(x1, c2, zero);
                 }
-                x0 = fma_f32x2(x0, make_float2(k4.x, k4.y), zero);
-                x1 = fma_f32x2(x1, make_float2(k4.z, k4.w), zero);
-                v[j] = __float_as_uint(x0.x);
-                v[j + 1] = __float_as_uint(x0.y);
-                v[j + 2] = __float_as_uint(x1.x);
-                v[j + 3] = __float_as_uint(x1.y);
+                const float2 t0 = fma_f32x2(x0, make_float2(k4.x, k4.y), zero),
+                             t1 = fma_f32x2(x1, make_float2(k4.z, k4.w), zero);
+                const float t[4] = {t0.x, t0.y, t1.x, t1.y}, x[4] = {x0.x, x0.y, x1.x, x1.y};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                  // Hidden scores stay -infinity whatever the token's scale is.
+                  const float u = full || x[i] != -INFINITY ? t[i] : -INFINITY;
+                  mx[i] = fmaxf(mx[i], u);
+                  v[j + i] = __float_as_uint(PRECISE ? x[i] : u);
+                }
               }
-            }
-            if (!full) {
+            } else {
 #pragma unroll
-              for (int j = 0; j < 64; j++) v[j] = 64 * h + j < lim ? v[j] : 0xFF800000u;
+              for (int j = 0; j < 64; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 64; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
             float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             if constexpr (!Q8) top *= c;
             top = on ? ceilf(top) + ev : -INFINITY;
@@ -1107,7 +1113,14 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
               for (int j = 0; j < 16; j++) {
                 const int e = 32 * ch + 2 * j;
                 float2 x = make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-                x = Q8 ? add_f32x2(x, m2) : fma_f32x2(x, c2, m2);
+                if constexpr (PRECISE && Q8) {
+                  // One rounding from the score to the exponent; a hidden
+                  // token's scale may be anything.
+                  const float2 k = *(const float2 *)(sc + 64 * h + e), y = fma_f32x2(x, k, m2);
+                  x = make_float2(x.x == -INFINITY ? x.x : y.x, x.y == -INFINITY ? x.y : y.y);
+                } else {
+                  x = Q8 ? add_f32x2(x, m2) : fma_f32x2(x, c2, m2);
+                }
                 x.x = ex2(x.x);
                 x.y = ex2(x.y);
                 l2[j & 1] = add_f32x2(l2[j & 1], x);
