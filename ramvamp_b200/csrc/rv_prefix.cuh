@@ -39,7 +39,10 @@ RV_DEVFN int prefix_suffix_len(const PrefixArgs &a, uint32_t b) {
 // Head dims other than 64 and 128 (multiples of 8 up to 256): one CTA of eight warps per
 // query row, a warp per key in turn, head_dim spread over the lanes, so a
 // score is one warp sum.  The keys and values of the prefix are read once per
-// query row, not once per batch.
+// query row, not once per batch, and a key waits for the sum before it: bound by
+// that latency (head_dim 96, f16, 16 query and 4 kv heads: one sequence over
+// 1,024 positions 56 us, 64 over 8,192 1.17 ms; head_dim 128 through the tensor
+// cores 13 and 27 us).
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
   __shared__ float s_m[8], s_l[8], s_o[8][256];
@@ -112,7 +115,8 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 // Work: a segment is a run of query rows of one kv head against the prefix or
 // against one sequence's suffix, cut into units of 128 keys.  The segments'
 // units stand on a line, with RV_PFX_OV places more for each segment's fixed
-// cost, and the line is split evenly; every stretch of a segment is a piece
+// cost (one place costs about what a tile does: the loads of Q, the first tiles
+// and the parts' stores), and the line is split evenly; every stretch of a segment is a piece
 // that leaves (m, l, O) of its rows in scratch, and k_prefix_join adds the
 // pieces of a row up.  The split follows from the lengths alone, so the result
 // does not depend on timing.
@@ -124,15 +128,27 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 //   pair: more than 128 query rows of a kv head share the prefix (f16 queries):
 //   the streams take 128 rows each of a segment of 256 and read the same key
 //   and value tiles, halving the traffic per product.  The prefix then has a
-//   line of its own, over a share of the CTAs that follows the costs.
+//   line of its own, over a share of the CTAs that follows the costs (128
+//   sequences over an f16 32K prompt 97 us, solo 112; 64 over an 8-bit 16K one
+//   58 and 72; with 128 rows or fewer there is no second stream to pair).
+//
+// What bounds it: a unit is 2,048 cycles of products and as many of
+// exponentials (16 a cycle and SM), and a stream's chain S -> exponentials -> P
+// V -> next S takes about twice that, so two streams keep the tensor pipe 0.42
+// active at 128 sequences over 32K positions (its floor is 40 us; K and V are
+// read from memory once, 119 MB).  Small calls are bound by the fixed chain of
+// planning, loading Q, one unit, and the join: 12 us at one short sequence.
 //
 // f32 queries are held to 2^-22 of their row's largest value as a sum of two
 // f16 (after scaling by a power of two), and so is P: products of f16 with the
 // f16 (or 8-bit) keys and values are exact, so the result carries f32's
-// rounding only; the price is twice the products, and for head_dim 128 query
+// rounding only (8 sequences over 4K positions: 6.6e-7 of the norm against 64
+// bits, f32 sums 1.6e-6; 42 over 21K: 5e-6 and 3e-6, as the tensor cores'
+// accumulator truncates); the price is twice the products, and for head_dim 128 query
 // tiles of 64 rows (two operands a stream in shared memory).  f16 queries round
-// P to f16 once, the size of the output's own rounding: two terms there took
-// 64 sequences over an 8-bit 16K prompt from 58 to 65 us.  P is lifted by 2^7 and
+// P to f16 once, the size of the output's own rounding (together 2.9e-4 of the
+// norm, where the output's alone is 2.1e-4): two terms there took 64 sequences
+// over an 8-bit 16K prompt from 58 to 65 us.  P is lifted by 2^7 and
 // the reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
 // normal f16 down to 2^-21 of the largest.
 //
@@ -1180,7 +1196,8 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
 // The parts of each query row added up: out = sum 2^(m_p - M) O_p / sum
 // 2^(m_p - M) l_p.  grid = (8-row groups of a kv head's rows, kv heads); a warp
 // holds eight rows times four part lanes (each takes every fourth part) and
-// two groups of four values, so a load is 128 contiguous bytes a part.
+// two groups of four values, so a load is 128 contiguous bytes a part.  Bound
+// by the latency of few loads a lane: 3 to 11 us of a call.
 #define RV_PFX_JOIN_ROWS 8
 template <int D, typename T>
 __global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) {
