@@ -741,6 +741,12 @@ def _stream_now() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _refuse_device(index: int):
+    """The kernels get plain pointers, and one to host memory would fault."""
+    raise KernelError(13, "InvalidArgument: tensors must be on one GPU, the cache's or the logits'"
+                          + (f" (cuda:{index})" if index >= 0 else ", which are in host memory"))
+
+
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # rv_dtype
 
 
@@ -801,6 +807,7 @@ class KvCache:
         c._c = _lib.KvCacheC(KV_F16, 1, cfg.n_kv_heads, cfg.head_dim, cfg.max_positions, k, v, None, None)
         c._ref = ctypes.addressof(c._c)
         c.device = torch.device(f"cuda:{engine.device}")
+        c._index = engine.device
         return c
 
     def _hold(self, k, v, ks, vs):
@@ -816,7 +823,9 @@ class KvCache:
             raise KernelError(9, "UnsupportedFormat: an f16 cache has no scales")
         self.k, self.v, self.k_scale, self.v_scale = k, v, ks, vs
         self.n_seqs, self.capacity, self.n_kv_heads, self.head_dim = k.shape
-        self.format, self.device = (KV_Q8 if q8 else KV_F16), k.device
+        self.format, self.device, self._index = (KV_Q8 if q8 else KV_F16), k.device, k.get_device()
+        if any(t is not None and t.get_device() != self._index for t in (v, ks, vs)):
+            raise KernelError(13, "InvalidArgument: a cache's tensors must be on one device")
         self._c = _lib.KvCacheC(self.format, *(self.n_seqs, self.n_kv_heads, self.head_dim), self.capacity, _p(k),
                                 _p(v), _p(ks), _p(vs))
         self._ref = ctypes.addressof(self._c)
@@ -824,13 +833,14 @@ class KvCache:
 
 def _rows_of(cache: KvCache, x: torch.Tensor):
     """(seq stride, token stride, tokens) of rows [n_seqs, n, n_kv_heads, head_dim]."""
-    if x.dim() != 4 or (x.shape[0], x.shape[2], x.shape[3]) != (cache.n_seqs, cache.n_kv_heads, cache.head_dim):
-        raise KernelError(5, f"LengthMismatch: rows {tuple(x.shape)} for a cache of {cache.n_seqs} sequences, "
+    shape = x.shape
+    if len(shape) != 4 or (shape[0], shape[2], shape[3]) != (cache.n_seqs, cache.n_kv_heads, cache.head_dim):
+        raise KernelError(5, f"LengthMismatch: rows {tuple(shape)} for a cache of {cache.n_seqs} sequences, "
                              f"{cache.n_kv_heads} kv heads of {cache.head_dim}")
     s = x.stride()
     if s[3] != 1 or (s[2] != cache.head_dim and cache.n_kv_heads > 1):
         raise KernelError(5, "LengthMismatch: the heads of a token must be contiguous")
-    return s[0], s[1], x.shape[1]
+    return s[0], s[1], shape[1]
 
 
 def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[torch.Tensor] = None,
@@ -842,6 +852,9 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[t
     seq, token, n = _rows_of(cache, k)
     if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
         raise KernelError(5, "LengthMismatch: k and v must be alike in shape, strides and type")
+    if not (0 <= cache._index == k.get_device() == v.get_device()) or (
+            lens is not None and lens.get_device() != cache._index):
+        _refuse_device(cache._index)
     _check(lib().rv_kv_append(cache._ref, _dtype(k), k.data_ptr(), v.data_ptr(), seq, token, n,
                               _i32(lens, cache.n_seqs, "lens"), position, _stream_now()))
 
@@ -850,6 +863,8 @@ def kv_read(cache: KvCache, n: int, lens: Optional[torch.Tensor] = None, positio
             dtype: torch.dtype = torch.float32):
     """(k, v) of n positions of every sequence, [n_seqs, n, n_kv_heads,
     head_dim] of `dtype`, chosen as in ``kv_append``."""
+    if cache._index < 0 or (lens is not None and lens.get_device() != cache._index):
+        _refuse_device(cache._index)
     k = torch.empty((cache.n_seqs, n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
     _check(lib().rv_kv_read(cache._ref, _dtype(k), n, _i32(lens, cache.n_seqs, "lens"), position, k.data_ptr(),
@@ -877,6 +892,12 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, n_q, H, D))
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise KernelError(5, "LengthMismatch: out must be contiguous and like q in shape and type")
+    if lens is None:
+        raise KernelError(13, "InvalidArgument: lens is required")
+    if not (0 <= suffix._index == q.get_device() == out.get_device() == lens.get_device()) or (
+            prefix is not None and prefix._index != suffix._index) or (
+            scratch is not None and scratch.get_device() != suffix._index):
+        _refuse_device(suffix._index)
     if scratch is None:
         scratch = q.new_empty(prefix_attention_scratch(n, n_q, H, suffix.n_kv_heads, D), dtype=torch.uint8)
     _check(lib().rv_prefix_attention(prefix._ref if prefix is not None else None, prefix_len, suffix._ref,
@@ -910,10 +931,14 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
         logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
     if u is None:
         raise KernelError(13, "InvalidArgument: u is required")
-    _check(lib().rv_sample(logits.data_ptr(), logits.stride(0), rows, n, _f32(u, rows, "u"),
-                           _f32(temperature, rows, "temperature"), _i32(top_k, rows, "top_k"),
-                           _f32(top_p, rows, "top_p"), _f32(min_p, rows, "min_p"), _i32(tokens, rows, "tokens"),
-                           _f32(logprobs, rows, "logprobs"), _stream_now()))
+    args = (_f32(u, rows, "u"), _f32(temperature, rows, "temperature"), _i32(top_k, rows, "top_k"),
+            _f32(top_p, rows, "top_p"), _f32(min_p, rows, "min_p"), _i32(tokens, rows, "tokens"),
+            _f32(logprobs, rows, "logprobs"))
+    index = logits.get_device()
+    for x in (u, temperature, top_k, top_p, min_p, tokens, logprobs):
+        if index < 0 or (x is not None and x.get_device() != index):
+            _refuse_device(index)
+    _check(lib().rv_sample(logits.data_ptr(), logits.stride(0), rows, n, *args, _stream_now()))
     return tokens, logprobs
 
 

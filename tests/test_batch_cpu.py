@@ -129,3 +129,24 @@ def test_python_checks(rv):
         rv.sample(torch.zeros(2, 4), torch.zeros(3))
     with pytest.raises(rv.KernelError):
         rv.sample(torch.zeros(2, 4), torch.zeros(2), top_k=torch.zeros(2))
+
+
+def test_host_tensors_are_refused(rv):
+    """Right in shape and type, but in host memory: refused before a pointer reaches a kernel."""
+    torch = pytest.importorskip("torch")
+    z = torch.zeros
+    c = rv.KvCache.of(z(1, 2, 3, 8).half(), z(1, 2, 3, 8).half())
+    lens = z(1, dtype=torch.int32)
+    for call in (lambda: rv.kv_append(c, z(1, 1, 3, 8), z(1, 1, 3, 8), lens=lens), lambda: rv.kv_read(c, 1),
+                 lambda: rv.prefix_attention(z(1, 1, 6, 8), None, 0, c, lens), lambda: rv.sample(z(2, 4), z(2)),
+                 lambda: rv.prefix_attention(z(1, 1, 6, 8), None, 0, c, None)):
+        with pytest.raises(rv.KernelError) as e:
+            call()
+        assert e.value.kind == "InvalidArgument"
+    # a cache on a GPU and host tensors beside it (the check comes before any pointer is used)
+    c._index = 0
+    for call in (lambda: rv.kv_append(c, z(1, 1, 3, 8), z(1, 1, 3, 8)), lambda: rv.kv_read(c, 1, lens=lens),
+                 lambda: rv.prefix_attention(z(1, 1, 6, 8), None, 0, c, lens)):
+        with pytest.raises(rv.KernelError) as e:
+            call()
+        assert e.value.kind == "InvalidArgument"
