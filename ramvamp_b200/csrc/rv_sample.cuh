@@ -30,7 +30,7 @@
 // reductions (13.8 us; its bytes are 0.1 us).  Many rows are bound by issue: a
 // token costs its comparisons, one exponential and the histograms' shared-memory
 // additions in each pass that weighs it (64 rows of 151,936, top-p: 69 us of GPU
-// time, 0.57 TB/s; 300 rows of 49,999, top-k 5,000 and top-p, 170 us).
+// time, 0.57 TB/s; 300 rows of 49,999, top-k 5,000 and top-p, 164 us).
 #pragma once
 #include "rv_internal.cuh"
 
@@ -353,8 +353,16 @@ RV_DEVFN SampleCut sample_cutoff(SampleShared &sh, const SampleRow &r, uint32_t 
     for (uint32_t i = (t >> 5) * r.size + r.rank; i < c.cnt; i += THREADS / 32 * r.size) {
       const u64 key = sh.list_key[i];
       u64 sum = 0;
-      for (uint32_t j = t & 31; j < c.cnt; j += 32) sum += sh.list_key[j] > key ? sh.list_w[j] : 0;
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(RV_FULL, sum, o);
+      if (weights) {
+#pragma unroll 4
+        for (uint32_t j = t & 31; j < c.cnt; j += 32) sum += sh.list_key[j] > key ? sh.list_w[j] : 0;
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(RV_FULL, sum, o);
+      } else {
+        uint32_t ahead = 0;
+#pragma unroll 4
+        for (uint32_t j = t & 31; j < c.cnt; j += 32) ahead += sh.list_key[j] > key;
+        sum = __reduce_add_sync(RV_FULL, ahead);
+      }
       sum += before;
       if (sum < goal && goal <= sum + sh.list_w[i] && (t & 31) < r.size) {
         st_cluster_u64(dsmem_addr(&sh.pick[2], t & 31), key);
