@@ -544,6 +544,8 @@ RV_DEVFN bool pfx_wait1(uint64_t *bar, uint32_t parity) {
 }
 // The same by a whole warp.
 RV_DEVFN bool pfx_wait(uint64_t *bar, uint32_t parity) { return __all_sync(RV_FULL, pfx_wait1(bar, parity)); }
+// Whether a role has given up, asked by a whole warp: its lanes leave together.
+RV_DEVFN bool pfx_failed(const volatile int *fail) { return __any_sync(RV_FULL, *fail); }
 
 template <int D, typename T, bool Q8>
 __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
@@ -744,7 +746,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       // stream 1 gives them back.
       int s = 0;
 #pragma unroll 1
-      for (; ok && (c.len || o.len) && !*s_fail; s ^= 1) {
+      for (; ok && (c.len || o.len) && !pfx_failed(s_fail); s ^= 1) {
         if (c.len) {
           const bool take = !(pair && s), give = !pair || s;
           const PfxPiece *p = &tab[pair ? 0 : s][c.at];
@@ -868,7 +870,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       }
       np[0] = c.np, nq[0] = c.nq, np[1] = o.np, nq[1] = o.nq;
       if (!ok) *s_fail = 1;
-      if (*s_fail) {  // products in flight end before tensor memory is freed
+      if (pfx_failed(s_fail)) {  // products in flight end before tensor memory is freed
         if (elect_one()) {
           tc_commit(drained);
           mbar_wait_bounded(drained, 0);
@@ -921,7 +923,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       };
       int half = 0;
       bool any = fetch(cur, 0);
-      for (; ok && any && !*s_fail; n++) {
+      for (; ok && any && !pfx_failed(s_fail); n++) {
         any = fetch(nxt, half ^ RV_PFX_N * D);  // in flight while this tile is converted
         if (any) asm volatile("cp.async.wait_group 1;" ::: "memory");
         else asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -1000,7 +1002,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     bool p_on = false, p_warp = false;
     float p_m = 0, p_l = 0;
 #pragma unroll 1
-    while (ok && !*s_fail) {
+    while (ok && !pfx_failed(s_fail)) {
       if (left) give_q(mytab[at], piece);
       if (p_part >= 0) {
         const int rw = p_head & 1 ? w.rw_s : w.rw_p;
@@ -1037,7 +1039,10 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       // the attention scale).  At least 2^-126, so that -infinity stays one.
       float c = Q8 ? 1.0f : scale;
       if constexpr (PRECISE) {
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory");  // the stream's four warps
+        // The exponents of the stream's four warps: each arrives with its rows'.
+        // A named barrier here would wait for ever on a warp that gave up.
+        ok = pfx_wait(&q_ready[s], piece & 1);
+        if (!ok) break;
         if (on) c *= __uint_as_float((uint32_t)(s_up[(2 * s + (piece & 1)) * C::SR + row] + 127) << 23);
       }
       c = fmaxf(c, 0x1p-126f);
