@@ -719,8 +719,6 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                       &kv_full[slot]);
       }
       if (!ok) *s_fail = 1;
-      if (*s_fail)  // let the copies in flight land before the CTA ends
-        for (int i = max(0, n - R); i < n; i++) mbar_wait_bounded(&kv_full[i % R], (i / R) & 1);
     }
     __syncwarp();
     n = __reduce_max_sync(RV_FULL, n);  // another lane may be elected in the next plan
@@ -870,13 +868,6 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       }
       np[0] = c.np, nq[0] = c.nq, np[1] = o.np, nq[1] = o.nq;
       if (!ok) *s_fail = 1;
-      if (pfx_failed(s_fail)) {  // products in flight end before tensor memory is freed
-        if (elect_one()) {
-          tc_commit(drained);
-          mbar_wait_bounded(drained, 0);
-        }
-        __syncwarp();
-      }
     } else if (Q8) {
       // ---------------------------------- 8-bit rows into f16 operands
       // 16 levels a load, D / 16 loads a token.  The next tile's levels are
@@ -1190,7 +1181,19 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();  // the table may be written again
-  if (*s_fail) break;
+  if (*s_fail) {
+    // A role gave up, perhaps after others had ended theirs: copies and products
+    // in flight end before the CTA does and tensor memory is freed.
+    if (!Q8 && warp == 0 && elect_one())
+      for (int i = max(0, n - R); i < n; i++) mbar_wait_bounded(&kv_full[i % R], (i / R) & 1);
+    if (warp == 1 && elect_one()) {
+      tc_commit(drained);
+      mbar_wait_bounded(drained, 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+    break;
+  }
   }
   if (warp == 0) {
     tc_fence_after();

@@ -34,3 +34,14 @@ def test_a_warp_leaves_its_role_as_one(source):
     assert len(loops) == 4
     plain = [x for x in loops if "pfx_failed(s_fail)" not in x]
     assert len(plain) == 1 and "pfx_feed(" in plain[0]  # the loads
+
+
+def test_a_cta_that_gives_up_waits_for_what_is_in_flight(source):
+    """A role may give up after the loads or the products have ended their own:
+    the copies and products in flight are waited for behind the CTA's barrier,
+    where every role's failure is known, and tensor memory is freed after that."""
+    end = source[source.rindex("__syncthreads();", 0, source.index("if (*s_fail) {")):source.index("tc_dealloc(")]
+    assert end.startswith("__syncthreads();") and "tc_commit(drained)" in end
+    assert "mbar_wait_bounded(&kv_full" in end and "mbar_wait_bounded(drained, 0)" in end
+    assert end.index("mbar_wait_bounded(drained, 0)") < end.rindex("__syncthreads();") < end.index("break;")
+    assert source.count("tc_commit(drained)") == 1  # in no role
