@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
            *q_ready = o_full + 2, *sc_full = q_ready + 2, *drained = sc_full + 2 * SLOTS;
   int *s_scan = (int *)(bars + C::NBARS);  // pieces in the streams' tables
   uint32_t *s_tmem = (uint32_t *)(s_scan + 2);
-  volatile int *s_fail = s_scan + 3, *s_bad = s_scan + 4;  // s_bad: [stream]
+  volatile int *s_fail = s_scan + 3, *s_bad = s_scan + 4;  // s_bad: [stream][piece & 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
   if (smem_addr(sm) & 1023) {
@@ -770,7 +770,9 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                 // of its queries, and 0 * NaN is not 0: a row that is not finite
                 // is taken out here, and its first key kept for the queries that
                 // see it, whose outputs become NaN.
-                int bad = c.j == 0 ? INT_MAX : s_bad[s];
+                // (The piece before may still be read: two places in turn.)
+                volatile int *const mark = s_bad + 2 * s + ((c.nq - 1) & 1);
+                int bad = c.j == 0 ? INT_MAX : *mark;
                 const int hidden = p->keys - (int)a.n_q + 1 - (p->tile0 + c.j) * RV_PFX_N;
                 for (int r = max(hidden, 0); r < valid; r++) {
                   uint4 *x = (uint4 *)(ring + (size_t)(nv % R) * TILE + (lane >> 3) * (RV_PFX_N * 128) +
@@ -785,7 +787,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                     bad = min(bad, (p->tile0 + c.j) * RV_PFX_N + r);
                   }
                 }
-                if (lane == 0) s_bad[s] = bad;
+                if (lane == 0) *mark = bad;
                 fence_proxy_async();
                 __syncwarp();
               }
@@ -1002,7 +1004,8 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         ok = pfx_wait(&o_full[s], (piece - 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        if (!Q8 && a.n_q > 1 && (p_head & 1) && p_seen > s_bad[s]) p_l = __uint_as_float(0x7FC00000u);
+        if (!Q8 && a.n_q > 1 && (p_head & 1) && p_seen > s_bad[2 * s + ((piece - 1) & 1)])
+          p_l = __uint_as_float(0x7FC00000u);
         if (p_on) (p_head & 1 ? w.ml_s : w.ml_p)[part * rw + row] = make_float2(p_m, p_l);
         if (p_warp) {
 #pragma unroll 1
