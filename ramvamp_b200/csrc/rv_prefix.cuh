@@ -1257,8 +1257,9 @@ __global__ void __launch_bounds__(D * 4) k_prefix_join(PrefixArgs a, PfxWork w) 
       const float2 x = ml[s][(size_t)i * step[s] * rw[s]];
       const float4 *q = po[s] + (size_t)i * step[s] * (D / 4) * rw[s];
       const float4 v[2] = {q[0], q[(D / 8) * rw[s]]};
-      // -infinity: the row saw none of the part's keys, whose O may be anything.
-      const bool sees = x.x != -INFINITY;
+      // -infinity: the row saw none of the part's keys, whose O may be anything --
+      // unless its sum is NaN: then every score it saw was (maxima pass NaN over).
+      const bool sees = x.x != -INFINITY || isnan(x.y);
       const float f = sees ? exp2f(x.x - M) : 0.0f;
       L += sees ? x.y * f : 0.0f;
 #pragma unroll
