@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 //
 // 8-bit cache: levels are exact in f16, so the products run on levels; a token's
 // key scale multiplies its score and its value scale its weight, both in f32.
-// With 2^ev above the tile's largest value scale the reference is m + ev, so
-// that P, which holds the value scale, stays in the range above.
+// P holds the value scale, so the reference is that of the products: with 2^e
+// above a token's value scale, the largest s + e of the keys that the row sees.
+// What a row does not see, or sees with next to no weight, does not move it.
 #define RV_PFX_CTAS 148       // CTAs at most: one per SM of a B200
 #define RV_PFX_THREADS 384    // loads, products and conversion; two softmax warpgroups
 #define RV_PFX_CONV 96        // threads that turn 8-bit rows into f16 (warps 0, 2, 3)
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 #define RV_PFX_LAG 8.0f       // the reference maximum may lag by this (log2)
 #define RV_PFX_LIFT 7.0f      // P is lifted by 2^7
 #define RV_PFX_SCALE_SLOTS 8  // tiles a stream whose token scales are in shared memory
-#define RV_PFX_SCALE (2 * RV_PFX_N + 4)  // floats of a tile's scales: keys', values', the values' largest by warp
+#define RV_PFX_SCALE (3 * RV_PFX_N)  // floats of a tile's scales: keys', values', the values' exponents
 #define RV_PFX_TABLE 32       // pieces a stream works through between plans: one a lane
 #define RV_PFX_O 256          // first tensor-memory column of O (S and P: 0..255)
 
@@ -924,22 +925,22 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         ok = pfx_wait(&kv_empty[slot], ((n / R) & 1) ^ 1);
         if (!ok) break;
         if (cur.at >= 0) {
-          float *sc = s_scale + cur.at * RV_PFX_SCALE, top = 0;
+          float *sc = s_scale + cur.at * RV_PFX_SCALE;
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const int tok = ct + j * RV_PFX_CONV;
             // A value scale that is not finite makes the token's weight NaN
             // through its key scale; as a factor it is 0, for the rows that do
-            // not see the token.
-            const bool fine = cur.vs[j] < INFINITY;
+            // not see the token.  Exponents from -80 up: the weights of tokens
+            // without a value then stay below 2^95.
+            const float size = fabsf(cur.vs[j]);
+            const bool fine = size < INFINITY;
             if (tok < RV_PFX_N) {
               sc[tok] = fine ? cur.ks[j] * fabsf(a.scale_log2) : __uint_as_float(0x7FC00000u);
               sc[RV_PFX_N + tok] = fine ? cur.vs[j] : 0.0f;
+              sc[2 * RV_PFX_N + tok] = (float)max((int)(__float_as_uint(size) >> 23) - 126, -80);
             }
-            if (fine) top = fmaxf(top, cur.vs[j]);
           }
-          for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(RV_FULL, top, o));
-          if (lane == 0) sc[2 * RV_PFX_N + ct / 32] = top;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sc_full[cur.at]);
         }
@@ -1041,7 +1042,6 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       }
       c = fmaxf(c, 0x1p-126f);
       float m_ref = -INFINITY, l = 0.0f;
-      int ev = 0;
       for (int t = 0; t < p.n; t++, unit++) {
         const int tile = p.tile0 + t, valid = min(RV_PFX_N, p.keys - tile * RV_PFX_N);
         const int lim = min(max(seen - tile * RV_PFX_N, 0), RV_PFX_N);
@@ -1054,13 +1054,6 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         if (warp_on) {
           const int halves = valid > 64 ? 2 : 1;
           const bool full = __all_sync(RV_FULL, lim == RV_PFX_N || !on);
-          if constexpr (Q8) {
-            // The tile's values reach 2^ev; P holds the tokens' scales, so the
-            // reference grows with it.
-            const float *vm = sc + 2 * RV_PFX_N;
-            const float vmax = fmaxf(vm[0], fmaxf(vm[1], vm[2]));
-            ev = max((int)(__float_as_uint(vmax) >> 23) - 126, -80);
-          }
 #pragma unroll 1
           for (int h = 0; h < halves; h++) {
             uint32_t v[64];
@@ -1075,20 +1068,22 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
 #pragma unroll
               for (int j = 0; j < 64; j += 4) {
                 const float4 k4 = *(const float4 *)(sc + 64 * h + j);
+                const float4 e4 = *(const float4 *)(sc + 2 * RV_PFX_N + 64 * h + j);
                 float2 x0 = make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                 float2 x1 = make_float2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
                 if constexpr (PRECISE) {  // by a power of two: exact
                   x0 = fma_f32x2(x0, c2, zero);
                   x1 = fma_f32x2(x1, c2, zero);
                 }
-                const float2 t0 = fma_f32x2(x0, make_float2(k4.x, k4.y), zero),
-                             t1 = fma_f32x2(x1, make_float2(k4.z, k4.w), zero);
-                const float t[4] = {t0.x, t0.y, t1.x, t1.y}, x[4] = {x0.x, x0.y, x1.x, x1.y};
+                // f32 queries use t for the maximum alone: the exponent comes with it.
+                const float2 t0 = fma_f32x2(x0, make_float2(k4.x, k4.y), PRECISE ? make_float2(e4.x, e4.y) : zero),
+                             t1 = fma_f32x2(x1, make_float2(k4.z, k4.w), PRECISE ? make_float2(e4.z, e4.w) : zero);
+                const float t[4] = {t0.x, t0.y, t1.x, t1.y}, x[4] = {x0.x, x0.y, x1.x, x1.y}, e[4] = {e4.x, e4.y, e4.z, e4.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                   // Hidden scores stay -infinity whatever the token's scale is.
                   const float u = full || x[i] != -INFINITY ? t[i] : -INFINITY;
-                  mx[i] = fmaxf(mx[i], u);
+                  mx[i] = fmaxf(mx[i], PRECISE ? u : u + e[i]);
                   v[j + i] = __float_as_uint(PRECISE ? x[i] : u);
                 }
               }
@@ -1098,7 +1093,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
             }
             float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             if constexpr (!Q8) top *= c;
-            top = on ? ceilf(top) + ev : -INFINITY;
+            top = on ? ceilf(top) : -INFINITY;
             if (t == 0 && h == 0) {
               m_ref = top;
             } else if (const bool move = top > m_ref + RV_PFX_LAG; __any_sync(RV_FULL, move)) {

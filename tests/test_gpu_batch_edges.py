@@ -143,3 +143,81 @@ def test_a_nan_key_gives_nan_where_it_is_all_that_a_part_sees(rv, fmt, dtype, di
     # a whole tile of a long prefix
     clean, got = run(3000, [5, 0, 130], lambda pre, suf: spoil(pre, 0, 1, list(range(1024, 1152))))
     assert torch.isnan(got[:, :, 4:]).all() and torch.equal(got[:, :, :4], clean[:, :, :4])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("factor", [2.0 ** 12, 2.0 ** 24, 2.0 ** 40, 2.0 ** 90])
+def test_8_bit_values_of_later_tokens_do_not_reach_earlier_queries(rv, dtype, dim, factor):
+    """Of five new tokens the fourth has finite values far larger than the
+    others': the first three queries keep their bits."""
+    for length in (5, 126, 131, 260):
+        pre, suf = caches(rv, 2, 300, 2, dim, 130, rv.KV_Q8, 91)
+        q = randn(95, 2, 5, 8, dim).to(dtype)
+        clean = rv.prefix_attention(q, pre, 130, suf, i32([300, length]))
+        suf.v_scale[1, length - 2] *= factor
+        got = rv.prefix_attention(q, pre, 130, suf, i32([300, length]))
+        assert torch.equal(got[0], clean[0]) and torch.equal(got[1, :3], clean[1, :3])
+        assert not torch.equal(got[1, 3:], clean[1, 3:])
+
+
+def attention_by_weight(q, pre, prefix_len, suf, lens, scale):
+    """(output, bound of the error) in 64 bits, one query token a sequence.
+
+    A score is off by at most delta_j = 2^-20 scale max|q| sum|k_j| (f32 sums of
+    at most 256 products: 2^-24 each, 16 of them allowed for), so a weight by
+    eps_j = 2 delta_j + 2^-19 of itself (exponential, running rescales), and by
+    2^-11 more where it is rounded to f16.  That moves the output by at most
+    sum p_j eps_j |v_j| + (sum p_j eps_j) sum p_j |v_j|.  Products of weight and
+    value scale below 2^-14, where the row's largest is 2^5 or more, are held
+    within 2^-25: 2^-30 of the largest product a key.  An f16 output is rounded
+    (2^-11 of it)."""
+    f16 = q.dtype == torch.float16
+    values = lambda c: [x.double() * s.double().unsqueeze(-1) for x, s in ((c.k, c.k_scale), (c.v, c.v_scale))]  # noqa: E731
+    (pk, pv), (sk, sv) = values(pre), values(suf)
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    G = q.shape[2] // pre.n_kv_heads
+    for b, n in enumerate(lens):
+        k, v = (torch.cat([p[0, :prefix_len], s[b, :n]]).repeat_interleave(G, 1) for p, s in ((pk, sk), (pv, sv)))
+        qq = q[b, 0].double()
+        p = torch.softmax(torch.einsum("hd,khd->hk", qq, k) * scale, -1)
+        eps = 2 * 2.0 ** -20 * scale * qq.abs().amax(-1)[:, None] * k.abs().sum(-1).t() + 2.0 ** -19 + f16 * 2.0 ** -11
+        size = torch.einsum("hk,khd->hd", p, v.abs())
+        out[b, 0] = torch.einsum("hk,khd->hd", p, v)
+        tol[b, 0] = torch.einsum("hk,khd->hd", p * eps, v.abs()) + (p * eps).sum(-1)[:, None] * size
+        tol[b, 0] += (len(k) * 2.0 ** -30 * (p * v.abs().amax(-1).t()).amax(-1))[:, None] + f16 * 2.0 ** -11 * out[b, 0].abs()
+    return out, tol
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+def test_8_bit_values_count_by_their_weight(rv, dtype, dim):
+    """Values far larger than the others' on keys that weigh next to nothing,
+    and sizes spread over many powers of two: the error is bounded by weight
+    times value, not by the largest value."""
+    n, prefix, lens = 3, 700, [1, 260, 129]
+    scale = dim ** -0.5
+    for factor in (2.0 ** 12, 2.0 ** 24, 2.0 ** 40, None):
+        pre, suf = caches(rv, n, 260, 2, dim, prefix, rv.KV_Q8, 101)
+        q = randn(105, n, 1, 8, dim)
+        q = (0.2 * q + q[:, :, :, :1].sign().expand_as(q)).to(dtype)  # all near + or - (1, .., 1)
+        q = q.abs()
+        if factor:
+            for cache, seq, at in ((pre, 0, 3), (pre, 0, 400), (suf, 1, 200), (suf, 2, 0)):
+                k = torch.full((1, 1, 2, dim), -100 / (scale * dim), device="cuda")  # a score of about -100
+                one = rv.KvCache(1, 1, 2, dim, rv.KV_Q8)
+                rv.kv_append(one, k, k)
+                cache.k[seq, at], cache.k_scale[seq, at] = one.k[0, 0], one.k_scale[0, 0]
+                cache.v_scale[seq, at] *= factor
+        else:
+            for cache, seed in ((pre, 106), (suf, 107)):
+                cache.v_scale *= torch.exp2(8 * randn(seed, *cache.v_scale.shape))
+        got = rv.prefix_attention(q, pre, prefix, suf, i32(lens), scale=scale)
+        want, tol = attention_by_weight(q, pre, prefix, suf, lens, scale)
+        if dtype == torch.float16 and factor is None:
+            fits = want.abs() < 60000
+            got, want, tol = got[fits], want[fits], tol[fits]
+            assert fits.double().mean() > 0.25
+        assert torch.isfinite(got).all()
+        assert ((got.double() - want).abs() <= tol).all()
