@@ -741,10 +741,17 @@ def _stream_now() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+def _elsewhere(index: int) -> bool:
+    """Whether tensors of GPU `index` (-1: host memory) are out of the current
+    device's reach, where the stream is and the kernels run."""
+    return index < 0 or index != torch._C._cuda_getDevice()
+
+
 def _refuse_device(index: int):
-    """The kernels get plain pointers, and one to host memory would fault."""
+    """The kernels get plain pointers, and one to host memory or to another GPU
+    would fault."""
     raise KernelError(13, "InvalidArgument: tensors must be on one GPU, the cache's or the logits'"
-                          + (f" (cuda:{index})" if index >= 0 else ", which are in host memory"))
+                          + (f" (cuda:{index}), which must be current" if index >= 0 else ", which are in host memory"))
 
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # rv_dtype
@@ -852,8 +859,8 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[t
     seq, token, n = _rows_of(cache, k)
     if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
         raise KernelError(5, "LengthMismatch: k and v must be alike in shape, strides and type")
-    if not (0 <= cache._index == k.get_device() == v.get_device()) or (
-            lens is not None and lens.get_device() != cache._index):
+    if not (cache._index == k.get_device() == v.get_device()) or (
+            lens is not None and lens.get_device() != cache._index) or _elsewhere(cache._index):
         _refuse_device(cache._index)
     _check(lib().rv_kv_append(cache._ref, _dtype(k), k.data_ptr(), v.data_ptr(), seq, token, n,
                               _i32(lens, cache.n_seqs, "lens"), position, _stream_now()))
@@ -863,7 +870,7 @@ def kv_read(cache: KvCache, n: int, lens: Optional[torch.Tensor] = None, positio
             dtype: torch.dtype = torch.float32):
     """(k, v) of n positions of every sequence, [n_seqs, n, n_kv_heads,
     head_dim] of `dtype`, chosen as in ``kv_append``."""
-    if cache._index < 0 or (lens is not None and lens.get_device() != cache._index):
+    if (lens is not None and lens.get_device() != cache._index) or _elsewhere(cache._index):
         _refuse_device(cache._index)
     k = torch.empty((cache.n_seqs, n, cache.n_kv_heads, cache.head_dim), dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
@@ -894,9 +901,9 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
         raise KernelError(5, "LengthMismatch: out must be contiguous and like q in shape and type")
     if lens is None:
         raise KernelError(13, "InvalidArgument: lens is required")
-    if not (0 <= suffix._index == q.get_device() == out.get_device() == lens.get_device()) or (
+    if not (suffix._index == q.get_device() == out.get_device() == lens.get_device()) or (
             prefix is not None and prefix._index != suffix._index) or (
-            scratch is not None and scratch.get_device() != suffix._index):
+            scratch is not None and scratch.get_device() != suffix._index) or _elsewhere(suffix._index):
         _refuse_device(suffix._index)
     if scratch is None:
         scratch = q.new_empty(prefix_attention_scratch(n, n_q, H, suffix.n_kv_heads, D), dtype=torch.uint8)
@@ -936,8 +943,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
             _f32(logprobs, rows, "logprobs"))
     index = logits.get_device()
     for x in (u, temperature, top_k, top_p, min_p, tokens, logprobs):
-        if index < 0 or (x is not None and x.get_device() != index):
+        if x is not None and x.get_device() != index:
             _refuse_device(index)
+    if _elsewhere(index):
+        _refuse_device(index)
     _check(lib().rv_sample(logits.data_ptr(), logits.stride(0), rows, n, *args, _stream_now()))
     return tokens, logprobs
 

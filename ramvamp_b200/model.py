@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass, field
+from functools import wraps
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -232,6 +233,17 @@ class Decoder:
         return [int(x) for x in ids[len(prompt) - 1:]]
 
 
+def _on_its_device(method):
+    """The method with its object's device current, where its kernels run."""
+
+    @wraps(method)
+    def run(self, *args, **kwargs):
+        with torch.cuda.device(self.device):
+            return method(self, *args, **kwargs)
+
+    return run
+
+
 class ParallelDecoder:
     """n continuations of one prompt, drawn together.  The prompt goes through
     ``Decoder`` once; its keys and values -- the engine's own f16 caches, or
@@ -262,6 +274,7 @@ class ParallelDecoder:
         self.scratch = torch.empty(prefix_attention_scratch(n, 1, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim),
                                    dtype=torch.uint8, device=d)
 
+    @_on_its_device
     def prefill(self, prompt: Sequence[int]) -> torch.Tensor:
         """The prompt's rows into the prefix; the logits of its last token."""
         if not 0 < len(prompt) <= self.max_prompt:
@@ -287,6 +300,7 @@ class ParallelDecoder:
         gemv(*head, in_dim, out_dim, acts, self.n, range(out_dim), out)
         return out.t().contiguous()
 
+    @_on_its_device
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
         """One token of every continuation (int32 [n], on the device) through
         the model (model/forward.rs:2548-2780 for each row): logits [n, vocab]."""
@@ -317,6 +331,7 @@ class ParallelDecoder:
         self.logits.copy_(self._rows(gemv_q8_k_batched, Q.Q6_K, w.lm_head, H, cfg.vocab, quantize_row_q8_k(self.normed)))
         return self.logits
 
+    @_on_its_device
     def generate(self, prompt: Sequence[int], n_new: int, seed: int = 0, temperature: float = 1.0, top_k: int = 0,
                  top_p: float = 1.0, min_p: float = 0.0):
         """n continuations of `prompt` by n_new tokens: (tokens int32, logprobs

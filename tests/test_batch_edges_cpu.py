@@ -1,0 +1,92 @@
+"""What the Python entry points of the batched-continuation operators let
+through to the kernels, with the library stubbed: no GPU, no launch."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Stub:
+    """Stands for the loaded library: records the calls it gets."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append((name, args)) or 0
+
+
+@pytest.fixture()
+def rv():
+    import ramvamp_b200
+
+    return ramvamp_b200
+
+
+@pytest.fixture()
+def on_gpu(rv, monkeypatch):
+    """on_gpu(tensors', current): tensors say that they are on one GPU while
+    another (or the same) is current; the stub in the library's place."""
+
+    def set_up(index, current):
+        stub = Stub()
+        monkeypatch.setattr(rv, "lib", lambda: stub)
+        monkeypatch.setattr(torch.Tensor, "get_device", lambda self: index, raising=False)
+        monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current, raising=False)
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
+        return stub
+
+    return set_up
+
+
+def calls(rv):
+    """(name, call) of the four operators on tensors that they accept."""
+    z = torch.zeros
+    c = rv.KvCache.of(z(1, 2, 3, 8).half(), z(1, 2, 3, 8).half())
+    lens, scratch = z(1, dtype=torch.int32), z(1 << 16, dtype=torch.uint8)
+    return {
+        "rv_kv_append": lambda: rv.kv_append(c, z(1, 1, 3, 8), z(1, 1, 3, 8), lens=lens),
+        "rv_kv_read": lambda: rv.kv_read(c, 1, lens=lens),
+        "rv_prefix_attention": lambda: rv.prefix_attention(z(1, 1, 6, 8), c, 2, c, lens, scratch=scratch),
+        "rv_sample": lambda: rv.sample(z(2, 4), z(2)),
+    }
+
+
+@pytest.mark.parametrize("name", ["rv_kv_append", "rv_kv_read", "rv_prefix_attention", "rv_sample"])
+def test_tensors_of_a_gpu_that_is_not_current_are_refused(rv, on_gpu, name):
+    """The stream and the kernels are the current device's: pointers of another
+    GPU must not reach them."""
+    stub = on_gpu(1, current=0)
+    with pytest.raises(rv.KernelError) as e:
+        calls(rv)[name]()
+    assert e.value.kind == "InvalidArgument" and stub.calls == []
+    stub = on_gpu(1, current=1)
+    calls(rv)[name]()
+    assert [c[0] for c in stub.calls] == [name]
+
+
+def test_the_parallel_decoder_runs_on_its_own_device(rv, monkeypatch):
+    """prefill, step and generate make the decoder's device current."""
+    from ramvamp_b200.model import ParallelDecoder
+
+    seen = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            seen.append(self.index)
+
+        def __exit__(self, *exc):
+            seen.append("out")
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    par = object.__new__(ParallelDecoder)
+    par.device, par.prompt_len, par.new, par.max_new, par.max_prompt, par.n = 1, 0, 0, 4, 4, 2
+    par.w = par.cfg = None
+    for call, error in ((lambda: par.prefill([]), ValueError), (lambda: par.step(torch.zeros(2)), (ValueError, AttributeError)),
+                        (lambda: par.generate([1], 2), AttributeError)):
+        seen.clear()
+        with pytest.raises(error):
+            call()
+        assert seen == [1, "out"]
