@@ -886,8 +886,8 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
     contiguous) over positions 0..prefix_len-1 of `prefix`, shared by all
     sequences, and each sequence's own `lens` suffix positions (int32, on the
     device; the n_q query tokens are the newest of them and see no later one).
-    scale defaults to head_dim ** -0.5; scratch: a uint8 tensor of at least
-    ``prefix_attention_scratch`` bytes."""
+    scale defaults to head_dim ** -0.5; scratch: a contiguous uint8 tensor of at
+    least ``prefix_attention_scratch`` bytes."""
     if q.dim() != 4 or q.shape[0] != suffix.n_seqs or q.shape[3] != suffix.head_dim:
         raise KernelError(5, f"LengthMismatch: queries {tuple(q.shape)} for a suffix of {suffix.n_seqs} sequences, "
                              f"head_dim {suffix.head_dim}")
@@ -899,6 +899,8 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, n_q, H, D))
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise KernelError(5, "LengthMismatch: out must be contiguous and like q in shape and type")
+    if scratch is not None and not scratch.is_contiguous():
+        raise KernelError(5, "LengthMismatch: scratch must be contiguous")
     if lens is None:
         raise KernelError(13, "InvalidArgument: lens is required")
     if not (suffix._index == q.get_device() == out.get_device() == lens.get_device()) or (

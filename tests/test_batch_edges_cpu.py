@@ -90,3 +90,17 @@ def test_the_parallel_decoder_runs_on_its_own_device(rv, monkeypatch):
         with pytest.raises(error):
             call()
         assert seen == [1, "out"]
+
+
+def test_scratch_with_gaps_is_refused(rv, on_gpu):
+    """A view of every other byte: as many elements as bytes are needed, but the
+    kernels would write between them and past them."""
+    stub = on_gpu(0, current=0)
+    z = torch.zeros
+    c = rv.KvCache.of(z(1, 2, 3, 8).half(), z(1, 2, 3, 8).half())
+    lens, wide = z(1, dtype=torch.int32), z(1 << 16, 2, dtype=torch.uint8)
+    with pytest.raises(rv.KernelError) as e:
+        rv.prefix_attention(z(1, 1, 6, 8), c, 2, c, lens, scratch=wide[:, 0])
+    assert e.value.kind == "LengthMismatch" and stub.calls == []
+    rv.prefix_attention(z(1, 1, 6, 8), c, 2, c, lens, scratch=wide)
+    assert [x[0] for x in stub.calls] == ["rv_prefix_attention"]
