@@ -839,7 +839,8 @@ class KvCache:
 
 
 def _rows_of(cache: KvCache, x: torch.Tensor):
-    """(seq stride, token stride, tokens) of rows [n_seqs, n, n_kv_heads, head_dim]."""
+    """(seq stride, token stride, tokens) of rows [n_seqs, n, n_kv_heads, head_dim];
+    of one sequence or one token, whose stride means nothing, that of contiguous rows."""
     shape = x.shape
     if len(shape) != 4 or (shape[0], shape[2], shape[3]) != (cache.n_seqs, cache.n_kv_heads, cache.head_dim):
         raise KernelError(5, f"LengthMismatch: rows {tuple(shape)} for a cache of {cache.n_seqs} sequences, "
@@ -847,7 +848,8 @@ def _rows_of(cache: KvCache, x: torch.Tensor):
     s = x.stride()
     if s[3] != 1 or (s[2] != cache.head_dim and cache.n_kv_heads > 1):
         raise KernelError(5, "LengthMismatch: the heads of a token must be contiguous")
-    return s[0], s[1], shape[1]
+    token = s[1] if shape[1] > 1 else shape[2] * shape[3]
+    return s[0] if shape[0] > 1 else shape[1] * token, token, shape[1]
 
 
 def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[torch.Tensor] = None,
@@ -856,8 +858,8 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, lens: Optional[t
     token and sequence strides, the same for both) as the last n positions of
     sequences of `lens` tokens (int32 [n_seqs], on the device, the new rows
     counted), or from `position` on."""
-    seq, token, n = _rows_of(cache, k)
-    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+    rows = seq, token, n = _rows_of(cache, k)
+    if k.shape != v.shape or k.dtype != v.dtype or (k.stride() != v.stride() and _rows_of(cache, v) != rows):
         raise KernelError(5, "LengthMismatch: k and v must be alike in shape, strides and type")
     if not (cache._index == k.get_device() == v.get_device()) or (
             lens is not None and lens.get_device() != cache._index) or _elsewhere(cache._index):

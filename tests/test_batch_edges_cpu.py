@@ -104,3 +104,29 @@ def test_scratch_with_gaps_is_refused(rv, on_gpu):
     assert e.value.kind == "LengthMismatch" and stub.calls == []
     rv.prefix_attention(z(1, 1, 6, 8), c, 2, c, lens, scratch=wide)
     assert [x[0] for x in stub.calls] == ["rv_prefix_attention"]
+
+
+def test_strides_of_one_token_or_sequence_do_not_matter(rv, on_gpu):
+    """k and v that differ only in the stride of a dimension of size 1 are alike;
+    where it counts, different strides are still refused."""
+    stub = on_gpu(0, current=0)
+    z = torch.zeros(4096)
+
+    def rows(n_seqs, n, seq, token, heads=3, head=8):
+        return z.as_strided((n_seqs, n, heads, 8), (seq, token, head, 1))
+
+    def cache(n_seqs, heads=3):
+        return rv.KvCache.of(torch.zeros(n_seqs, 4, heads, 8).half(), torch.zeros(n_seqs, 4, heads, 8).half())
+
+    rv.kv_append(cache(1), rows(1, 1, 24, 24), rows(1, 1, 7, 5))          # a sequence's only new token
+    rv.kv_append(cache(4), rows(4, 1, 100, 24), rows(4, 1, 100, 100))     # one token of each
+    rv.kv_append(cache(1), rows(1, 3, 72, 40), rows(1, 3, 1, 40))         # a prompt
+    rv.kv_append(cache(2, 1), rows(2, 2, 64, 16, 1, 8), rows(2, 2, 64, 16, 1, 3))  # one head
+    assert [(x[0], x[1][4:7]) for x in stub.calls] == [("rv_kv_append", (24, 24, 1)), ("rv_kv_append", (100, 24, 1)),
+                                                       ("rv_kv_append", (120, 40, 3)), ("rv_kv_append", (64, 16, 2))]
+    for n_seqs, k, v in ((4, rows(4, 1, 100, 24), rows(4, 1, 101, 24)), (1, rows(1, 3, 72, 40), rows(1, 3, 72, 41)),
+                         (1, rows(1, 3, 72, 40), rows(1, 2, 72, 40)), (1, rows(1, 1, 24, 24), rows(1, 1, 24, 24, 3, 9))):
+        with pytest.raises(rv.KernelError) as e:
+            rv.kv_append(cache(n_seqs), k, v)
+        assert e.value.kind == "LengthMismatch"
+    assert len(stub.calls) == 4
