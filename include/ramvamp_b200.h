@@ -740,7 +740,7 @@ RV_API int rv_prefix_attention_scratch(size_t n_seqs, size_t n_q, size_t n_heads
                                        size_t *bytes_out);
 
 /* Draws one token of each of n_rows rows of logits (device f32, row r at
- * r*row_stride, n of them, n <= 720896).  Per row, with l the logits (NaN as
+ * r*row_stride, n of them, n <= 720896; a stride of 0 draws all from one row).  Per row, with l the logits (NaN as
  * -infinity): z = (l - max l) / temperature, weights exp(z); in descending
  * order of l, equal values by ascending index, top_k keeps the first k tokens
  * (k <= 0 or >= n: all), top_p < 1 of those the tokens whose preceding weight

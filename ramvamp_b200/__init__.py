@@ -930,9 +930,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
            top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
            min_p: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None,
            logprobs: Optional[torch.Tensor] = None):
-    """Draw one token of each row of logits [n_rows, n] (f32, rows contiguous)
-    with the uniforms u [n_rows] in [0, 1): (tokens int32, logprobs f32).  The
-    filters are per-row device arrays (top_k int32); ``None`` switches one off."""
+    """Draw one token of each row of logits [n_rows, n] (f32, rows contiguous; an
+    expanded row may stand for all) with the uniforms u [n_rows] in [0, 1):
+    (tokens int32, logprobs f32).  The filters are per-row device arrays (top_k
+    int32); ``None`` switches one off."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError(5, "LengthMismatch: logits must be float32 [n_rows, n] with contiguous rows")
     rows, n = logits.shape

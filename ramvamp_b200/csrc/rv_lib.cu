@@ -2968,7 +2968,8 @@ extern "C" int rv_sample(const float *logits, size_t row_stride, size_t n_rows, 
   if (n == 0) RV_FAIL(RV_ERR_EMPTY, "sample: no logits");
   if (n > RV_SAMPLE_MOST) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu logits a row (<= %d)", n, RV_SAMPLE_MOST);
   if (n_rows >= (1ull << 27)) RV_FAIL(RV_ERR_UNIMPLEMENTED, "sample: %zu rows (< 2^27)", n_rows);
-  if (row_stride < n && n_rows > 1) RV_FAIL(RV_ERR_LENGTH_MISMATCH, "sample: row stride %zu below %zu logits", row_stride, n);
+  if (row_stride && row_stride < n && n_rows > 1)
+    RV_FAIL(RV_ERR_LENGTH_MISMATCH, "sample: row stride %zu below %zu logits", row_stride, n);
   if (!logits || !u || !tokens ||
       (((uintptr_t)logits | (uintptr_t)u | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p |
         (uintptr_t)min_p | (uintptr_t)tokens | (uintptr_t)logprobs) & 3))

@@ -344,7 +344,7 @@ class ParallelDecoder:
         filters = (full(temperature), torch.full((self.n,), top_k, dtype=torch.int32, device=d), full(top_p), full(min_p))
         tokens = torch.empty(n_new, self.n, dtype=torch.int32, device=d)
         logprobs = torch.empty(n_new, self.n, dtype=torch.float32, device=d)
-        logits = self.prefill(prompt).expand(self.n, -1).contiguous()
+        logits = self.prefill(prompt).expand(self.n, -1)
         for i in range(n_new):
             sample(logits, u[i], *filters, tokens=tokens[i], logprobs=logprobs[i])
             if i + 1 < n_new:

@@ -130,3 +130,10 @@ def test_strides_of_one_token_or_sequence_do_not_matter(rv, on_gpu):
             rv.kv_append(cache(n_seqs), k, v)
         assert e.value.kind == "LengthMismatch"
     assert len(stub.calls) == 4
+
+
+def test_sample_takes_a_row_stride_of_zero(rv):
+    """The checks go on to the null pointer behind the stride's."""
+    name = lambda stride: rv.lib().rv_status_name(  # noqa: E731
+        rv.lib().rv_sample(None, stride, 2, 100, 0x1000, None, None, None, None, 0x1000, None, None)).decode()
+    assert name(0) == name(100) == "InvalidArgument" and name(99) == name(1) == "LengthMismatch"

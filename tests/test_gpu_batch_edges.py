@@ -221,3 +221,14 @@ def test_8_bit_values_count_by_their_weight(rv, dtype, dim):
             assert fits.double().mean() > 0.25
         assert torch.isfinite(got).all()
         assert ((got.double() - want).abs() <= tol).all()
+
+
+def test_sample_draws_many_from_one_row(rv):
+    """An expanded row (stride 0) as a copy of it in every row."""
+    logits = 2 * randn(111, 1, 5003)
+    u = torch.rand(40, device="cuda", generator=gen(112))
+    k = i32([50] * 40)
+    tokens, logprobs = rv.sample(logits.expand(40, -1), u, top_k=k)
+    want = rv.sample(logits.expand(40, -1).contiguous(), u, top_k=k)
+    assert torch.equal(tokens, want[0]) and torch.equal(logprobs, want[1])
+    assert len(set(tokens.tolist())) > 1
