@@ -683,7 +683,7 @@ typedef enum rv_dtype { RV_F32 = 0, RV_F16 = 1, RV_BF16 = 2 } rv_dtype;
 typedef enum rv_kv_format { RV_KV_F16 = 0, RV_KV_Q8 = 1 } rv_kv_format;
 
 /* A cache of n_seqs sequences in the caller's device memory (16-byte aligned
- * planes).  head_dim: a multiple of 8 up to 256.  One layer of an rv_attn
+ * planes, which may be NULL at capacity 0).  head_dim: a multiple of 8 up to 256.  One layer of an rv_attn
  * engine is such a cache: n_seqs 1, RV_KV_F16, the pointers of
  * rv_attn_cache. */
 typedef struct rv_kv_cache {

@@ -2659,6 +2659,7 @@ static int check_kv_cache(const char *what, const rv_kv_cache *c) {
   return RV_OK;
 }
 static int check_kv_planes(const char *what, const rv_kv_cache *c) {
+  if (c->capacity == 0) return RV_OK;  // no memory to point at
   if (!c->k || !c->v || (((uintptr_t)c->k | (uintptr_t)c->v) & 15))
     RV_FAIL(RV_ERR_INVALID_ARGUMENT, "%s: null cache plane or one not 16-byte aligned", what);
   if (c->format == RV_KV_Q8 &&
@@ -2861,9 +2862,9 @@ static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t 
   w.out_aligned = ((uintptr_t)a.out & 15) == 0;
   CUtensorMap m[4] = {};
   if (!Q8) {
-    const size_t cap = std::max<size_t>(a.cap, 1);
-    int rc = kv_plane_map(a.sk, a.n_seqs, cap, cap, a.n_kv, D, &m[2]);
-    if (rc == RV_OK) rc = kv_plane_map(a.sv, a.n_seqs, cap, cap, a.n_kv, D, &m[3]);
+    int rc = RV_OK;  // a cache without positions has no tiles to load
+    if (a.cap) rc = kv_plane_map(a.sk, a.n_seqs, a.cap, a.cap, a.n_kv, D, &m[2]);
+    if (rc == RV_OK && a.cap) rc = kv_plane_map(a.sv, a.n_seqs, a.cap, a.cap, a.n_kv, D, &m[3]);
     if (rc == RV_OK && a.prefix_len) rc = kv_plane_map(a.pk, 1, a.prefix_len, a.prefix_len, a.n_kv, D, &m[0]);
     if (rc == RV_OK && a.prefix_len) rc = kv_plane_map(a.pv, 1, a.prefix_len, a.prefix_len, a.n_kv, D, &m[1]);
     if (rc) return rc;

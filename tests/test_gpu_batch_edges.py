@@ -232,3 +232,25 @@ def test_sample_draws_many_from_one_row(rv):
     want = rv.sample(logits.expand(40, -1).contiguous(), u, top_k=k)
     assert torch.equal(tokens, want[0]) and torch.equal(logprobs, want[1])
     assert len(set(tokens.tolist())) > 1
+
+
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_Q8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+def test_a_suffix_without_room_leaves_the_prefix(rv, fmt, dtype, dim):
+    """A suffix cache of capacity 0 (tensors without memory): attention over the
+    prefix alone, as with an empty suffix; a length above 0 is reported."""
+    fmt = getattr(rv, fmt)
+    pre, one = caches(rv, 3, 1, 2, dim, 9000, fmt, 121)  # long enough for both to fill the GPU
+    none = rv.KvCache(3, 0, 2, dim, fmt)
+    q = randn(125, 3, 2, 8, dim).to(dtype)
+    zero = i32([0, 0, 0])
+    want = rv.prefix_attention(q, pre, 9000, one, zero)
+    assert torch.isfinite(want).all() and want.any()
+    assert torch.equal(rv.prefix_attention(q, pre, 9000, none, zero), want)
+    assert not rv.prefix_attention(q, None, 0, none, zero).any()
+    rv.device_status(0)
+    assert torch.equal(rv.prefix_attention(q, pre, 9000, none, i32([0, 1, 0])), want)
+    with pytest.raises(rv.KernelError) as e:
+        rv.device_status(0)
+    assert e.value.kind == "CapacityExceeded"
