@@ -29,6 +29,12 @@ struct PrefixArgs {
   float scale_log2;      // scale * log2(e)
 };
 
+// The power of two of a scale's size: f32 queries take it before they meet the
+// levels of 8-bit keys (exactly), so that large ones do not overflow there.
+RV_DEVFN float prefix_pow2(float scale) {
+  return __uint_as_float(max(__float_as_uint(scale) & 0x7F800000u, 0x00800000u));
+}
+
 // A sequence's suffix length, held inside its cache.
 RV_DEVFN int prefix_suffix_len(const PrefixArgs &a, uint32_t b) {
   const int n = a.lens[b];
@@ -54,6 +60,9 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
   const bool on = e < a.hd;
   float q[8] = {0, 0, 0, 0, 0, 0, 0, 0}, o[8] = {0, 0, 0, 0, 0, 0, 0, 0}, m = -INFINITY, l = 0;
   if (on) kv_load8((const T *)a.q + b * a.q_seq_stride + i * a.q_token_stride + (size_t)h * a.hd + e, false, q);
+  const float p2 = prefix_pow2(a.scale_log2), rest = a.scale_log2 / p2;
+#pragma unroll
+  for (int t = 0; t < 8; t++) q[t] *= p2;
   for (long long j = warp; j < total; j += 8) {
     const bool pre = j < a.prefix_len;
     const size_t at = (pre ? (size_t)j : (size_t)b * a.cap + (size_t)(j - a.prefix_len)) * a.n_kv + kvh;
@@ -79,7 +88,7 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
       s *= (pre ? a.pks : a.sks)[at];
       vs = (pre ? a.pvs : a.svs)[at];
     }
-    s *= a.scale_log2;
+    s *= rest;
     const float mn = fmaxf(m, s), c = m == mn ? 1.0f : exp2f(m - mn);
     // A score of -infinity adds nothing, and neither does it as the maximum.
     const float p = s == -INFINITY ? 0.0f : exp2f(s - mn);
@@ -926,6 +935,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         if (!ok) break;
         if (cur.at >= 0) {
           float *sc = s_scale + cur.at * RV_PFX_SCALE;
+          const float scale = PRECISE ? fabsf(a.scale_log2) / prefix_pow2(a.scale_log2) : fabsf(a.scale_log2);
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const int tok = ct + j * RV_PFX_CONV;
@@ -936,7 +946,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
             const float size = fabsf(cur.vs[j]);
             const bool fine = size < INFINITY;
             if (tok < RV_PFX_N) {
-              sc[tok] = fine ? cur.ks[j] * fabsf(a.scale_log2) : __uint_as_float(0x7FC00000u);
+              sc[tok] = fine ? cur.ks[j] * scale : __uint_as_float(0x7FC00000u);
               sc[RV_PFX_N + tok] = fine ? cur.vs[j] : 0.0f;
               sc[2 * RV_PFX_N + tok] = (float)max((int)(__float_as_uint(size) >> 23) - 126, -80);
             }
@@ -1031,8 +1041,9 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
       int seen = on ? p.keys : 0;  // keys of the segment that this row sees
       if (suffix && on) seen = min(max(p.keys - (int)a.n_q + 1 + w.by_g(r), 0), p.keys);
       // Scores times c are in units of log2 (8-bit keys: their scales hold
-      // the attention scale).  At least 2^-126, so that -infinity stays one.
-      float c = Q8 ? 1.0f : scale;
+      // the attention scale, for f32 queries but its power of two).  At least
+      // 2^-126, so that -infinity stays one.
+      float c = !Q8 ? scale : PRECISE ? prefix_pow2(scale) : 1.0f;
       if constexpr (PRECISE) {
         // The exponents of the stream's four warps: each arrives with its rows'.
         // A named barrier here would wait for ever on a warp that gave up.

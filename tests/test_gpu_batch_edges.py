@@ -254,3 +254,18 @@ def test_a_suffix_without_room_leaves_the_prefix(rv, fmt, dtype, dim):
     with pytest.raises(rv.KernelError) as e:
         rv.device_status(0)
     assert e.value.kind == "CapacityExceeded"
+
+
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("factor", [1e34, 1e36])
+def test_f32_queries_near_the_end_of_their_range_over_8_bit_rows(rv, dim, factor):
+    """The attention scale brings the scores back: products of queries and
+    levels must not overflow before it is applied."""
+    n, prefix, lens = 2, 300, [40, 7]
+    pre, suf = caches(rv, n, 40, 1, dim, prefix, rv.KV_Q8, 131)
+    q = randn(135, n, 1, 8, dim) * factor
+    scale = dim ** -0.5 / factor
+    got = rv.prefix_attention(q, pre, prefix, suf, i32(lens), scale=scale)
+    want, tol = attention_by_weight(q, pre, prefix, suf, lens, scale)
+    assert torch.isfinite(got).all()
+    assert ((got.double() - want).abs() <= tol).all()
