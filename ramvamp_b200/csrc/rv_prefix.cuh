@@ -497,7 +497,7 @@ RV_DEVFN void pfx_load_q(const PrefixArgs &a, const PfxWork &w, const PfxPiece &
 #pragma unroll
         for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(RV_FULL, m, o));
         // Both 2^e and 2^-e are normal floats.
-        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -100), 126);
+        const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 126);
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), sg = neg ? -down : down;
         if (row >= nr) continue;
         if (c == 0) up[row] = (int8_t)e;

@@ -269,3 +269,19 @@ def test_f32_queries_near_the_end_of_their_range_over_8_bit_rows(rv, dim, factor
     want, tol = attention_by_weight(q, pre, prefix, suf, lens, scale)
     assert torch.isfinite(got).all()
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_Q8"])
+@pytest.mark.parametrize("dim", [64, 128, 96])
+@pytest.mark.parametrize("factor", [1e-32, 1e-36])
+def test_f32_queries_near_the_small_end_of_their_range(rv, fmt, dim, factor):
+    """Queries below 2^-100 keep their bits: times a power of two they give what
+    ordinary ones do."""
+    n, prefix, lens = 2, 300, [40, 7]
+    pre, suf = caches(rv, n, 40, 1, dim, prefix, getattr(rv, fmt), 141)
+    q = randn(145, n, 1, 8, dim)
+    two = 2.0 ** round(math.log2(factor))
+    want = rv.prefix_attention(q, pre, prefix, suf, i32(lens), scale=dim ** -0.5)
+    got = rv.prefix_attention(q * two, pre, prefix, suf, i32(lens), scale=dim ** -0.5 / two)
+    # the same products, but for values of q * two below 2^-126 that lose bits
+    assert (got - want).abs().max() <= 2.0 ** -18 * want.abs().max()
