@@ -151,10 +151,14 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 // f32 queries are held to 2^-22 of their row's largest value as a sum of two
 // f16 (after scaling by a power of two), and so is P: products of f16 with the
 // f16 (or 8-bit) keys and values are exact, so the result carries f32's
-// rounding only (8 sequences over 4K positions: 6.6e-7 of the norm against 64
-// bits, f32 sums 1.6e-6; 42 over 21K: 5e-6 and 3e-6, as the tensor cores'
-// accumulator truncates); the price is twice the products, and for head_dim 128 query
-// tiles of 64 rows (two operands a stream in shared memory).  f16 queries round
+// rounding only.  The tensor cores' accumulator truncates, so O leaves it every
+// RV_PFX_RUN tiles and is summed up in the part, by f32 additions in memory that
+// nothing waits for (8 sequences over 4K positions: 6e-7 of the norm against 64
+// bits, f32 sums 1.6e-6; 1,024 tokens over 32K: 1.8e-6 and 3.5e-6, values of one sign
+// 3.3e-6 and 4.9e-6; in one accumulation these were 6e-5 and 2e-4.  Runs of 8
+// tiles: up to 7e-6, and 2 % faster on 128 sequences over 32K).  The price of f32 is
+// twice the products, and for head_dim 128 query tiles of 64 rows (two operands a
+// stream in shared memory).  f16 queries round
 // P to f16 once, the size of the output's own rounding (together 2.9e-4 of the
 // norm, where the output's alone is 2.1e-4): two terms there took 64 sequences
 // over an 8-bit 16K prompt from 58 to 65 us.  P is lifted by 2^7 and
@@ -173,6 +177,7 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 #define RV_PFX_N 128          // keys of a tile
 #define RV_PFX_OV 1           // a segment's fixed cost, in units
 #define RV_PFX_LAG 8.0f       // the reference maximum may lag by this (log2)
+#define RV_PFX_RUN 4          // tiles that an f32 row's O is summed over in tensor memory
 #define RV_PFX_LIFT 7.0f      // P is lifted by 2^7
 #define RV_PFX_SCALE_SLOTS 8  // tiles a stream whose token scales are in shared memory
 #define RV_PFX_SCALE (3 * RV_PFX_N)  // floats of a tile's scales: keys', values', the values' exponents
@@ -258,6 +263,7 @@ struct PfxCfg {
   static constexpr int QT = SR * D * 2;                         // bytes of one query operand
   static constexpr int QS = QT * (PRECISE ? 2 : 1);             // of a stream's
   static constexpr int TILE = RV_PFX_N * D * 2;                 // of a K or V tile
+  static constexpr bool RUNS = PRECISE;                         // O leaves tensor memory every RV_PFX_RUN tiles
   static constexpr int R = D == 64 ? (Q8 ? 6 : 8) : Q8 ? 3 : 5;  // K/V ring stages
   static constexpr int RAW = Q8 ? 2 * RV_PFX_N * D : 0;         // two tiles of levels on their way
   static constexpr int SCALES = Q8 ? 2 * RV_PFX_SCALE_SLOTS * RV_PFX_SCALE * 4 : 0;
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     tc_relinquish();
   }
   // Counters that run on over the plans (each role uses its own).
-  int n = 0, np[2] = {0, 0}, nq[2] = {0, 0}, unit = 0, piece = 0;
+  int n = 0, np[2] = {0, 0}, nq[2] = {0, 0}, unit = 0, piece = 0, run = 0;
   bool ok = true;
   PfxFeed feed{};
   for (int base = 0;; base += RV_PFX_TABLE) {
@@ -822,11 +828,11 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
                   if (kk < steps) {
                     const uint32_t pa = p0 + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * lo;
                     const uint64_t bd = mk(lbo_v | (vb + (uint32_t)kk * (2048 >> 4)), hi_sw);
-                    tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || c.j != 0 || lo != PRECISE);
+                    tc_mma_f16_ta(d, pa, bd, idesc_o, kk != 0 || (C::RUNS ? c.j % RV_PFX_RUN : c.j) != 0 || lo != PRECISE);
                   }
                 }
               }
-              if (!next) tc_commit(&o_full[s]);
+              if (!next || (C::RUNS && (c.j + 1) % RV_PFX_RUN == 0)) tc_commit(&o_full[s]);
               if (give) tc_commit(&kv_empty[nv % R]);
             }
             __syncwarp();
@@ -1000,19 +1006,21 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
     };
     int at = 0, left;
     pfx_entry(mytab, mycount, at, left);
-    // What the piece before leaves, written while this one's first scores are
-    // on their way.
+    // What the run before leaves, written while this one's first scores are on
+    // their way.
     int p_head = 0, p_part = -1, p_seen = 0;
-    bool p_on = false, p_warp = false;
-    float p_m = 0, p_l = 0;
+    bool p_on = false, p_warp = false, p_add = false;
+    float p_m = 0, p_l = 0, p_up = 0;
+    int t = 0;  // the piece's next tile
+    float m_ref = -INFINITY, m_part = -INFINITY, l = 0;  // m_part: the reference of what the part holds
 #pragma unroll 1
     while (ok && !pfx_failed(s_fail)) {
-      if (left) give_q(mytab[at], piece);
+      if (left && (!C::RUNS || t == 0)) give_q(mytab[at], piece);
       if (p_part >= 0) {
         const int rw = p_head & 1 ? w.rw_s : w.rw_p;
         const size_t part = (size_t)p_part + (pair ? s : 0);
         float4 *po = (p_head & 1 ? w.o_s : w.o_p) + part * (D / 4) * rw + row;
-        ok = pfx_wait(&o_full[s], (piece - 1) & 1);
+        ok = pfx_wait(&o_full[s], (run - 1) & 1);
         if (!ok) break;
         tc_fence_after();
         if (!Q8 && a.n_q > 1 && (p_head & 1) && p_seen > s_bad[2 * s + ((piece - 1) & 1)])
@@ -1025,9 +1033,18 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
             tc_ld_wait(tO + 16 * ch, v);
             if (p_on) {
 #pragma unroll
-              for (int j = 0; j < 4; j++)
-                po[(4 * ch + j) * rw] = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
-                                                    __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+              for (int j = 0; j < 4; j++) {
+                float4 x = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                       __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+                if constexpr (C::RUNS) x = make_float4(x.x * p_up, x.y * p_up, x.z * p_up, x.w * p_up);
+                float4 *const to = po + (4 * ch + j) * rw;
+                if (C::RUNS && p_add)
+                  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(x.x),
+                               "f"(x.y), "f"(x.z), "f"(x.w)
+                               : "memory");
+                else
+                  *to = x;
+              }
             }
           }
           tc_fence_before();
@@ -1052,8 +1069,9 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         if (on) c *= __uint_as_float((uint32_t)(s_up[(2 * s + (piece & 1)) * C::SR + row] + 127) << 23);
       }
       c = fmaxf(c, 0x1p-126f);
-      float m_ref = -INFINITY, l = 0.0f;
-      for (int t = 0; t < p.n; t++, unit++) {
+      const int t0 = C::RUNS ? t : 0, end = C::RUNS ? min(p.n, t0 + RV_PFX_RUN) : p.n;  // of the run
+      if (t0 == 0) m_ref = m_part = -INFINITY, l = 0;
+      for (t = t0; t < end; t++, unit++) {
         const int tile = p.tile0 + t, valid = min(RV_PFX_N, p.keys - tile * RV_PFX_N);
         const int lim = min(max(seen - tile * RV_PFX_N, 0), RV_PFX_N);
         const int slot = (pair ? 0 : s) * SLOTS + unit % SLOTS;
@@ -1118,7 +1136,7 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
               l *= f;
               const __half2 f2 = __float2half2_rn(f);
 #pragma unroll 1
-              for (int ch = t > 0 ? 0 : D / 16; ch < D / 16 + 4 * h; ch++) {
+              for (int ch = t > t0 ? 0 : D / 16; ch < D / 16 + 4 * h; ch++) {
                 uint32_t o[16];
                 const bool is_p = ch >= D / 16;  // P of the tile's first half
                 const uint32_t at = is_p ? tS + 16 * (ch - D / 16) : tO + 16 * ch;
@@ -1173,15 +1191,27 @@ __global__ void __launch_bounds__(RV_PFX_THREADS, 1)
         if (lane == 0) mbar_arrive(&p_ready[s]);
       }
       if (!ok) break;
-      // The products have read this piece's queries (S came after them), so the
-      // next piece's may take their place under the last P V.
+      if constexpr (C::RUNS) {
+        // The run's O goes to the part, times a power of two where the reference
+        // has moved since.  Past these limits what the part holds counts for
+        // nothing (below them O and l stay in range).
+        const float d = m_ref - m_part;
+        p_add = t0 > 0 && d <= (Q8 ? 48.0f : 80.0f);
+        p_up = p_add ? __uint_as_float((uint32_t)(127 + (int)d) << 23) : 1.0f;
+      }
+      if (!p_add) m_part = m_ref;
       p_head = p.head;
       p_part = p.part;
       p_on = on;
       p_seen = seen;
       p_warp = warp_on;
-      p_m = m_ref == -INFINITY ? -INFINITY : m_ref - RV_PFX_LIFT;
-      p_l = l;
+      p_m = m_part == -INFINITY ? -INFINITY : m_part - RV_PFX_LIFT;
+      p_l = C::RUNS ? l * p_up : l;
+      run++;
+      if (C::RUNS && t < p.n) continue;
+      // The products have read this piece's queries (S came after them), so the
+      // next piece's may take their place under the last P V.
+      t = 0;
       at++;
       pfx_entry(mytab, mycount, at, left);
       piece++;

@@ -285,3 +285,30 @@ def test_f32_queries_near_the_small_end_of_their_range(rv, fmt, dim, factor):
     got = rv.prefix_attention(q * two, pre, prefix, suf, i32(lens), scale=dim ** -0.5 / two)
     # the same products, but for values of q * two below 2^-126 that lose bits
     assert (got - want).abs().max() <= 2.0 ** -18 * want.abs().max()
+
+
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_Q8"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f32_sums_over_a_long_prompt(rv, fmt, dim):
+    """So many rows that a stream runs through hundreds of tiles of one segment,
+    values of one sign, weights nearly alike.  Within 512 keys the products are
+    summed by the tensor cores: 64 additions that lose less than 2^-23 of the sum
+    each, 2^-17; sums of these are f32 (at most 128 of them: 2^-17 at worst).  The
+    weights are off by 2 delta_j + 2^-19 as above."""
+    n, Q, H, prefix = 128, 16, 8, 32768
+    pre, suf = caches(rv, n, 16, 1, dim, prefix, getattr(rv, fmt), 151)
+    pre.v.abs_()
+    suf.v.abs_()
+    q = 0.02 * randn(155, n, Q, H, dim)
+    got = rv.prefix_attention(q, pre, prefix, suf, i32([Q] * n))
+    value = lambda x, s: x.double() if s is None else x.double() * s.double().unsqueeze(-1)  # noqa: E731
+    for b in (0, 77):
+        k = torch.cat([value(pre.k, pre.k_scale)[0], value(suf.k, suf.k_scale)[b]])[:, 0]
+        v = torch.cat([value(pre.v, pre.v_scale)[0], value(suf.v, suf.v_scale)[b]])[:, 0]
+        s = q[b].double() @ k.t() * dim ** -0.5
+        s.masked_fill_(torch.arange(len(k), device="cuda") > prefix + torch.arange(Q, device="cuda")[:, None, None], -math.inf)
+        p = torch.softmax(s, -1)
+        eps = 2 * 2.0 ** -20 * dim ** -0.5 * q[b].double().abs().amax(-1, keepdim=True) * k.abs().sum(-1) + 2.0 ** -19
+        want = p @ v  # all terms are positive: the sums of their sizes, too
+        tol = (p * eps) @ v + (p * eps).sum(-1, keepdim=True) * want + 2.0 ** -16 * want
+        assert ((got[b].double() - want).abs() <= tol).all()
