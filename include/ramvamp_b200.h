@@ -720,9 +720,12 @@ RV_API int rv_kv_read(const rv_kv_cache *cache, int dtype, size_t n, const int32
  * queries' own) counted.  Token i of sequence b sees the whole prefix and
  * suffix positions 0..lens[b]-n_q+i (none when that is negative); a row that
  * sees nothing is written as zeros.  Nothing outside what a row sees reaches
- * it, infinities and NaN included; in an f16 cache a value row of the n_q newest
- * tokens that is not finite makes the whole output row NaN for the queries that
- * see it.  q: device, dtype RV_F32 or RV_F16,
+ * it, infinities and NaN included; a NaN in the query, in a key that
+ * it sees or in a value that it sees does (a value's in its column; in an f16
+ * cache a value row of the n_q - 1 newest tokens that is not finite makes the
+ * whole output row NaN).  f32 queries are held to 2^-22 of their row's largest
+ * value and give sums of f32's accuracy; with f16 ones the softmax weights are
+ * rounded to f16 before they multiply the values.  q: device, dtype RV_F32 or RV_F16,
  * element (b, i, h, d) at b*q_seq_stride + i*q_token_stride + h*head_dim + d;
  * query head h reads kv head h / (n_heads / n_kv_heads); out: device,
  * [n_seqs][n_q][n_heads][head_dim] contiguous, the same dtype.  scratch:

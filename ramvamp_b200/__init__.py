@@ -888,8 +888,10 @@ def prefix_attention(q: torch.Tensor, prefix: Optional[KvCache], prefix_len: int
     contiguous) over positions 0..prefix_len-1 of `prefix`, shared by all
     sequences, and each sequence's own `lens` suffix positions (int32, on the
     device; the n_q query tokens are the newest of them and see no later one).
-    scale defaults to head_dim ** -0.5; scratch: a contiguous uint8 tensor of at
-    least ``prefix_attention_scratch`` bytes."""
+    f32 queries give sums of f32's accuracy; with f16 ones the softmax weights are
+    rounded to f16 before they multiply the values.  scale defaults to
+    head_dim ** -0.5; scratch: a contiguous uint8 tensor of at least
+    ``prefix_attention_scratch`` bytes."""
     if q.dim() != 4 or q.shape[0] != suffix.n_seqs or q.shape[3] != suffix.head_dim:
         raise KernelError(5, f"LengthMismatch: queries {tuple(q.shape)} for a suffix of {suffix.n_seqs} sequences, "
                              f"head_dim {suffix.head_dim}")

@@ -2765,7 +2765,8 @@ static void prefix_shape(size_t n_seqs, size_t n_q, size_t n_heads, size_t n_kv,
   w->tp = (int)((prefix_len + RV_PFX_N - 1) / RV_PFX_N);
   w->rows_s = (int)(n_q * G);
   w->rows_p = (int)(n_seqs * n_q * G);
-  // Paired: 58 against 72 us (64 sequences, 8 heads a kv head, 8-bit 16K prompt).
+  // Paired: 62 against 72 us (64 sequences, 8 heads a kv head, 8-bit 16K prompt); at
+  // 136 rows, the fewest of whole sequences of 8 heads, 39 against 45.
   w->pair = may_pair && w->rows_p > RV_PFX_M && prefix_len;
   w->sr_p = w->pair ? 2 * RV_PFX_M : (int)sr;
   w->sr_s = (int)sr;
@@ -2854,9 +2855,10 @@ static int prefix_tc_launch(const PrefixArgs &a, uint8_t *scratch, cudaStream_t 
   w.o_p = (float4 *)(scratch + o.o_p);
   w.o_s = (float4 *)(scratch + o.o_s);
   const size_t eb = sizeof(T);
-  // What a paired unit costs a CTA, in solo places (measured, f16 caches: 5.3
-  // and 2.5 thousand cycles; 8-bit caches, where the conversion of twice the
-  // tiles bounds solo streams: 4.3 and 7).
+  // What a paired unit costs a CTA, in solo places (measured at head_dim 128, f16
+  // caches: 5.3 and 2.5 thousand cycles; 8-bit caches, where the conversion of
+  // twice the tiles bounds solo streams: 4.3 and 7).  head_dim 64 uses the same
+  // and gains as much from pairs (77 against 94 us, 53 against 60).
   w.pair_cost = Q8 ? 1.3f : 2.0f;
   w.q_aligned = (((uintptr_t)a.q | a.q_seq_stride * eb | a.q_token_stride * eb) & 15) == 0;
   w.out_aligned = ((uintptr_t)a.out & 15) == 0;

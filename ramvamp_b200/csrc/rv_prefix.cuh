@@ -46,9 +46,9 @@ RV_DEVFN int prefix_suffix_len(const PrefixArgs &a, uint32_t b) {
 // query row, a warp per key in turn, head_dim spread over the lanes, so a
 // score is one warp sum.  The keys and values of the prefix are read once per
 // query row, not once per batch, and a key waits for the sum before it: bound by
-// that latency (head_dim 96, f16, 16 query and 4 kv heads: one sequence over
-// 1,024 positions 56 us, 64 over 8,192 1.17 ms; head_dim 128 through the tensor
-// cores 13 and 27 us).
+// that latency (head_dim 96, f16 rows, 16 query and 4 kv heads: one sequence over
+// 1,024 positions 55 us, 64 over 8,192 1.17 ms; head_dim 128 through the tensor
+// cores 13 and 27 us, f32 queries 14 and 42).
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
   __shared__ float s_m[8], s_l[8], s_o[8][256];
@@ -137,39 +137,51 @@ __global__ void __launch_bounds__(256) k_prefix_any(PrefixArgs a) {
 //   pair: more than 128 query rows of a kv head share the prefix (f16 queries):
 //   the streams take 128 rows each of a segment of 256 and read the same key
 //   and value tiles, halving the traffic per product.  The prefix then has a
-//   line of its own, over a share of the CTAs that follows the costs (128
-//   sequences over an f16 32K prompt 97 us, solo 112; 64 over an 8-bit 16K one
-//   58 and 72; with 128 rows or fewer there is no second stream to pair).
+//   line of its own, over a share of the CTAs that follows the costs (8 query
+//   heads a kv head; 128 sequences over an f16 32K prompt 98 us, solo 113, at
+//   head_dim 64 77 and 94; 64 over an 8-bit 16K one 62 and 72, at head_dim 64 53
+//   and 60; 17 sequences, 136 rows: 38 and 41, 8-bit 39 and 45; with 128 rows or
+//   fewer there is no second stream to pair).
 //
 // What bounds it: a unit is 2,048 cycles of products and as many of
 // exponentials (16 a cycle and SM), and a stream's chain S -> exponentials -> P
 // V -> next S takes about twice that, so two streams keep the tensor pipe 0.42
 // active at 128 sequences over 32K positions (its floor is 40 us; K and V are
-// read from memory once, 119 MB).  Small calls are bound by the fixed chain of
-// planning, loading Q, one unit, and the join: 12 us at one short sequence.
+// read from memory once, 119 MB).  Over an 8-bit cache the pipe is 0.20 active
+// and no memory or issue slot is full: a tile's conversion to f16 by three warps
+// stands in the chain before its products.  f32 queries: 278 us there, the pipe
+// 0.52 active with four times the products, and half the rows of each are empty
+// at head_dim 128.  Small calls are bound by the fixed chain of planning, loading
+// Q, one unit, and the join: 13 us at one short sequence.
 //
 // f32 queries are held to 2^-22 of their row's largest value as a sum of two
 // f16 (after scaling by a power of two), and so is P: products of f16 with the
 // f16 (or 8-bit) keys and values are exact, so the result carries f32's
 // rounding only.  The tensor cores' accumulator truncates, so O leaves it every
 // RV_PFX_RUN tiles and is summed up in the part, by f32 additions in memory that
-// nothing waits for (8 sequences over 4K positions: 6e-7 of the norm against 64
+// nothing waits for and that the row's own thread gives in order (8 sequences over 4K positions: 6e-7 of the norm against 64
 // bits, f32 sums 1.6e-6; 1,024 tokens over 32K: 1.8e-6 and 3.5e-6, values of one sign
 // 3.3e-6 and 4.9e-6; in one accumulation these were 6e-5 and 2e-4.  Runs of 8
 // tiles: up to 7e-6, and 2 % faster on 128 sequences over 32K).  The price of f32 is
 // twice the products, and for head_dim 128 query tiles of 64 rows (two operands a
-// stream in shared memory).  f16 queries round
-// P to f16 once, the size of the output's own rounding (together 2.9e-4 of the
-// norm, where the output's alone is 2.1e-4): two terms there took 64 sequences
-// over an 8-bit 16K prompt from 58 to 65 us.  P is lifted by 2^7 and
-// the reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
+// stream in shared memory).
+// f16 queries round P to f16 once, the size of the output's own rounding
+// (together 2.9e-4 of the norm, where the output's alone is 2.1e-4), and sum a
+// piece in one accumulation (values of one sign over 32K positions: 2.4e-4, the
+// output's rounding alone 1.8e-4).  P in two terms took 48 sequences' own tokens
+// from 36 to 40 us, 64 over an 8-bit 16K prompt from 62 to 72, 128 over 32K from
+// 98 to 123.  P is lifted by 2^7 and the reference maximum may lag by 2^8, so P stays below 2^15 and a weight is a
 // normal f16 down to 2^-21 of the largest.
 //
 // 8-bit cache: levels are exact in f16, so the products run on levels; a token's
-// key scale multiplies its score and its value scale its weight, both in f32.
+// key scale multiplies its score and its value scale its weight, both in f32
+// (f32 queries take the attention scale's power of two first, so that large ones
+// do not overflow against the levels).
 // P holds the value scale, so the reference is that of the products: with 2^e
 // above a token's value scale, the largest s + e of the keys that the row sees.
-// What a row does not see, or sees with next to no weight, does not move it.
+// What a row does not see, or sees with next to no weight, does not move it
+// (with one exponent a tile, for its largest value, it did, and 64 sequences took
+// 58 us for 62, f32 queries 155 for 162).
 #define RV_PFX_CTAS 148       // CTAs at most: one per SM of a B200
 #define RV_PFX_THREADS 384    // loads, products and conversion; two softmax warpgroups
 #define RV_PFX_CONV 96        // threads that turn 8-bit rows into f16 (warps 0, 2, 3)

@@ -27,10 +27,13 @@
 // 2^18) cannot overflow one.
 //
 // What bounds it: one row of 151,936 is a chain of cluster barriers and
-// reductions (13.8 us; its bytes are 0.1 us).  Many rows are bound by issue: a
-// token costs its comparisons, one exponential and the histograms' shared-memory
-// additions in each pass that weighs it (64 rows of 151,936, top-p: 69 us of GPU
-// time, 0.57 TB/s; 300 rows of 49,999, top-k 5,000 and top-p, 164 us).
+// reductions (13.8 us; its bytes are 0.1 us).  Many rows alternate passes that
+// issue -- a token costs its comparisons, one exponential and the histograms'
+// shared-memory additions in each pass that weighs it -- with barriers: issue
+// slots 0.45 to 0.51 used, the barrier the largest stall (64 rows of 151,936,
+// top-p: 68 us of GPU time, 0.57 TB/s; 300 rows of 49,999, top-k 5,000 and top-p,
+// 164 us).  Clusters also come in rounds: 37 of 8 CTAs or 74 of 4 at a time, so 64
+// rows take two and 300 take five, the last nearly empty.
 #pragma once
 #include "rv_internal.cuh"
 
