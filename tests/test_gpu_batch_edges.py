@@ -312,3 +312,15 @@ def test_f32_sums_over_a_long_prompt(rv, fmt, dim):
         want = p @ v  # all terms are positive: the sums of their sizes, too
         tol = (p * eps) @ v + (p * eps).sum(-1, keepdim=True) * want + 2.0 ** -16 * want
         assert ((got[b].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_Q8"])
+def test_f32_sums_over_a_long_prompt_repeat_bit_for_bit(rv, fmt):
+    """A row's runs are added in memory by one thread, in order."""
+    pre, suf = caches(rv, 128, 16, 1, 128, 32768, getattr(rv, fmt), 161)
+    q = randn(165, 128, 8, 8, 128)
+    lens = i32([8 + b % 9 for b in range(128)])
+    first = rv.prefix_attention(q, pre, 32768, suf, lens)
+    assert torch.isfinite(first).all()
+    for _ in range(10):
+        assert torch.equal(rv.prefix_attention(q, pre, 32768, suf, lens), first)
